@@ -6,6 +6,7 @@
 
 #include <atomic>
 
+#include "bindings.h"
 #include "fmb_api.h"
 
 
@@ -847,8 +848,11 @@ Tensor attn_bwd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
 
 }  // namespace
 
+void fmb_count_launches(int kernels) { g_launches.fetch_add(kernels, std::memory_order_relaxed); }
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "forgeminds_b200 native kernels (sm_100a)";
+  fmb_bind_rows(m);
   m.def("launch_count", &launch_count);
   m.def("gemm", &gemm);
   m.def("rmsnorm_fwd", &rmsnorm_fwd);

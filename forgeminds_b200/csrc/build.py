@@ -24,6 +24,9 @@ TARGET = PKG / "_C.so"
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--use_fast_math",
               "-DFMB_BUILD"]
+# Translation units whose results are held to fp32 accuracy (scores that are compared, statistics, losses): accurate
+# division, square root and expf; the fast forms are written out where a kernel means them.
+ACCURATE = ("distill", "layernorm", "rotary", "route")
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-Wno-attributes", "-DFMB_WITH_ATTENTION"]
 
 
@@ -77,7 +80,8 @@ def build(verbose: bool = False, force: bool = False, debug_bounds: bool = False
     for src in sorted(HERE.glob("*.cu")):
         checked = debug_bounds and src.stem in DEBUG_SOURCES
         stem = src.stem + (".dbg" if checked else "")
-        sig = _digest([src], hdr_sig)
+        flags = [f for f in NVCC_FLAGS if f != "--use_fast_math" or src.stem not in ACCURATE]
+        sig = _digest([src], hdr_sig + " ".join(flags))
         obj = OBJ / f"{stem}.{sig}.o"
         objects.append(obj)
         if obj.exists() and not force:
@@ -86,7 +90,7 @@ def build(verbose: bool = False, force: bool = False, debug_bounds: bool = False
             if checked or ".dbg." not in stale.name:
                 stale.unlink()
         extra = ["-DFMB_DEBUG_BOUNDS"] if checked else []
-        jobs.append(([_nvcc(), *NVCC_FLAGS, *extra, "-I", str(HERE), "-c", str(src), "-o", str(obj)],
+        jobs.append(([_nvcc(), *flags, *extra, "-I", str(HERE), "-c", str(src), "-o", str(obj)],
                      OBJ / f"{stem}.log"))
     torch_inc = [f"-I{p}" for p in ce.include_paths()]
     py_inc = f"-I{sysconfig.get_paths()['include']}"

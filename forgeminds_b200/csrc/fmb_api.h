@@ -53,6 +53,28 @@ int fmb_softmax_bwd(const void* y, const void* dy, void* dx, long long rows, int
 int fmb_topk(const void* x, void* values, long long* indices, long long rows, int n, int k, int dtype,
              cudaStream_t stream);
 
+// ---- LayerNorm (layernorm.cu)
+// y = (x - mean) * rstd * w + b over rows of d values, `ldx` elements apart; w and b may be null. With `delta` the norm is
+// that of x + delta as it is stored to xsum. stats [rows] float2 = (mean, rstd), may be null. y and xsum are contiguous.
+int fmb_layernorm_fwd(const void* x, long long ldx, const void* delta, long long ldd, const void* w, const void* b,
+                      void* xsum, void* y, float* stats, long long rows, int d, float eps, int dtype, int w_dtype,
+                      cudaStream_t stream);
+// dx (contiguous) = norm backward (+ dres); with `partial` ([nblocks, 2, d] fp32 scratch) dw and db (w_dtype, may be null)
+// receive the weight's and bias's gradients.
+int fmb_layernorm_bwd_blocks(long long rows, int d, int dtype);
+int fmb_layernorm_bwd(const void* dy, long long ldy, const void* x, long long ldx, const void* w, const float* stats,
+                      const void* dres, long long ldr, void* dx, float* partial, void* dw, void* db, long long rows, int d,
+                      int dtype, int w_dtype, int nblocks, cudaStream_t stream);
+
+// ---- rotary positions (rotary.cu)
+// src [batch, T, heads, D] by strides (elements; D contiguous), dst contiguous; heads may be 0
+typedef struct { const void* src; void* dst; long long sb, st, sh; int heads; } FmbRotaryTensor;
+// Rotates the first R values of every head by the angles of table row `position` (the token's place in its sequence, or
+// positions[b * pos_b + t], int32 or int64): negative leaves the head as it is, past the table gives NaN. sign -1: backward.
+int fmb_rotary(const FmbRotaryTensor* q, const FmbRotaryTensor* k, const float* cos, const float* sin, long long ldt,
+               long long table, const void* positions, int wide_positions, long long pos_b, long long batch, int T, int D,
+               int R, int interleaved, float sign, int dtype, cudaStream_t stream);
+
 // ---- losses (loss.cu)
 // In place: logits[rows, V] (bf16) become dlogits = (softmax - onehot) * grad_scale; per-row loss
 // (lse - logit[label], 0 for ignored rows) goes to row_loss.
@@ -62,6 +84,34 @@ int fmb_ce_fwd_bwd(void* logits, const long long* labels, float* row_loss, long 
 int fmb_kl_fwd_bwd(const void* student, const void* teacher, float* row_loss, void* grad, long long rows, int V,
                    float grad_scale, int dtype, int write_grad, cudaStream_t stream);
 int fmb_sum_f32(const float* x, float* out, long long n, float scale, int accumulate, cudaStream_t stream);
+
+// ---- distillation from a teacher's top logits (distill.cu)
+#define FMB_KL_MAX_KEEP 1024
+// Row losses, row statistics (float2: maximum, sum of exponentials) and, when given, the gradient for an upstream
+// gradient of 1 (rows `ldg` apart; may be the student itself). values / index [rows, K]; lse [rows] may be null. ws: two
+// ints of scratch, ws[0] receives the number of rows that count when `mean` and no `count` is given. loss (may be null):
+// the sum of the rows, divided by the count when `mean`.
+int fmb_kl_topk_fwd(const void* student, long long ld, const void* values, const long long* index, const float* lse,
+                    float* row_loss, float* stats, void* grad, long long ldg, const int* count, int* ws, float* loss,
+                    long long rows, int V, int K, float tau, int mean, int dtype, int t_dtype, cudaStream_t stream);
+// The gradient for `upstream` (one number, or one per row). skip_one: rows whose upstream is 1 are there already.
+int fmb_kl_topk_bwd(const void* student, long long ld, const void* values, const long long* index, const float* lse,
+                    const float* stats, void* grad, long long ldg, const int* count, const float* upstream,
+                    int upstream_rows, int skip_one, long long rows, int V, int K, float tau, int dtype, int t_dtype,
+                    cudaStream_t stream);
+
+// ---- routing to experts (route.cu)
+#define FMB_ROUTE_MAX_EXPERTS 512
+#define FMB_ROUTE_MAX_K 32
+// counts [E] is cleared and filled; partial ([blocks, E + 1] fp32) and aux are given together, or neither is.
+int fmb_route_blocks(long long tokens, int E);
+int fmb_route_fwd(const void* logits, long long ld, int dtype, const float* bias, float* weights, int* idx, int* counts,
+                  float* partial, float* aux, long long tokens, int E, int k, int softmax, int groups, int top_groups, int best,
+                  int renorm, float scale, float aux_coef, float z_coef, int blocks, cudaStream_t stream);
+// dweights [tokens, k] and daux (one number) may be null
+int fmb_route_bwd(const void* logits, long long ld, int dtype, const float* weights, const int* idx, const float* dweights,
+                  const float* daux, const int* counts, void* dlogits, long long tokens, int E, int k, int softmax, int renorm,
+                  float scale, float aux_coef, float z_coef, cudaStream_t stream);
 
 // ---- router (moe.cu)
 int fmb_router_blocks(long long rows);

@@ -1,0 +1,483 @@
+// LayerNorm of rows, forward (with the residual add in front of it when asked) and backward.
+//
+//   mean = sum x / d,  var = sum (x - mean)^2 / d,  r = 1 / sqrt(var + eps),  xh = (x - mean) r,  y = xh w + b
+//   g = dy w,  dx = r (g - sum g / d - xh sum (g xh) / d) (+ dres),  dw = sum over rows dy xh,  db = sum over rows dy
+//
+// Bound by HBM bandwidth: about ten operations per element. A row lives in the registers of the threads that
+// share it (16-byte chunks), so that mean and variance are two exact passes and memory is read once. Sums,
+// statistics and the weight's gradients are fp32.
+#include "fmb_api.h"
+#include "launch.cuh"
+#include "rows.cuh"
+
+namespace fmb {
+
+// How a thread of a row's TPR threads sees it: chunk i of N values. VEC: 16 contiguous bytes; otherwise N single
+// values TPR apart (widths, pitches or addresses that are no multiple of 16 bytes), still coalesced.
+template <typename T, int TPR, bool VEC> struct RowMap {
+  static constexpr int N = Vec16<T>::N;
+  static __device__ __forceinline__ int col(int i, int j, int t) {
+    return VEC ? (i * TPR + t) * N + j : (i * N + j) * TPR + t;
+  }
+  static __device__ __forceinline__ uint4 load(const T* row, int i, int t, int d) {
+    uint4 u = make_uint4(0, 0, 0, 0);
+    if constexpr (VEC) {
+      if (col(i, 0, t) < d) u = *reinterpret_cast<const uint4*>(row + col(i, 0, t));
+    } else if constexpr (sizeof(T) == 2) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int a = col(i, 2 * j, t), b = col(i, 2 * j + 1, t);
+        const uint32_t lo = a < d ? reinterpret_cast<const unsigned short*>(row)[a] : 0;
+        const uint32_t hi = b < d ? reinterpret_cast<const unsigned short*>(row)[b] : 0;
+        w[j] = lo | hi << 16;
+      }
+      u = make_uint4(w[0], w[1], w[2], w[3]);
+    } else {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = col(i, j, t) < d ? reinterpret_cast<const uint32_t*>(row)[col(i, j, t)] : 0;
+      u = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return u;
+  }
+  static __device__ __forceinline__ void store(T* row, const float (&f)[N], int i, int t, int d) {
+    if constexpr (VEC) {
+      if (col(i, 0, t) < d) *reinterpret_cast<uint4*>(row + col(i, 0, t)) = Vec16<T>::pack(f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (col(i, j, t) < d) row[col(i, j, t)] = from_f32<T>(f[j]);
+    }
+  }
+  template <typename WT> static __device__ __forceinline__ void weights(const WT* w, float (&f)[N], int i, int t, int d, float none) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) f[j] = none;
+    if (w == nullptr) return;
+    if constexpr (VEC) {
+      if (col(i, 0, t) < d) load_f32<WT, N>(w + col(i, 0, t), f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (col(i, j, t) < d) f[j] = to_f32(w[col(i, j, t)]);
+    }
+  }
+};
+
+// Sum over the TPR threads of a row of two values at once. `scratch`: two floats per warp, a buffer of its own for
+// each call until every thread has passed the next barrier (callers alternate between two).
+template <int TPR> __device__ __forceinline__ float2 row_sum2(float a, float b, float2* scratch) {
+  a = lanes_sum<32>(a);
+  b = lanes_sum<32>(b);
+  if constexpr (TPR > 32) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) scratch[warp] = make_float2(a, b);
+    __syncthreads();
+    constexpr int W = TPR / 32;
+    const int first = warp / W * W;
+    const float2 s = scratch[first + (threadIdx.x & 31) % W];
+    a = lanes_sum<(W < 32 ? W : 32)>(s.x);
+    b = lanes_sum<(W < 32 ? W : 32)>(s.y);
+  }
+  return make_float2(a, b);
+}
+template <int TPR> __device__ __forceinline__ float row_sum1(float a, float* scratch) {
+  a = lanes_sum<32>(a);
+  if constexpr (TPR > 32) {
+    const int warp = threadIdx.x >> 5;
+    if ((threadIdx.x & 31) == 0) scratch[warp] = a;
+    __syncthreads();
+    constexpr int W = TPR / 32;
+    a = lanes_sum<(W < 32 ? W : 32)>(scratch[warp / W * W + (threadIdx.x & 31) % W]);
+  }
+  return a;
+}
+
+// ------------------------------------------------------------------ forward
+template <typename T, typename WT, int TPR, int VPL, bool VEC, bool ADD>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+layernorm_fwd_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ delta, long long ldd,
+                     const WT* __restrict__ w, const WT* __restrict__ b, T* __restrict__ xsum, T* __restrict__ y,
+                     float2* __restrict__ stats, long long rows, int d, float inv_d, float eps) {
+  using M = RowMap<T, TPR, VEC>;
+  constexpr int N = M::N, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+  __shared__ float s_a[THREADS / 32], s_b[THREADS / 32];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int t = threadIdx.x % TPR;
+  const long long row = static_cast<long long>(blockIdx.x) * RPB + threadIdx.x / TPR;
+  const int width = row < rows ? d : 0;                   // threads without a row take part in the sums with nothing
+  const long long at = row < rows ? row : 0;
+  float v[VPL][N];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) Vec16<T>::unpack(M::load(x + at * ldx, i, t, width), v[i]);
+  if constexpr (ADD) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      float e[N];
+      Vec16<T>::unpack(M::load(delta + at * ldd, i, t, width), e);
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[i][j] = to_f32(from_f32<T>(v[i][j] + e[j]));     // the norm is that of the stored sum
+      M::store(xsum + at * d, v[i], i, t, width);
+    }
+  }
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) s += v[i][j];
+  const float mean = row_sum1<TPR>(s, s_a) * inv_d;
+  float q = 0.f;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      v[i][j] -= mean;
+      if (M::col(i, j, t) < width) q += v[i][j] * v[i][j];
+    }
+  const float r = rsqrtf(row_sum1<TPR>(q, s_b) * inv_d + eps);
+  if (width > 0 && t == 0 && stats != nullptr) stats[row] = make_float2(mean, r);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    float wv[N], bv[N];
+    M::weights(w, wv, i, t, width, 1.f);
+    M::weights(b, bv, i, t, width, 0.f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[i][j] = v[i][j] * r * wv[j] + bv[j];
+    M::store(y + at * d, v[i], i, t, width);
+  }
+}
+
+// Rows too wide for registers: one block per row, which is read again from the caches for the variance and the result.
+template <typename T, typename WT, bool ADD>
+__global__ void __launch_bounds__(1024)
+layernorm_fwd_wide_kernel(const T* __restrict__ x, long long ldx, const T* __restrict__ delta, long long ldd,
+                          const WT* __restrict__ w, const WT* __restrict__ b, T* __restrict__ xsum, T* __restrict__ y,
+                          float2* __restrict__ stats, int d, float inv_d, float eps) {
+  __shared__ float s_a[32], s_b[32];
+  const long long row = blockIdx.x;
+  const T* xr = x + row * ldx;
+  T* sr = ADD ? xsum + row * d : nullptr;
+  float s = 0.f;
+  for (int c = threadIdx.x; c < d; c += 1024) {
+    float v = to_f32(xr[c]);
+    if constexpr (ADD) {
+      const T sum = from_f32<T>(v + to_f32(delta[row * ldd + c]));
+      sr[c] = sum;                                        // read back below by the thread that wrote it
+      v = to_f32(sum);
+    }
+    s += v;
+  }
+  const float mean = row_sum1<1024>(s, s_a) * inv_d;
+  const T* vr = ADD ? sr : xr;
+  float q = 0.f;
+  for (int c = threadIdx.x; c < d; c += 1024) {
+    const float v = to_f32(vr[c]) - mean;
+    q += v * v;
+  }
+  const float r = rsqrtf(row_sum1<1024>(q, s_b) * inv_d + eps);
+  if (threadIdx.x == 0 && stats != nullptr) stats[row] = make_float2(mean, r);
+  for (int c = threadIdx.x; c < d; c += 1024)
+    y[row * d + c] = from_f32<T>((to_f32(vr[c]) - mean) * r * (w != nullptr ? to_f32(w[c]) : 1.f) + (b != nullptr ? to_f32(b[c]) : 0.f));
+}
+
+// ------------------------------------------------------------------ backward
+// Blocks walk over the rows. A thread keeps its columns' sums of dy xh and dy in registers; a block leaves them as
+// one row of `partial` [blocks, 2, d], which the column kernel below adds in a fixed order.
+template <typename T, typename WT, int TPR, int VPL, bool VEC>
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
+                     const WT* __restrict__ w, const float2* __restrict__ stats, const T* __restrict__ dres, long long ldr,
+                     T* __restrict__ dx, float* __restrict__ partial, long long rows, int d, float inv_d) {
+  using M = RowMap<T, TPR, VEC>;
+  constexpr int N = M::N, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+  __shared__ float2 scratch[2][THREADS / 32];
+  extern __shared__ float s_fold[];                       // [2, d], when several rows share a block
+  pdl_wait();
+  pdl_launch_dependents();
+  const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  float wv[VPL][N], dwa[VPL][N], dba[VPL][N];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    M::weights(w, wv[i], i, t, d, 1.f);
+#pragma unroll
+    for (int j = 0; j < N; ++j) { dwa[i][j] = 0.f; dba[i][j] = 0.f; }
+  }
+  int turn = 0;
+  for (long long base = static_cast<long long>(blockIdx.x) * RPB; base < rows; base += static_cast<long long>(gridDim.x) * RPB) {
+    const long long row = base + sub;
+    const int width = row < rows ? d : 0;
+    const long long at = row < rows ? row : 0;
+    const float2 st = stats[at];
+    uint4 rx[VPL], rg[VPL], rr[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      rg[i] = M::load(dy + at * ldy, i, t, width);
+      rx[i] = M::load(x + at * ldx, i, t, width);
+      if (dres != nullptr) rr[i] = M::load(dres + at * ldr, i, t, width);
+    }
+    float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      float g[N], xh[N];
+      Vec16<T>::unpack(rg[i], g);
+      Vec16<T>::unpack(rx[i], xh);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {                       // where there is no column dy is 0 and nothing is added
+        xh[j] = (xh[j] - st.x) * st.y;
+        dwa[i][j] += g[j] * xh[j];
+        dba[i][j] += g[j];
+        g[j] *= wv[i][j];
+        s1 += g[j];
+        s2 += g[j] * xh[j];
+      }
+    }
+    const float2 sums = row_sum2<TPR>(s1, s2, scratch[turn]);
+    turn ^= 1;
+    const float c1 = sums.x * inv_d, c2 = sums.y * inv_d;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+      float g[N], xh[N], o[N];
+      Vec16<T>::unpack(rg[i], g);
+      Vec16<T>::unpack(rx[i], xh);
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        xh[j] = (xh[j] - st.x) * st.y;
+        o[j] = st.y * (g[j] * wv[i][j] - c1 - xh[j] * c2);
+      }
+      if (dres != nullptr) {
+        float e[N];
+        Vec16<T>::unpack(rr[i], e);
+#pragma unroll
+        for (int j = 0; j < N; ++j) o[j] += e[j];
+      }
+      M::store(dx + at * d, o, i, t, width);
+    }
+  }
+  if (partial == nullptr) return;
+  float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * d;
+  if constexpr (RPB > 1) {
+    for (int who = 0; who < RPB; ++who) {                 // the block's row groups one after another: a fixed order
+      __syncthreads();
+      if (sub == who) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const int c = M::col(i, j, t);
+            if (c < d) {
+              s_fold[c] = (who ? s_fold[c] : 0.f) + dwa[i][j];
+              s_fold[d + c] = (who ? s_fold[d + c] : 0.f) + dba[i][j];
+            }
+          }
+      }
+    }
+    __syncthreads();
+    for (int c = threadIdx.x; c < 2 * d; c += THREADS) mine[c] = s_fold[c];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = M::col(i, j, t);
+        if (c < d) { mine[c] = dwa[i][j]; mine[d + c] = dba[i][j]; }
+      }
+  }
+}
+
+// Rows too wide for the accumulators: dx by one block per row, and the weight's gradients by blocks of 256 columns
+// that read dy and x once more (they need the rows' statistics only).
+template <typename T, typename WT>
+__global__ void __launch_bounds__(1024)
+layernorm_bwd_wide_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
+                          const WT* __restrict__ w, const float2* __restrict__ stats, const T* __restrict__ dres, long long ldr,
+                          T* __restrict__ dx, int d, float inv_d) {
+  __shared__ float2 scratch[32];
+  const long long row = blockIdx.x;
+  const float2 st = stats[row];
+  float s1 = 0.f, s2 = 0.f;
+  for (int c = threadIdx.x; c < d; c += 1024) {
+    const float g = to_f32(dy[row * ldy + c]) * (w != nullptr ? to_f32(w[c]) : 1.f);
+    s1 += g;
+    s2 += g * ((to_f32(x[row * ldx + c]) - st.x) * st.y);
+  }
+  const float2 sums = row_sum2<1024>(s1, s2, scratch);
+  const float c1 = sums.x * inv_d, c2 = sums.y * inv_d;
+  for (int c = threadIdx.x; c < d; c += 1024) {
+    const float g = to_f32(dy[row * ldy + c]) * (w != nullptr ? to_f32(w[c]) : 1.f);
+    float o = st.y * (g - c1 - (to_f32(x[row * ldx + c]) - st.x) * st.y * c2);
+    if (dres != nullptr) o += to_f32(dres[row * ldr + c]);
+    dx[row * d + c] = from_f32<T>(o);
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+layernorm_bwd_cols_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
+                          const float2* __restrict__ stats, float* __restrict__ partial, long long rows, int d) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= d) return;
+  float a = 0.f, b = 0.f;
+  for (long long row = blockIdx.y; row < rows; row += gridDim.y) {
+    const float2 st = stats[row];
+    const float g = to_f32(dy[row * ldy + c]);
+    a += g * ((to_f32(x[row * ldx + c]) - st.x) * st.y);
+    b += g;
+  }
+  float* mine = partial + static_cast<long long>(blockIdx.y) * 2 * d;
+  mine[c] = a;
+  mine[d + c] = b;
+}
+
+// Sums of the columns of partial [n, 2d] in a fixed order: 32 columns x 32 groups of rows per block.
+template <typename WT>
+__global__ void __launch_bounds__(1024)
+layernorm_cols_kernel(const float* __restrict__ partial, WT* __restrict__ dw, WT* __restrict__ db, int n, int d) {
+  __shared__ float red[32][33];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int c = blockIdx.x * 32 + threadIdx.x;
+  float s = 0.f;
+  if (c < 2 * d)
+    for (int r = threadIdx.y; r < n; r += 32) s += partial[static_cast<long long>(r) * 2 * d + c];
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  s = lanes_sum<32>(red[threadIdx.x][threadIdx.y]);       // warp y adds column y's 32 groups
+  const int out = blockIdx.x * 32 + threadIdx.y;
+  if (threadIdx.x == 0 && out < 2 * d) {
+    WT* to = out < d ? dw : db;
+    if (to != nullptr) to[out < d ? out : out - d] = from_f32<WT>(s);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+constexpr int FWD_CHUNKS = 2048;     // most chunks of a row that the forward kernel holds in registers (512 threads x 4)
+constexpr int BWD_CHUNKS = 1024;     // and the backward kernel (512 x 2)
+
+template <typename T, typename WT, bool VEC, bool ADD>
+cudaError_t fwd_launch(const T* x, long long ldx, const T* delta, long long ldd, const WT* w, const WT* b, T* xsum, T* y,
+                       float2* stats, long long rows, int d, float eps, cudaStream_t stream) {
+  const int chunks = (d + Vec16<T>::N - 1) / Vec16<T>::N;
+  const float inv_d = 1.f / static_cast<float>(d);
+#define FMB_LN_FWD(TPR, VPL)                                                                                            \
+  do {                                                                                                                  \
+    constexpr int RPB = TPR > 256 ? 1 : 256 / TPR;                                                                      \
+    return launch_pdl(layernorm_fwd_kernel<T, WT, TPR, VPL, VEC, ADD>, dim3(static_cast<unsigned>((rows + RPB - 1) / RPB)), \
+                      dim3(TPR > 256 ? TPR : 256), 0, stream, x, ldx, delta, ldd, w, b, xsum, y, stats, rows, d, inv_d, eps); \
+  } while (0)
+  if (chunks <= 32) FMB_LN_FWD(32, 1);
+  if (chunks <= 64) FMB_LN_FWD(32, 2);
+  if (chunks <= 128) FMB_LN_FWD(32, 4);
+  if (chunks <= 256) FMB_LN_FWD(128, 2);
+  if (chunks <= 512) FMB_LN_FWD(256, 2);
+  if (chunks <= 1024) FMB_LN_FWD(256, 4);
+  if (chunks <= FWD_CHUNKS) FMB_LN_FWD(512, 4);
+#undef FMB_LN_FWD
+  layernorm_fwd_wide_kernel<T, WT, ADD><<<static_cast<unsigned>(rows), 1024, 0, stream>>>(x, ldx, delta, ldd, w, b, xsum, y,
+                                                                                         stats, d, inv_d, eps);
+  return cudaGetLastError();
+}
+
+template <typename T, typename WT>
+int fwd_run(const void* x, long long ldx, const void* delta, long long ldd, const void* w, const void* b, void* xsum, void* y,
+            float* stats, long long rows, int d, float eps, cudaStream_t stream) {
+  constexpr int N = Vec16<T>::N;
+  const bool vec = d % N == 0 && ldx % N == 0 && ldd % N == 0 && aligned16(x) && aligned16(delta) && aligned16(w) &&
+                   aligned16(b) && aligned16(y) && aligned16(xsum);
+  const T *xp = static_cast<const T*>(x), *dp = static_cast<const T*>(delta);
+  const WT *wp = static_cast<const WT*>(w), *bp = static_cast<const WT*>(b);
+  T *sp = static_cast<T*>(xsum), *yp = static_cast<T*>(y);
+  float2* st = reinterpret_cast<float2*>(stats);
+  cudaError_t e;
+  if (delta != nullptr)
+    e = vec ? fwd_launch<T, WT, true, true>(xp, ldx, dp, ldd, wp, bp, sp, yp, st, rows, d, eps, stream)
+            : fwd_launch<T, WT, false, true>(xp, ldx, dp, ldd, wp, bp, sp, yp, st, rows, d, eps, stream);
+  else
+    e = vec ? fwd_launch<T, WT, true, false>(xp, ldx, dp, ldd, wp, bp, sp, yp, st, rows, d, eps, stream)
+            : fwd_launch<T, WT, false, false>(xp, ldx, dp, ldd, wp, bp, sp, yp, st, rows, d, eps, stream);
+  return e == cudaSuccess ? 0 : -3;
+}
+
+template <typename T, typename WT, bool VEC>
+cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, const WT* w, const float2* stats, const T* dres,
+                       long long ldr, T* dx, float* partial, long long rows, int d, int nblocks, cudaStream_t stream) {
+  const int chunks = (d + Vec16<T>::N - 1) / Vec16<T>::N;
+  const float inv_d = 1.f / static_cast<float>(d);
+#define FMB_LN_BWD(TPR, VPL)                                                                                             \
+  return launch_pdl(layernorm_bwd_kernel<T, WT, TPR, VPL, VEC>, dim3(nblocks), dim3(TPR > 256 ? TPR : 256),              \
+                    TPR < 256 && partial != nullptr ? 2 * d * sizeof(float) : 0, stream, dy, ldy, x, ldx, w, stats, dres, ldr, \
+                    dx, partial, rows, d, inv_d)
+  if (chunks <= 32) FMB_LN_BWD(32, 1);
+  if (chunks <= 64) FMB_LN_BWD(64, 1);
+  if (chunks <= 128) FMB_LN_BWD(128, 1);
+  if (chunks <= 256) FMB_LN_BWD(256, 1);
+  if (chunks <= 512) FMB_LN_BWD(512, 1);
+  if (chunks <= BWD_CHUNKS) FMB_LN_BWD(512, 2);
+#undef FMB_LN_BWD
+  layernorm_bwd_wide_kernel<T, WT><<<static_cast<unsigned>(rows), 1024, 0, stream>>>(dy, ldy, x, ldx, w, stats, dres, ldr, dx,
+                                                                                    d, inv_d);
+  if (partial != nullptr)
+    layernorm_bwd_cols_kernel<T><<<dim3((d + 255) / 256, nblocks), 256, 0, stream>>>(dy, ldy, x, ldx, stats, partial, rows, d);
+  return cudaGetLastError();
+}
+
+template <typename T, typename WT>
+int bwd_run(const void* dy, long long ldy, const void* x, long long ldx, const void* w, const float* stats, const void* dres,
+            long long ldr, void* dx, float* partial, void* dw, void* db, long long rows, int d, int nblocks,
+            cudaStream_t stream) {
+  constexpr int N = Vec16<T>::N;
+  const bool vec = d % N == 0 && ldx % N == 0 && ldy % N == 0 && ldr % N == 0 && aligned16(x) && aligned16(dy) &&
+                   aligned16(dres) && aligned16(w) && aligned16(dx);
+  const float2* st = reinterpret_cast<const float2*>(stats);
+  const T *gp = static_cast<const T*>(dy), *xp = static_cast<const T*>(x), *rp = static_cast<const T*>(dres);
+  const WT* wp = static_cast<const WT*>(w);
+  T* op = static_cast<T*>(dx);
+  cudaError_t e = vec ? bwd_launch<T, WT, true>(gp, ldy, xp, ldx, wp, st, rp, ldr, op, partial, rows, d, nblocks, stream)
+                      : bwd_launch<T, WT, false>(gp, ldy, xp, ldx, wp, st, rp, ldr, op, partial, rows, d, nblocks, stream);
+  if (e == cudaSuccess && partial != nullptr)
+    e = launch_pdl(layernorm_cols_kernel<WT>, dim3((2 * d + 31) / 32), dim3(32, 32), 0, stream, partial, static_cast<WT*>(dw),
+                   static_cast<WT*>(db), nblocks, d);
+  return e == cudaSuccess ? 0 : -3;
+}
+
+}  // namespace fmb
+
+using namespace fmb;
+
+extern "C" int fmb_layernorm_fwd(const void* x, long long ldx, const void* delta, long long ldd, const void* w, const void* b,
+                                 void* xsum, void* y, float* stats, long long rows, int d, float eps, int dtype, int w_dtype,
+                                 cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (d <= 0 || rows > 0x7fffffffLL) return -2;
+  if (dtype == FMB_BF16 && w_dtype == FMB_BF16)
+    return fwd_run<__nv_bfloat16, __nv_bfloat16>(x, ldx, delta, ldd, w, b, xsum, y, stats, rows, d, eps, stream);
+  if (dtype == FMB_BF16 && w_dtype == FMB_F32)
+    return fwd_run<__nv_bfloat16, float>(x, ldx, delta, ldd, w, b, xsum, y, stats, rows, d, eps, stream);
+  if (dtype == FMB_F32 && w_dtype == FMB_F32)
+    return fwd_run<float, float>(x, ldx, delta, ldd, w, b, xsum, y, stats, rows, d, eps, stream);
+  return -1;
+}
+
+extern "C" int fmb_layernorm_bwd_blocks(long long rows, int d, int dtype) {
+  const int n = dtype == FMB_BF16 ? 8 : 4;
+  const int chunks = (d + n - 1) / n;
+  if (chunks > BWD_CHUNKS) return static_cast<int>(rows < 32 ? (rows < 1 ? 1 : rows) : 32);
+  const int per_row = chunks <= 32 ? 32 : chunks <= 64 ? 64 : chunks <= 128 ? 128 : 256;
+  const long long need = (rows + 256 / per_row - 1) / (256 / per_row);
+  const long long most = static_cast<long long>(sm_count()) * (chunks <= 256 ? 4 : 2);
+  return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
+}
+
+extern "C" int fmb_layernorm_bwd(const void* dy, long long ldy, const void* x, long long ldx, const void* w, const float* stats,
+                                 const void* dres, long long ldr, void* dx, float* partial, void* dw, void* db, long long rows,
+                                 int d, int dtype, int w_dtype, int nblocks, cudaStream_t stream) {
+  if (rows <= 0) return 0;
+  if (d <= 0 || rows > 0x7fffffffLL || nblocks < 1) return -2;
+  if (dtype == FMB_BF16 && w_dtype == FMB_BF16)
+    return bwd_run<__nv_bfloat16, __nv_bfloat16>(dy, ldy, x, ldx, w, stats, dres, ldr, dx, partial, dw, db, rows, d, nblocks, stream);
+  if (dtype == FMB_BF16 && w_dtype == FMB_F32)
+    return bwd_run<__nv_bfloat16, float>(dy, ldy, x, ldx, w, stats, dres, ldr, dx, partial, dw, db, rows, d, nblocks, stream);
+  if (dtype == FMB_F32 && w_dtype == FMB_F32)
+    return bwd_run<float, float>(dy, ldy, x, ldx, w, stats, dres, ldr, dx, partial, dw, db, rows, d, nblocks, stream);
+  return -1;
+}

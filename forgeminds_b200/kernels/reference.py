@@ -113,3 +113,115 @@ def topk(x, k: int):
 
 def softmax(x):
     return torch.softmax(x, dim=-1)
+
+
+# ------------------------------------------------------------------------------ LayerNorm
+def layer_norm(x, w=None, b=None, eps: float = 1e-5):
+    xf = _wide(x)
+    centred = xf - xf.mean(dim=-1, keepdim=True)
+    y = centred * torch.rsqrt(centred.square().mean(dim=-1, keepdim=True) + eps)
+    if w is not None:
+        y = y * _wide(w)
+    if b is not None:
+        y = y + _wide(b)
+    return y.to(x.dtype)
+
+
+def add_layer_norm(x, delta, w=None, b=None, eps: float = 1e-5):
+    summed = x + delta
+    return summed, layer_norm(summed, w, b, eps)
+
+
+# ------------------------------------------------------------------------------ rotary positions
+def rotary(x, cos, sin, positions=None, interleaved: bool = False):
+    """Rotation of the first ``2 * cos.shape[-1]`` values of each head of ``x [B, T, H, D]`` by the angles of table row
+    ``position``: a negative position leaves the head as it is, one past the table gives NaN."""
+    T, R = x.shape[1], 2 * cos.shape[-1]
+    if positions is None:
+        c, s = cos[:T], sin[:T]
+    else:
+        at = positions.clamp(0, max(cos.shape[0] - 1, 0)).long()
+        stay, past = (positions < 0).unsqueeze(-1), (positions >= cos.shape[0]).unsqueeze(-1)
+        c = cos[at].masked_fill(stay, 1.0).masked_fill(past, float("nan"))
+        s = sin[at].masked_fill(stay, 0.0).masked_fill(past, float("nan"))
+    c, s = c.unsqueeze(-2), s.unsqueeze(-2)
+    xf = _wide(x)
+    a, b = (xf[..., 0:R:2], xf[..., 1:R:2]) if interleaved else (xf[..., : R // 2], xf[..., R // 2: R])
+    u, v = a * c - b * s, a * s + b * c
+    turned = torch.stack((u, v), dim=-1).flatten(-2) if interleaved else torch.cat((u, v), dim=-1)
+    return torch.cat((turned, xf[..., R:]), dim=-1).to(x.dtype)
+
+
+# ------------------------------------------------------------------------------ distillation from top logits
+def kl_topk_counts(values, index, vocab: int):
+    """Which slots count: an index inside the vocabulary and a teacher logit that is not ``-inf``."""
+    return (index >= 0) & (index < vocab) & (values != float("-inf"))
+
+
+def kl_topk(student, values, index, lse=None, temperature: float = 1.0):
+    """Per-row ``sum_k p_k (log p_k - log q[index_k])`` (fp32, or fp64 for fp64 logits) of 2-D inputs."""
+    held = kl_topk_counts(values, index, student.shape[-1])
+    has = held.any(dim=-1, keepdim=True)
+    z = (_wide(student) / temperature).masked_fill(~has, 0.0)
+    t = (values.to(z.dtype) / temperature).masked_fill(~held, float("-inf"))
+    if lse is None:
+        logp = torch.log_softmax(t.masked_fill(~has, 0.0), dim=-1)
+    else:
+        logp = t - lse.to(z.dtype).unsqueeze(-1)
+    p = logp.exp().masked_fill(~held, 0.0)
+    logq = torch.log_softmax(z, dim=-1).gather(-1, index.masked_fill(~held, 0))
+    return torch.where(held & (p != 0), p * (logp - logq), torch.zeros_like(p)).sum(dim=-1)
+
+
+# ------------------------------------------------------------------------------ routing to experts
+def route_experts(logits, k: int, softmax: bool = True, bias=None, groups: int = 1, top_groups: int = 1, best: int = 2,
+                  renorm: bool = True, scale: float = 1.0, aux_coef: float = 0.0, z_coef: float = 0.0):
+    """``(weights [N, k], idx int32 [N, k], counts int32 [E], aux or None)``. The choice is made in 64 bits: neighbours in
+    the order of scores may differ by less than 32 bits hold."""
+    N, E = logits.shape
+    with torch.no_grad():
+        z = logits.double()
+        if softmax:
+            pick = torch.softmax(z.masked_fill((z == float("-inf")).all(dim=-1, keepdim=True), 0.0), dim=-1)
+            pick = pick.masked_fill((z == float("-inf")).all(dim=-1, keepdim=True), 0.0)
+        else:
+            pick = torch.sigmoid(z)
+        pick = pick if bias is None else pick + bias.double()
+        order = z if bias is None else pick           # without a bias the logits have the scores' order
+        largest = lambda t: torch.nan_to_num(t, nan=float("inf"), posinf=float("inf"), neginf=float("-inf"))  # noqa: E731
+        order, pick = largest(order), largest(pick)
+        shut = torch.zeros_like(order, dtype=torch.bool)
+        if groups > 1:
+            each = pick.view(N, groups, -1)
+            score = largest(each.sort(dim=-1, descending=True).values[..., :best].sum(dim=-1))
+            out = score.sort(dim=-1, descending=True, stable=True).indices[:, top_groups:]
+            shut = torch.zeros_like(score, dtype=torch.bool).scatter_(-1, out, True)
+            shut = shut.unsqueeze(-1).expand_as(each).reshape(N, E)
+        rank = order.sort(dim=-1, descending=True, stable=True).indices
+        open_first = shut.gather(-1, rank).to(torch.uint8).sort(dim=-1, stable=True).indices      # shut ones to the end
+        idx = rank.gather(-1, open_first)[:, :k]
+        counts = torch.zeros(E, dtype=torch.int32, device=logits.device)
+        counts.scatter_add_(0, idx.reshape(-1), torch.ones(N * k, dtype=torch.int32, device=logits.device))
+    zf = _wide(logits)
+    dead = (zf == float("-inf")).all(dim=-1, keepdim=True)
+    zf = zf.masked_fill(dead, 0.0)
+    probs = torch.softmax(zf, dim=-1).masked_fill(dead, 0.0)
+    if renorm:      # shares of the chosen alone, from the logarithms of their scores: they may vanish in fp32 and still have shares
+        at = zf.gather(-1, idx)
+        logs = at if softmax else F.logsigmoid(at)
+        none = dead | (logs == float("-inf")).all(dim=-1, keepdim=True)
+        weights = torch.softmax(logs.masked_fill(none, 0.0), dim=-1).masked_fill(none, 0.0)
+    else:
+        weights = probs.gather(-1, idx) if softmax else torch.sigmoid(zf).masked_fill(dead, 0.0).gather(-1, idx)
+    aux = None
+    if aux_coef or z_coef:
+        share = probs
+        if not softmax:
+            scores = torch.sigmoid(zf).masked_fill(dead, 0.0)
+            total = scores.sum(dim=-1, keepdim=True)
+            share = scores / torch.where(total == 0, torch.ones_like(total), total)
+        load = counts.to(zf.dtype) / max(1, N * k)
+        lse = torch.logsumexp(zf, dim=-1).masked_fill(dead.squeeze(-1), 0.0)
+        n = max(1, N)
+        aux = aux_coef * E * (load * (share.sum(dim=0) / n)).sum() + z_coef * lse.square().sum() / n
+    return weights * scale, idx.to(torch.int32), counts, aux
