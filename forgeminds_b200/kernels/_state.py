@@ -14,6 +14,7 @@ _BACKEND = "auto"
 _COUNTS = {"fast": 0, "fallback": 0, "reason": {}}
 _FORCE_CUSTOM_OPS = False
 _DTYPES = (torch.float32, torch.bfloat16)
+_SERVED: set = set()         # devices that the kernels have been found to run on: asking again costs 4 us a call
 
 
 def _has_native() -> bool:
@@ -83,6 +84,7 @@ def fast_ok(*tensors) -> bool:
         return _miss("backend=fallback")
     if tracing():
         return False
+    device = None
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             continue
@@ -92,10 +94,16 @@ def fast_ok(*tensors) -> bool:
             return _miss("not cuda")
         if t.dtype not in _DTYPES:
             return _miss(f"dtype {t.dtype}")
+        device = t.get_device()
+    if device in _SERVED:
+        _COUNTS["fast"] += 1
+        return True
     from .. import ops
     if not ops.available():
         if _BACKEND == "native" or torch.cuda.is_available():
             ops.require()          # a GPU box without the extension is an error, not a fallback
         return _miss("no native extension")
+    if device is not None and torch.cuda.get_device_capability(device)[0] == 10:
+        _SERVED.add(device)
     _COUNTS["fast"] += 1
     return True

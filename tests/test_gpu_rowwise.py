@@ -487,7 +487,7 @@ def test_route_strides_and_no_tokens():
         check_route(z, 5, "sigmoid", 0.01 * randn(64, seed=85))
     z = torch.empty(0, 16, device="cuda", requires_grad=True)
     w, idx, counts, aux = K().route_experts(z, 3, aux_coef=0.1)
-    assert w.shape == (0, 3) and idx.shape == (0, 3) and not counts.any() and float(aux) == 0.0
+    assert w.shape == (0, 3) and idx.shape == (0, 3) and not counts.any() and float(aux.detach()) == 0.0
     assert torch.autograd.grad(w.sum(), z)[0].shape == (0, 16)
 
 
