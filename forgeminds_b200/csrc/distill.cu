@@ -10,6 +10,7 @@
 // 2^x of the special function unit (relative error 2^-22) with the argument folded into one multiply-add.
 #include "fmb_api.h"
 #include "launch.cuh"
+#include "ptx_sm100.cuh"
 #include "rows.cuh"
 
 namespace fmb {
@@ -55,6 +56,7 @@ struct KlParams {
   long long ldg;
   const int* count;                // rows that count (mean), or null
   int* ticket;                     // 0 before the launch; the block that makes it `blocks` adds the rows' losses
+  int* taken;                      // 0 before the launch: rows that have been given out
   float* loss;                     // the sum (mean) of row_loss, or null
   const float* upstream;           // backward: gradient of the loss, one number or one per row
   int upstream_rows, skip_one;     // skip_one: the gradient is there already for an upstream of 1
@@ -252,13 +254,385 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
   }
 }
 
+// ------------------------------------------------------------------ rows that stay in shared memory
+// A row is split over the CTAs of a cluster, at most 64 KB for each so that three of them share an SM: the logits are read
+// from memory once, and maximum, sum and gradient are taken from there. A thread keeps to its own 16-byte vectors, and as
+// soon as the gradient has used one, the same place receives the next row's: loads, exponentials and stores of the SM's
+// CTAs overlap. Few threads per row (256), because the reductions and the row's bookkeeping cost each warp as much as some
+// fifty vectors do. Kept logit k belongs to thread k, whose maximum and sums join the row's own reductions. The CTAs of a
+// row exchange (maximum, sum around it, loss) once. Rows are given out one by one: clusters that find no place at first,
+// while an earlier kernel still holds some SMs, would otherwise be a second wave.
+// Measured, with gradient, bf16: 8192 x 32000 in 204 us (5.1 TB/s of logits and gradient; one block per row that reads it
+// twice: 386), 4096 x 128259 over four CTAs in 472 us (4.5 TB/s; 758): there a row's CTAs wait for one another for a fifth
+// of the time. Both exponentials of a logit together hold the special function unit for 60 % of it.
+struct KlPart {
+  float m, s, a;                                           // maximum, sum of exponentials around it, sum e (log e - x / tau)
+};
+
+// A row of V values: `head` of them before the first 16-byte boundary, then nv whole vectors, then the rest. The up to
+// 2 N - 2 values outside the vectors are held singly by the first threads of the row's first CTA.
+template <typename T> struct KlRow {
+  static constexpr int N = Vec16<T>::N;
+  const T* at;
+  int head, nv;
+  __device__ __forceinline__ KlRow(const T* p, int V) : at(p), head(head_of(p, V)) { nv = (V - head) / N; }
+  __device__ __forceinline__ const uint4* vectors() const { return reinterpret_cast<const uint4*>(at + head); }
+  __device__ __forceinline__ int single(int t) const { return t < head ? t : nv * N + t; }       // of thread t
+};
+
+// two fp32 values in one register pair, and the instructions that take both at once
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 f2_parts(F2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+__device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+
+constexpr int KL_ROW_THREADS = 256;
+constexpr int KL_ROW_BYTES = 64 * 1024;                    // most of a row in one CTA
+constexpr int KL_MARKS = 1024;                             // words of the marks by which an index that stands twice is found
+
+template <typename T, typename TT>
+__global__ void __launch_bounds__(KL_ROW_THREADS, 3)
+kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
+  constexpr int N = Vec16<T>::N, H = N / 2, THREADS = KL_ROW_THREADS, WARPS = THREADS / 32;
+  extern __shared__ uint4 s_row[];                         // [per_cta]: this CTA's part of the row
+  __shared__ unsigned s_marks[KL_MARKS];
+  __shared__ int s_at[THREADS];
+  __shared__ float s_e[THREADS];
+  __shared__ KlPart s_part[2][8];
+  __shared__ float2 s_max[WARPS];
+  __shared__ float3 s_sum[WARPS];
+  __shared__ float scratch[32], s_single[2 * N];
+  __shared__ int s_last;
+  __shared__ int2 s_given[2];                              // rows that this CTA is told
+  for (int i = threadIdx.x; i < KL_MARKS; i += THREADS) s_marks[i] = 0;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
+  // tells a row (two at the start) to all CTAs of this one's cluster; they see it behind the next barrier
+  auto give = [&](int which, int a, int b) {
+    for (int i = 0; i < split; ++i) {
+      if (split > 1) {
+        const uint32_t to = mapa_shared(smem_u32(&s_given[which]), i);
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to), "r"(a) : "memory");
+        asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(to + 4), "r"(b) : "memory");
+      } else {
+        s_given[which] = make_int2(a, b);
+      }
+    }
+  };
+  const float c = LOG2E / p.tau, inv_tau = 1.f / p.tau;
+  const float scale = (p.count != nullptr ? 1.f / static_cast<float>(max(*p.count, 1)) : 1.f) * inv_tau;
+  const int first = rank * per_cta;                        // this CTA's first vector
+  const bool slot = threadIdx.x < p.K;
+  const F2 c2 = f2(c, c);
+  float single = -CUDART_INF_F;
+  // vectors of this CTA in a row
+  auto held = [&](const KlRow<T>& r) { return min(per_cta, r.nv - first); };
+  const uint32_t s_mine = smem_u32(s_row);
+  auto fetch = [&](const uint4* from, int i) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(s_mine + i * 16), "l"(from + i) : "memory");
+  };
+  auto load_single = [&](const KlRow<T>& r) {
+    return rank == 0 && static_cast<int>(threadIdx.x) < p.V - r.nv * N ? to_f32(r.at[r.single(threadIdx.x)]) : -CUDART_INF_F;
+  };
+  // This thread's kept logit. The loads for the next row are issued a row ahead and looked at when that row begins: a
+  // comparison where they are issued would hold the CTA up for their 2800 cycles.
+  long long slot_index = -1;
+  TT slot_value = from_f32<TT>(0.f);
+  float lse = 0.f;
+  auto load_slot = [&](long long r) {
+    slot_index = -1;
+    if (p.lse != nullptr && r < p.rows) lse = p.lse[r];
+    if (slot && r < p.rows) {
+      slot_index = p.index[r * p.K + threadIdx.x];
+      slot_value = static_cast<const TT*>(p.values)[r * p.K + threadIdx.x];
+    }
+  };
+  if (split > 1) cluster_sync_all();                       // every CTA of the row runs before one writes to another
+  if (rank == 0 && threadIdx.x == 0) {
+    const int first_row = atomicAdd(p.taken, 2);
+    give(0, first_row, first_row + 1);
+  }
+  if (split > 1) cluster_sync_all();
+  else __syncthreads();
+  long long row = s_given[0].x, next = s_given[0].y;
+  if (row < p.rows) {
+    const KlRow<T> r(static_cast<const T*>(p.student) + row * p.ld, p.V);
+    const int n = held(r);
+    for (int i = threadIdx.x; i < n; i += THREADS) fetch(r.vectors() + first, i);
+    single = load_single(r);
+    load_slot(row);
+  }
+  int side = 0;
+  while (row < p.rows) {
+    side ^= 1;
+    int after = 0;                                         // the row after the next one
+    if (rank == 0 && threadIdx.x == 0 && next < p.rows) after = atomicAdd(p.taken, 1);
+    const KlRow<T> r(static_cast<const T*>(p.student) + row * p.ld, p.V);
+    const int n = held(r);
+    const int at = slot_counts(slot_index, slot_value, p.V) ? static_cast<int>(slot_index) : -1;
+    const float t = at >= 0 ? to_f32(slot_value) * inv_tau : -CUDART_INF_F;
+    asm volatile("cp.async.wait_all;" ::: "memory");       // its own copies: other threads read them behind a barrier
+    // maxima of this CTA's part and of the teacher's logits
+    float m = single;
+    if constexpr (sizeof(T) == 2) {
+      uint32_t top = 0xff80ff80u;                          // -inf
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        const uint4 x = s_row[i];
+        top = max_bf16x2(max_bf16x2(max_bf16x2(top, x.x), max_bf16x2(x.y, x.z)), x.w);
+      }
+      m = fmaxf(m, fmaxf(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u)));
+    } else {
+#pragma unroll 4
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        float f[N];
+        Vec16<T>::unpack(s_row[i], f);
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = fmaxf(m, f[j]);
+      }
+    }
+    m = lanes_max<32>(m);
+    float ref = lanes_max<32>(t);
+    if (lane == 0) s_max[warp] = make_float2(m, ref);
+    if (threadIdx.x < 2 * N) s_single[threadIdx.x] = single;
+    const bool some = __syncthreads_or(at >= 0);
+    {
+      const float2 o = s_max[lane % WARPS];
+      m = lanes_max<WARPS>(o.x);
+      ref = lanes_max<WARPS>(o.y);
+    }
+    if (p.lse != nullptr) ref = lse;
+    else if (ref == -CUDART_INF_F) ref = 0.f;              // nothing counts, or NaN alone
+    const KlRow<T> rn(static_cast<const T*>(p.student) + next * p.ld, p.V);
+    const int nn = next < p.rows ? held(rn) : 0;
+    float next_single = next < p.rows ? load_single(rn) : -CUDART_INF_F;
+    load_slot(next);
+    // sums: exponentials of the student, e = exp(t - ref) of the teacher, and e (t - ref - x / tau) where x is held here
+    const float mc = m == -CUDART_INF_F ? 0.f : m * c;
+    F2 sums = 0;
+    {
+      const F2 mc2 = f2(-mc, -mc);
+      F2 more = 0;
+#pragma unroll 2
+      for (int i = threadIdx.x; i < n; i += THREADS) {
+        float f[N];
+        Vec16<T>::unpack(s_row[i], f);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          const float2 o = f2_parts(f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, mc2));
+          if (j % 2) more = f2_add(more, f2(exp2_unit(o.x), exp2_unit(o.y)));
+          else sums = f2_add(sums, f2(exp2_unit(o.x), exp2_unit(o.y)));
+        }
+      }
+      sums = f2_add(sums, more);
+    }
+    float s = f2_parts(sums).x + f2_parts(sums).y + exp2_unit(fmaf(single, c, -mc)), e = 0.f, a = 0.f, xk = 0.f;
+    bool mine = false, twice = false;                      // whether the student's logit at the index is held here
+    int mark = -1;
+    if (at >= 0) {
+      const int v = at - r.head, w = v - first * N;
+      if (v < 0 || v >= r.nv * N) {
+        mine = rank == 0;
+        xk = s_single[v < 0 ? at : at - r.nv * N];
+      } else if (w >= 0 && w < per_cta * N) {
+        mine = true;
+        xk = to_f32(reinterpret_cast<const T*>(s_row)[w]);
+      }
+      e = expf(t - ref);
+      if (mine && !(e == 0.f)) a = e * (t - ref - xk * inv_tau);
+      // a mark that is set already: an index that stands twice, or in a few rows of a hundred two that share a mark
+      const unsigned h = static_cast<unsigned>(at) * 2654435761u >> 17;
+      mark = h >> 5;
+      twice = atomicOr(s_marks + mark, 1u << (h & 31)) >> (h & 31) & 1;
+    }
+    if (slot) {
+      s_at[threadIdx.x] = at;
+      s_e[threadIdx.x] = e;
+    }
+    s = lanes_sum<32>(s);
+    float mass = lanes_sum<32>(e);
+    a = lanes_sum<32>(a);
+    if (lane == 0) s_sum[warp] = make_float3(s, mass, a);
+    if (rank == 0 && threadIdx.x == 0) give(side, next < p.rows ? after : static_cast<int>(p.rows), 0);
+    twice = __syncthreads_or(twice);                       // also: every logit at an index has been taken from the row's copy
+    if (mark >= 0) s_marks[mark] = 0;                      // the next row's first mark is behind another barrier
+    {
+      const float3 o = s_sum[lane % WARPS];
+      s = lanes_sum<WARPS>(o.x);
+      mass = lanes_sum<WARPS>(o.y);
+      a = lanes_sum<WARPS>(o.z);
+    }
+    if (split > 1) {
+      if (threadIdx.x < split) {                           // a copy of this CTA's part for each of the row's CTAs
+        const uint32_t to = mapa_shared(smem_u32(&s_part[side][rank]), threadIdx.x);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(m) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(s) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a) : "memory");
+      }
+      cluster_sync_all();
+      m = s_part[side][0].m;
+      for (int i = 1; i < split; ++i) m = fmaxf(m, s_part[side][i].m);
+      s = a = 0.f;
+      for (int i = 0; i < split; ++i) {
+        const KlPart o = s_part[side][i];
+        s += o.m == -CUDART_INF_F ? o.s : o.s * exp2_unit((o.m - m) * c);
+        a += o.a;
+      }
+    }
+    // p = e / sum e, or e itself beside the teacher's own normaliser
+    const float norm = p.lse != nullptr || !some ? 1.f : __fdividef(1.f, mass);
+    const float whole = p.lse != nullptr ? mass : 1.f;     // sum p
+    if (rank == 0 && threadIdx.x == 0) {
+      p.row_loss[row] = some ? a * norm - (p.lse != nullptr ? 0.f : logf(mass)) + whole * (m * inv_tau + logf(s)) : 0.f;
+      p.stats[row] = make_float2(m, s);
+    }
+    const uint4* from = rn.vectors() + first;
+    if (p.grad == nullptr) {
+      for (int i = threadIdx.x; i < nn; i += THREADS) fetch(from, i);
+    } else {
+      const float share = __fdividef(whole, s), gmc = m * c;
+      T* gr = static_cast<T*>(p.grad) + row * p.ldg;
+      T* to = gr + r.head + first * N;
+      const bool wide = ((reinterpret_cast<uintptr_t>(r.at) ^ reinterpret_cast<uintptr_t>(gr)) & 15) == 0;
+      if (rank == 0 && static_cast<int>(threadIdx.x) < p.V - r.nv * N)
+        gr[r.single(threadIdx.x)] = from_f32<T>(some ? exp2_unit(fmaf(single, c, -gmc)) * (share * scale) : 0.f);
+      if (wide && some) {
+        const F2 gmc2 = f2(-gmc, -gmc), by2 = f2(share * scale, share * scale);
+#pragma unroll 2
+        for (int i = threadIdx.x; i < n; i += THREADS) {
+          float f[N];
+          Vec16<T>::unpack(s_row[i], f);
+#pragma unroll
+          for (int j = 0; j < H; ++j) {
+            float2 o = f2_parts(f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, gmc2));
+            o = f2_parts(f2_mul(f2(exp2_unit(o.x), exp2_unit(o.y)), by2));
+            f[2 * j] = o.x;
+            f[2 * j + 1] = o.y;
+          }
+          reinterpret_cast<uint4*>(to)[i] = Vec16<T>::pack(f);
+          if (i < nn) fetch(from, i);                      // the vector has been used: its place is free
+        }
+      } else {                                             // a row without slots that count, or rows that lie differently in
+        for (int i = threadIdx.x; i < n; i += THREADS) {   // the gradient: single values
+          float f[N];
+          Vec16<T>::unpack(s_row[i], f);
+#pragma unroll
+          for (int j = 0; j < N; ++j) to[i * N + j] = from_f32<T>(some ? exp2_unit(fmaf(f[j], c, -gmc)) * (share * scale) : 0.f);
+          if (i < nn) fetch(from, i);
+        }
+      }
+      // a row of odd length may have one vector more than the one before it
+      for (int i = threadIdx.x + (n > static_cast<int>(threadIdx.x) ? (n - threadIdx.x + THREADS - 1) / THREADS * THREADS : 0); i < nn; i += THREADS)
+        fetch(from, i);
+      if (some) {
+        __syncthreads();                                   // the kept logits' own part goes over what has just been written
+        if (mine) {
+          float want = e;
+          if (twice) {                                     // each of its slots writes the same sum, taken in slot order
+            want = 0.f;
+            for (int j = 0; j < p.K; ++j) want += s_at[j] == at ? s_e[j] : 0.f;
+          }
+          gr[at] = from_f32<T>((exp2_unit(fmaf(xk, c, -gmc)) * share - want * norm) * scale);
+        }
+      }
+    }
+    single = next_single;
+    row = next;
+    next = s_given[side].x;
+  }
+  if (p.loss != nullptr) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) s_last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
+    __syncthreads();
+    if (s_last) {                                          // the last CTA adds the rows in a fixed order
+      __threadfence();
+      float v = 0.f;
+      for (long long i = threadIdx.x; i < p.rows; i += THREADS) v += __ldcg(p.row_loss + i);
+      v = block_sum(v, scratch);
+      if (threadIdx.x == 0) *p.loss = p.count != nullptr ? v / static_cast<float>(max(*p.count, 1)) : v;
+    }
+  }
+}
+
+// Clusters of `split` CTAs with `smem` bytes each that the device holds together; 0 where the kernel does not run. (A second
+// wave of a walk over all rows would double its time: of 74 clusters of 4 that 148 SMs have room for by numbers, 71 fit.)
+template <typename T, typename TT> int kl_fit(int split, size_t smem) {
+  auto kernel = kl_topk_row_kernel<T, TT>;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(sm_count() / split * split);
+  cfg.blockDim = dim3(KL_ROW_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int got = 0;
+  if (cudaOccupancyMaxActiveClusters(&got, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return got;
+}
+
+template <typename T, typename TT> int kl_row_launch(const KlParams& p, int split, int per_cta, cudaStream_t stream) {
+  auto kernel = kl_topk_row_kernel<T, TT>;
+  static bool opted[64] = {};
+  int dev = 0;
+  const size_t smem = sizeof(uint4) * per_cta;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
+  if (!opted[dev]) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KL_ROW_BYTES) != cudaSuccess) return -3;
+    opted[dev] = true;
+  }
+  const long long fit = kl_fit<T, TT>(split, smem);
+  if (fit < 1) return -3;
+  const long long groups = p.rows < fit ? p.rows : fit;
+  const dim3 grid(static_cast<unsigned>(groups * split));
+  const cudaError_t e = split == 1 ? launch_pdl(kernel, grid, dim3(KL_ROW_THREADS), smem, stream, p, split, per_cta)
+                                   : launch_pdl_cluster(kernel, grid, dim3(KL_ROW_THREADS), smem, split, stream, p, split, per_cta);
+  return e == cudaSuccess ? 0 : -3;
+}
+
 template <typename T, typename TT>
 int kl_run(KlParams p, bool fwd, int* ws, bool mean, const int* count, cudaStream_t stream) {
   const size_t smem = static_cast<size_t>(p.K) * 16;
   cudaError_t e = cudaSuccess;
   if (fwd) {
-    if (cudaMemsetAsync(ws, 0, 2 * sizeof(int), stream) != cudaSuccess) return -3;
+    if (cudaMemsetAsync(ws, 0, 3 * sizeof(int), stream) != cudaSuccess) return -3;
     p.ticket = ws + 1;
+    p.taken = ws + 2;
   }
   if (mean) {
     if (count == nullptr) {
@@ -271,6 +645,16 @@ int kl_run(KlParams p, bool fwd, int* ws, bool mean, const int* count, cudaStrea
       }
     }
     p.count = count;
+  }
+  if (fwd) {
+    // the fewest CTAs (1, 2, 4 or 8) that hold a row, more while SMs would be left without one
+    constexpr int N = Vec16<T>::N, MOST = KL_ROW_BYTES / 16;
+    const int vectors = p.V / N > 0 ? p.V / N : 1;
+    int split = 1;
+    while (split < 8 && (vectors + split - 1) / split > MOST) split *= 2;
+    while (split < 8 && p.rows * split < sm_count() && vectors / split > 4 * KL_ROW_THREADS) split *= 2;
+    if (p.K <= KL_ROW_THREADS && (vectors + split - 1) / split <= MOST)
+      return kl_row_launch<T, TT>(p, split, (vectors + split - 1) / split, stream);
   }
   const long long blocks = p.rows < 4LL * sm_count() ? p.rows : 4LL * sm_count();
   e = fwd ? launch_pdl(kl_topk_kernel<T, TT, true>, dim3(static_cast<unsigned>(blocks)), dim3(KL_THREADS), smem, stream, p)
