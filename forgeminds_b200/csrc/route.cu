@@ -6,11 +6,12 @@
 //   w = scale s / sum of the chosen s (or scale s)
 //   aux = aux_coef E sum_e f_e mean(s_e / sum s) + z_coef mean(logsumexp(z)^2),  f_e = share of all choices that fell on e
 //
-// LPT lanes share a token, each with VPL experts in registers (groups of four neighbours, so that the lanes' 16-byte
-// loads join up). Few lanes per token keep the shuffles of the k arg-max rounds few; the rounds bound the kernel, not
-// memory. The order must be that of the exact scores: without a bias it is that of the logits, which are compared as
-// they are; with one, or for sums over a group, scores are compared in fp32, and a token where two neighbours of the
-// order are nearer than fp32 errors is decided again in 64 bits.
+// Forward: LPT lanes share a token, each with VPL neighbouring experts. The order must be that of the exact scores. What
+// is compared are whole numbers of 32 bits: 23 bits of the score in fixed point, 9 of the expert's number, so that one
+// maximum finds value and expert and no two are equal. Each lane sorts its own by a network once; a round of the choice is
+// then a maximum over the lanes' first ones. A token where two neighbours of the order are nearer than the errors of score
+// and fixed point, and not equal by their inputs, is decided again in 64 bits; so is one with NaN or +inf.
+// Bound by these instructions (about 350 per token of 256 experts and 8 choices), not by memory.
 #include "fmb_api.h"
 #include "launch.cuh"
 #include "rows.cuh"
@@ -18,8 +19,6 @@
 namespace fmb {
 
 constexpr int ROUTE_THREADS = 128;
-constexpr int TAKEN = static_cast<int>(0x80000000);        // below the key of every value
-
 struct RouteParams {
   const void* logits;
   long long ld, tokens;
@@ -31,15 +30,6 @@ struct RouteParams {
   int E, k, softmax, groups, gsize, top_groups, best, renorm, vec;
   float scale;
 };
-
-// Whole numbers in the order of the values; NaN counts as the largest, -0 as 0.
-__device__ __forceinline__ int order_key(float v) {
-  v += 0.f;
-  if (v != v) return 0x7fffffff;
-  const int b = __float_as_int(v);
-  return b ^ ((b >> 31) & 0x7fffffff);
-}
-__device__ __forceinline__ float order_value(int key) { return __int_as_float(key ^ ((key >> 31) & 0x7fffffff)); }
 
 template <int LPT> __device__ __forceinline__ int expert_of(int i, int lane) { return (i >> 2) * (LPT * 4) + lane * 4 + (i & 3); }
 
@@ -62,60 +52,74 @@ __device__ __forceinline__ void load_logits(const T* row, int lane, int E, int v
 
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
 
-// A token's choice in 64 bits by its LPT lanes: writes the chosen experts to pick[0, k). Rare: the loops are plain.
-template <typename T, int LPT>
+// A token's choice in 64 bits by its LPT lanes: writes the chosen experts to pick[0, k). c, g: shared memory for E scores
+// and the groups'. Rare, and 30000 cycles long: a pair of neighbours alone is put in order without it.
+template <typename T, int LPT, int VPL>
 __device__ __noinline__ void choose_exactly(const RouteParams& p, const T* row, int lane, double* c, double* g, int* pick) {
+  const int e0 = lane * VPL;
+  double own[VPL];
   double top = -CUDART_INF, sum = 0.0;
+  unsigned open = 0;                                       // experts of this lane that can be chosen
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    own[i] = e0 + i < p.E ? static_cast<double>(to_f32(row[e0 + i])) : -CUDART_INF;
+    if (e0 + i < p.E) open |= 1u << i;
+    top = fmax(top, own[i]);
+  }
   if (p.softmax) {
-    for (int e = lane; e < p.E; e += LPT) top = fmax(top, static_cast<double>(to_f32(row[e])));
 #pragma unroll
     for (int o = LPT / 2; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (top == -CUDART_INF) top = 0.0;
+#pragma unroll 1
     for (int e = lane; e < p.E; e += LPT) sum += exp(static_cast<double>(to_f32(row[e])) - top);
 #pragma unroll
     for (int o = LPT / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sum == 0.0) sum = 1.0;
   }
-  for (int e = lane; e < p.E; e += LPT) {
-    const double z = to_f32(row[e]);
-    double v = (p.softmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z))) + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
-    c[e] = v != v ? CUDART_INF : v;
+  if (p.bias != nullptr || p.groups > 1) {
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += LPT) {
+      const double z = to_f32(row[e]);
+      const double v = (p.softmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z))) + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
+      c[e] = v != v ? CUDART_INF : v;
+    }
+    __syncwarp();
   }
-  __syncwarp();
-  unsigned kept = 0xffffffffu;
   if (p.groups > 1) {
     for (int n = lane; n < p.groups; n += LPT) {
       double a = -CUDART_INF, b = -CUDART_INF;             // the two largest
       for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
-        if (c[e] > a) { b = a; a = c[e]; } else if (c[e] > b) b = c[e];
+        const double v = c[e];
+        b = fmax(b, fmin(a, v));
+        a = fmax(a, v);
       }
       const double v = p.best > 1 && p.gsize > 1 ? a + b : a;
       g[n] = v != v ? CUDART_INF : v;
     }
     __syncwarp();
-    kept = 0;
-    for (int n = 0; n < p.groups; ++n) {
+    unsigned kept = 0;
+    for (int n = lane; n < p.groups; n += LPT) {
       int ahead = 0;
       for (int m = 0; m < p.groups; ++m) ahead += g[m] > g[n] || (g[m] == g[n] && m < n);
       if (ahead < p.top_groups) kept |= 1u << n;
     }
+#pragma unroll
+    for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e0 + i < p.E && !(kept >> ((e0 + i) / p.gsize) & 1)) open &= ~(1u << i);
   }
-  if (p.bias == nullptr)                                   // among the kept ones the order of the logits is the scores'
-    for (int e = lane; e < p.E; e += LPT) {
-      const double z = to_f32(row[e]);
-      c[e] = z != z ? CUDART_INF : z;
-    }
-  double last = CUDART_INF;
-  int last_e = -1;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {                          // without a bias the order of the logits is the scores'
+    if (p.bias != nullptr && e0 + i < p.E) own[i] = c[e0 + i];
+    if (own[i] != own[i]) own[i] = CUDART_INF;
+  }
   for (int j = 0; j < p.k; ++j) {
     double bv = -CUDART_INF;
     int be = 0x7fffffff;
-    for (int e = lane; e < p.E; e += LPT) {
-      const double v = c[e];
-      const bool open = p.groups == 1 || (kept >> (e / p.gsize) & 1);
-      const bool after = v < last || (v == last && e > last_e);
-      if (open && after && (v > bv || (v == bv && e < be))) { bv = v; be = e; }
-    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if ((open >> i & 1) && (own[i] > bv || be == 0x7fffffff)) { bv = own[i]; be = e0 + i; }
 #pragma unroll
     for (int o = LPT / 2; o > 0; o >>= 1) {
       const double ov = __shfl_xor_sync(0xffffffffu, bv, o);
@@ -123,38 +127,139 @@ __device__ __noinline__ void choose_exactly(const RouteParams& p, const T* row, 
       if (ov > bv || (ov == bv && oe < be)) { bv = ov; be = oe; }
     }
     if (lane == 0) pick[j] = be;
-    last = bv;
-    last_e = be;
+    if (be >= e0 && be < e0 + VPL) open &= ~(1u << (be - e0));
   }
   __syncwarp();
 }
 
+// 1 / (1 + e^-z) for comparisons: within 6e-7 (2^x to 2^-22, its argument to a unit, one addition, one reciprocal)
+__device__ __forceinline__ float sigmoid_near(float z) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + exp2_unit(z * -1.4426950408889634f)));
+  return r;
+}
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+constexpr int NUMBER_BITS = 9, FIXED = 1 << 23;            // a key: 23 bits of score, then 511 - expert
+constexpr unsigned NUMBER = (1u << NUMBER_BITS) - 1;
+// y up to 2^24 - 1, from 2^23 on rounded to a whole number by the addition that brought it there; less (or NaN) counts as 2^23
+__device__ __forceinline__ unsigned route_key(float y, int e) {
+  return (__float_as_uint(fmaxf(y, 8388608.f)) << NUMBER_BITS) + (NUMBER - e);
+}
+__device__ __forceinline__ unsigned key_score(unsigned key) { return key >> NUMBER_BITS; }
+__device__ __forceinline__ int key_expert(unsigned key) { return NUMBER - (key & NUMBER); }
+
+template <int W> __device__ __forceinline__ unsigned lanes_umax(unsigned v) {
+  if constexpr (W == 32) return __reduce_max_sync(0xffffffffu, v);
+#pragma unroll
+  for (int o = W / 2; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
+}
+
+// Falling order of N keys in registers: Batcher's merge exchange, no branches (19 exchanges for 8, 63 for 16).
+template <int N> __device__ __forceinline__ void sort_falling(unsigned (&v)[N]) {
+  if constexpr (N > 1)
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const unsigned a = v[i + j], b = v[i + j + k];
+            v[i + j] = max(a, b);
+            v[i + j + k] = min(a, b);
+          }
+}
+
+// VPL neighbouring experts' logits; -inf where there is none
+template <typename T, int VPL> __device__ __forceinline__ void load_own(const T* row, int e0, int E, int vec, float (&z)[VPL]) {
+  constexpr int BYTES = VPL * sizeof(T);
+  if (vec) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) z[i] = -CUDART_INF_F;
+    if (e0 < E) {
+      if constexpr (BYTES >= 16) load_f32<T, VPL>(row + e0, z);
+      else if constexpr (BYTES == 8 && sizeof(T) == 4) {
+        const float2 f = __ldg(reinterpret_cast<const float2*>(row + e0));
+        z[0] = f.x; z[1] = f.y;
+      } else if constexpr (BYTES == 8) load_f32<T, 4>(row + e0, z);
+      else if constexpr (BYTES == 4 && sizeof(T) == 2) {
+        const uint32_t u = __ldg(reinterpret_cast<const uint32_t*>(row + e0));
+        z[0] = __uint_as_float(u << 16); z[1] = __uint_as_float(u & 0xffff0000u);
+      } else z[0] = to_f32(row[e0]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) z[i] = e0 + i < E ? to_f32(row[e0 + i]) : -CUDART_INF_F;
+  }
+}
+
 template <typename T, int LPT, int VPL, bool AUX>
-__global__ void __launch_bounds__(ROUTE_THREADS) route_fwd_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kernel(const __grid_constant__ RouteParams p) {
   constexpr int TPB = ROUTE_THREADS / LPT;                 // tokens that a block has in hand
   constexpr int MOST_K = LPT * VPL < FMB_ROUTE_MAX_K ? LPT * VPL : FMB_ROUTE_MAX_K, PER = (MOST_K + LPT - 1) / LPT;
-  extern __shared__ double s_mem[];                        // c in 64 bits [TPB, E] and of groups [TPB, groups], when needed
-  __shared__ int s_pick[TPB][MOST_K + 1], s_key[TPB][MOST_K + 1];
-  extern __shared__ int s_dyn[];
+  extern __shared__ double s_mem[];                        // for the choice in 64 bits: scores [TPB, E], groups [TPB, groups]
+  __shared__ unsigned s_key[TPB][MOST_K + 2];
+  __shared__ int s_pick[TPB][MOST_K];
+  __shared__ float s_range[2][ROUTE_THREADS / 32];
+  double* c64 = s_mem + static_cast<size_t>(threadIdx.x / LPT) * p.E;
+  double* g64 = s_mem + static_cast<size_t>(TPB) * p.E + threadIdx.x / LPT * p.groups;
+  unsigned* s_n = reinterpret_cast<unsigned*>(c64);        // groups that are no whole lanes: the token's fixed-point scores
+  int* s_count = reinterpret_cast<int*>(s_mem + static_cast<size_t>(TPB) * (p.E + p.groups));   // [E]
+  float* s_acc = reinterpret_cast<float*>(s_count + p.E);                                       // [E + 1]
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT;
-  const bool by_logit = p.bias == nullptr, check_order = !by_logit, grouped = p.groups > 1;
-  const bool check_groups = grouped && !(by_logit && p.best == 1);
-  const bool exact_too = check_order || check_groups;
-  // How far a score in fp32 may be from the exact one, as a part of it: expf is within 2 units, the sum 1 + e and the
-  // division within half of one each; a softmax divides by a sum of up to 512 terms, 35 roundings deep. Scores are at
-  // most 1, so two scores of a group and two of another one are within 4 times that.
-  const float off = p.softmax ? 2.6e-6f : 4e-7f;
-  double* c64 = s_mem + static_cast<size_t>(slot) * p.E;
-  double* g64 = s_mem + static_cast<size_t>(TPB) * p.E + slot * p.groups;
-  float* c32 = reinterpret_cast<float*>(c64);              // read for the last time before the first store of 64 bits
-  int* s_count = s_dyn + (exact_too || grouped ? 2 * TPB * (p.E + p.groups) : 0);            // [E]
-  float* s_acc = reinterpret_cast<float*>(s_count + p.E);                             // [E + 1]
+  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT, e0 = lane * VPL;
+  const bool biased = p.bias != nullptr, grouped = p.groups > 1;
+  const bool by_score = biased || (grouped && p.best > 1); // else the order of the logits is the scores'
+  // groups that are a power of two of whole lanes
+  const int span = p.gsize / VPL;
+  const bool whole_lanes = p.gsize % VPL == 0 && (span & (span - 1)) == 0 && span <= LPT;
   for (int e = threadIdx.x; e < p.E; e += ROUTE_THREADS) s_count[e] = 0;
   if (AUX)
     for (int e = threadIdx.x; e <= p.E; e += ROUTE_THREADS) s_acc[e] = 0.f;
+  // the range of scores in fixed point: [0, 1] and what the finite biases add
+  float lo = 0.f, hi = 1.f;
+  bool bad_bias = false;                                   // NaN or +inf: every choice is then made in 64 bits
+  bool flat_bias = false;                                  // one finite bias for all
+  float bias[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    bias[i] = biased && e0 + i < p.E ? p.bias[e0 + i] : 0.f;
+    bad_bias |= !(bias[i] < CUDART_INF_F);
+  }
+  if (biased) {
+    float a = CUDART_INF_F, b = -CUDART_INF_F;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e0 + i < p.E && fabsf(bias[i]) < CUDART_INF_F) { a = fminf(a, bias[i]); b = fmaxf(b, bias[i]); }
+    a = -lanes_max<32>(-a);
+    b = lanes_max<32>(b);
+    if (threadIdx.x % 32 == 0) { s_range[0][threadIdx.x / 32] = a; s_range[1][threadIdx.x / 32] = b; }
+    __syncthreads();
+    for (int w = 0; w < ROUTE_THREADS / 32; ++w) { a = fminf(a, s_range[0][w]); b = fmaxf(b, s_range[1][w]); }
+    if (a <= b) { lo = a; hi = 1.f + b; }
+    bool same = a == b;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) same &= e0 + i >= p.E || bias[i] == a;
+    flat_bias = __all_sync(0xffffffffu, same);
+  }
   __syncthreads();
+  // steps per score, so few less that no rounding goes past the last one; what the bias adds to the fixed point
+  const float unit = static_cast<float>(FIXED - 16) / (hi - lo);
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) bias[i] = fmaf(bias[i] - lo, unit, 8388608.f);
+  // How far a score may be from the exact one. Sigmoid: s (1 - s) <= 1/4 of the error of e^-z (2^-22, and its argument's
+  // rounding, 3.3e-7 at |z| = 5.5 and less in s beyond), 1.8e-7 from addition and reciprocal: 3.4e-7. Softmax, divided by a
+  // sum of up to 512 terms some 30 roundings deep: 3e-6. Then a step of the fixed point. Two of those.
+  const unsigned near = static_cast<unsigned>(fminf((p.softmax ? 6e-6f : 6.8e-7f) * unit + 3.f, 1e6f));
   float acc[AUX ? VPL : 1], acc_z = 0.f;
 #pragma unroll
   for (int i = 0; i < (AUX ? VPL : 1); ++i) acc[i] = 0.f;
@@ -164,136 +269,202 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_fwd_kernel(const RoutePar
     const long long token = live ? base + slot : p.tokens - 1;       // lanes without a token go along with the last one
     const T* row = static_cast<const T*>(p.logits) + token * p.ld;
     float z[VPL];
-    load_logits<T, LPT, VPL>(row, lane, p.E, p.vec, z);
-    float top = 0.f, mass = 1.f;
-    if (p.softmax || AUX) {
-      top = z[0];
+    load_own<T, VPL>(row, e0, p.E, p.vec, z);
+    float top = z[0], mass = 1.f;
 #pragma unroll
-      for (int i = 1; i < VPL; ++i) top = fmaxf(top, z[i]);
-      top = lanes_max<LPT>(top);
+    for (int i = 1; i < VPL; ++i) top = max_or_nan(top, z[i]);
+    bool doubt = bad_bias || !(top < CUDART_INF_F);         // NaN or +inf, or an order that fp32 leaves open
+    if (p.softmax || AUX || !biased) top = lanes_max<LPT>(top);
+    const float high = top;
+    if (p.softmax || AUX) {
       if (top == -CUDART_INF_F) top = 0.f;                  // a row of nothing but -inf: scores of 0
       mass = 0.f;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) mass += expert_of<LPT>(i, lane) < p.E ? expf(z[i] - top) : 0.f;
+      for (int i = 0; i < VPL; ++i) mass += e0 + i < p.E ? expf(z[i] - top) : 0.f;
       mass = lanes_sum<LPT>(mass);
       if (mass == 0.f) mass = 1.f;
     }
     if constexpr (AUX) {
-      float norm = 1.f;
+      float norm = mass;
       if (!p.softmax) {
         norm = 0.f;
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) norm += expert_of<LPT>(i, lane) < p.E ? sigmoid(z[i]) : 0.f;
+        for (int i = 0; i < VPL; ++i) norm += e0 + i < p.E ? sigmoid(z[i]) : 0.f;
         norm = lanes_sum<LPT>(norm);
         if (norm == 0.f) norm = 1.f;
       }
       if (live) {
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-          if (expert_of<LPT>(i, lane) < p.E) acc[i] += p.softmax ? expf(z[i] - top) / mass : sigmoid(z[i]) / norm;
+          if (e0 + i < p.E) acc[i] += (p.softmax ? expf(z[i] - top) : sigmoid(z[i])) / norm;
         const float lse = top + logf(mass);
         if (lane == 0) acc_z += lse * lse;
       }
     }
-    int key[VPL];
+    // fixed-point scores and keys; group_n: scores for the groups' sums, where the keys are of logits
+    unsigned key[VPL], group_n[VPL];
+    if (by_score) {
+      const float inv_mass = __fdividef(1.f, mass);
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      const int e = expert_of<LPT>(i, lane);
-      float c = z[i];
-      if (!by_logit) c = (p.softmax ? expf(c - top) / mass : sigmoid(c)) + (e < p.E ? __ldg(p.bias + e) : 0.f);
-      key[i] = e < p.E ? order_key(c) : TAKEN;
+      for (int i = 0; i < VPL; ++i) {
+        const float c = p.softmax ? exp2_unit((z[i] - top) * 1.4426950408889634f) * inv_mass : sigmoid_near(z[i]);
+        group_n[i] = key[i] = route_key(fmaf(c, unit, bias[i]), e0 + i);
+      }
     }
-    bool doubt = false;
+    if (!biased) {                                          // 32 units of logit below the largest one in 23 bits
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) key[i] = route_key(fmaf(z[i] - high, 262144.f, 16777215.f), e0 + i);
+      if (!by_score)
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) group_n[i] = key[i];
+    }
+    if (e0 + VPL > p.E) {                                   // the last expert's key is above 0: its number is
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (e0 + i >= p.E) key[i] = group_n[i] = 0;
+    }
     if (grouped) {
-      // scores of the groups: each lane takes some of them from shared memory
-      __syncwarp();
+      unsigned low = 0, out = 0;                            // the lowest group kept and the highest left out
+      if (whole_lanes) {
+        unsigned a = 0, b = 0;                              // the two largest of the lane, then of the group
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int e = expert_of<LPT>(i, lane);
-        if (e < p.E) {
-          float c = order_value(key[i]);
-          if (by_logit && p.best > 1) c = p.softmax ? expf(z[i] - top) / mass : sigmoid(z[i]);
-          c32[e] = key[i] == 0x7fffffff ? CUDART_INF_F : c;
+        for (int i = 0; i < VPL; ++i) {
+          const unsigned v = group_n[i];
+          b = max(b, min(a, v));
+          a = max(a, v);
         }
-      }
-      __syncwarp();
-      float* g32 = reinterpret_cast<float*>(g64);
-      for (int n = lane; n < p.groups; n += LPT) {
-        float a = -CUDART_INF_F, b = -CUDART_INF_F;
-        for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
-          const float v = c32[e];
-          b = fmaxf(b, fminf(a, v));
-          a = fmaxf(a, v);
+        for (int o = 1; o < span; o *= 2) {
+          const unsigned oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+          b = max(max(b, ob), min(a, oa));
+          a = max(a, oa);
         }
-        const float v = p.best > 1 && p.gsize > 1 ? a + b : a;
-        g32[n] = v != v ? CUDART_INF_F : v;
-      }
-      __syncwarp();
-      unsigned kept = 0;
-      for (int n = lane; n < p.groups; n += LPT) {
-        const float mine = g32[n];
-        int ahead = 0;
-        for (int m = 0; m < p.groups; ++m) {
-          const float v = g32[m];
-          ahead += v > mine || (v == mine && m < n);
-          if (check_groups && m != n) doubt |= !(fabsf(v - mine) > 4.f * off + 2.4e-7f * (fabsf(v) + fabsf(mine)));
+        // the group's score above 31 - its number, the same in all its lanes
+        const unsigned at = lane / span;
+        unsigned mine = at < static_cast<unsigned>(p.groups)
+                            ? (key_score(a) + (p.best > 1 && p.gsize > 1 ? key_score(b) : 0u)) << 5 | (31 - at) : 0u;
+        bool kept = false;
+        for (int n = 0; n < p.top_groups; ++n) {
+          low = lanes_umax<LPT>(mine);
+          if (mine == low) {
+            kept = true;
+            mine = 0;
+          }
         }
-        if (ahead < p.top_groups) kept |= 1u << n;
-      }
+        out = lanes_umax<LPT>(mine);
+        if (!kept || at >= static_cast<unsigned>(p.groups)) {
 #pragma unroll
-      for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+          for (int i = 0; i < VPL; ++i) key[i] = 0;
+        }
+      } else {
+        __syncwarp();
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const int e = expert_of<LPT>(i, lane);
-        if (e < p.E && !(kept >> (e / p.gsize) & 1)) key[i] = TAKEN;
+        for (int i = 0; i < VPL; ++i)
+          if (e0 + i < p.E) s_n[e0 + i] = key_score(group_n[i]);
+        __syncwarp();
+        unsigned* s_g = reinterpret_cast<unsigned*>(g64);
+        for (int n = lane; n < p.groups; n += LPT) {
+          unsigned a = 0, b = 0;
+          for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
+            const unsigned v = s_n[e];
+            b = max(b, min(a, v));
+            a = max(a, v);
+          }
+          s_g[n] = (a + (p.best > 1 && p.gsize > 1 ? b : 0u)) << 5 | (31 - n);
+        }
+        __syncwarp();
+        unsigned kept = 0;
+        for (int n = lane; n < p.groups; n += LPT) {
+          int ahead = 0;
+          for (int m = 0; m < p.groups; ++m) ahead += s_g[m] > s_g[n];
+          if (ahead < p.top_groups) kept |= 1u << n;
+          if (ahead == p.top_groups - 1) low = s_g[n];
+          if (ahead >= p.top_groups) out = max(out, s_g[n]);
+        }
+#pragma unroll
+        for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+        low = lanes_umax<LPT>(low);
+        out = lanes_umax<LPT>(out);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+          if (e0 + i < p.E && !(kept >> ((e0 + i) / p.gsize) & 1)) key[i] = 0;
+        __syncwarp();
       }
+      const unsigned apart = by_score ? 2 * near : 3;
+      doubt |= p.top_groups < p.groups && (low >> 5) - (out >> 5) <= apart;
     }
-    // k rounds of arg-max, and one more to see how far behind the next one is
-    const int rounds = check_order ? p.k + 1 : p.k;
-    for (int j = 0; j < rounds; ++j) {
-      int bk = TAKEN, be = 0x7fffffff;
+    sort_falling(key);
+    // k rounds of the largest first key, and one more to see how far behind the next one is
+    auto round = [&](int j) {
+      const unsigned w = lanes_umax<LPT>(key[0]);
+      if (lane == 0) s_key[slot][j] = w;
+      if (key[0] == w) {
 #pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (key[i] > bk) { bk = key[i]; be = expert_of<LPT>(i, lane); }
-#pragma unroll
-      for (int o = LPT / 2; o > 0; o >>= 1) {
-        const int ok = __shfl_xor_sync(0xffffffffu, bk, o), oe = __shfl_xor_sync(0xffffffffu, be, o);
-        if (ok > bk || (ok == bk && oe < be)) { bk = ok; be = oe; }
+        for (int i = 0; i + 1 < VPL; ++i) key[i] = key[i + 1];
+        key[VPL - 1] = 0;
       }
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (expert_of<LPT>(i, lane) == be) key[i] = TAKEN;
-      if (lane == 0) { s_pick[slot][j] = be; s_key[slot][j] = bk; }
-    }
+    };
+    for (int j = 0; j <= p.k; ++j) round(j);
     __syncwarp();
-    if (check_order) {
-      for (int j = lane; j < p.k; j += LPT) {
-        const int ka = s_key[slot][j], kb = s_key[slot][j + 1];
-        if (kb == TAKEN) continue;                          // every expert is chosen
-        const int ea = s_pick[slot][j], eb = s_pick[slot][j + 1];
-        const float a = order_value(ka), b = order_value(kb), ba = p.bias[ea], bb = p.bias[eb];
-        const bool near = !(a - b > off * (fabsf(a - ba) + fabsf(b - bb)) + 1.2e-7f * (fabsf(a) + fabsf(b)) + 1e-37f);
-        const bool same = j + 1 < p.k && ka == kb && ba == bb && to_f32(row[ea]) == to_f32(row[eb]);    // in any precision
-        doubt |= near && !same;
-      }
+    const unsigned apart = biased ? near : 3;
+    // neighbours j, j + 1 of the order that are too near to tell
+    auto close = [&](int j) {
+      const unsigned ka = s_key[slot][j], kb = s_key[slot][j + 1];
+      return ka != 0 && kb != 0 && key_score(ka) - key_score(kb) <= apart;
+    };
+    bool hit = false;
+    for (int j = lane; j < p.k; j += LPT) {
+      const unsigned ka = s_key[slot][j];
+      s_pick[slot][j] = min(key_expert(ka), p.E - 1);       // (a token in doubt may have fewer keys than choices)
+      doubt |= ka == 0;
+      hit |= close(j);
     }
-    if (exact_too) {
-      unsigned who = __ballot_sync(0xffffffffu, doubt);
+    if (__any_sync(0xffffffffu, hit)) {
+      round(p.k + 1);
+      __syncwarp();
+      for (int j = lane; j < p.k; j += LPT) {
+        if (!close(j)) continue;
+        const int a = key_expert(s_key[slot][j]), b = key_expert(s_key[slot][j + 1]);
+        const float za = to_f32(row[a]), zb = to_f32(row[b]);
+        if (za == zb && (!biased || p.bias[a] == p.bias[b])) {
+          // equal in any precision, and the lower number is first; at the last choice the next one might belong before both
+          doubt |= j == p.k - 1 && close(j + 1);
+        } else if (p.softmax || !biased || (j > 0 && close(j - 1)) || close(j + 1)) {
+          doubt = true;
+        } else {                                            // a pair alone: in order by its exact scores
+          const double ca = 1.0 / (1.0 + exp(-static_cast<double>(za))) + static_cast<double>(p.bias[a]);
+          const double cb = 1.0 / (1.0 + exp(-static_cast<double>(zb))) + static_cast<double>(p.bias[b]);
+          if (cb > ca || (cb == ca && b < a)) {
+            s_pick[slot][j] = b;
+            if (j + 1 < p.k) s_pick[slot][j + 1] = a;
+          }
+        }
+      }
+      __syncwarp();
+    }
+    {
+      const unsigned who = __ballot_sync(0xffffffffu, doubt);
       if (who) {                                            // some token of this warp: all its lanes go, the others keep theirs
         const unsigned seg = LPT == 32 ? 0xffffffffu : ((1u << LPT) - 1u) << (threadIdx.x % 32 / LPT * LPT);
-        const bool mine = (who & seg) != 0;
+        // a row of one logit throughout (an untrained router, a padded token) is in order as it is, with equal biases
+        float floor = CUDART_INF_F;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+          if (e0 + i < p.E) floor = fminf(floor, z[i]);
+        floor = -lanes_max<LPT>(-floor);
+        const bool mine = (who & seg) != 0 && !(floor == high && (!biased || flat_bias));
         int keep[PER];
+        __syncwarp();
 #pragma unroll
         for (int n = 0; n < PER; ++n) keep[n] = n * LPT + lane < p.k ? s_pick[slot][n * LPT + lane] : 0;
         __syncwarp();
-        choose_exactly<T, LPT>(p, row, lane, c64, g64, s_pick[slot]);
+        if (__any_sync(0xffffffffu, mine)) choose_exactly<T, LPT, VPL>(p, row, lane, c64, g64, s_pick[slot]);
         if (!mine) {
 #pragma unroll
           for (int n = 0; n < PER; ++n)
             if (n * LPT + lane < p.k) s_pick[slot][n * LPT + lane] = keep[n];
         }
-        __syncwarp();
       }
+      __syncwarp();
     }
     // weights of the chosen, each by a lane of its own
     float sum = 0.f, best = -CUDART_INF_F, chosen[PER];
@@ -303,7 +474,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_fwd_kernel(const RoutePar
       chosen[n] = j < p.k ? to_f32(row[s_pick[slot][j]]) : -CUDART_INF_F;
       best = fmaxf(best, chosen[n]);
     }
-    best = lanes_max<LPT>(best);
+    if (p.softmax) best = lanes_max<LPT>(best);
     // shares of the chosen alone are taken around their own maximum: they may all lie far below the row's
     const float from = !p.renorm ? top : best == -CUDART_INF_F ? 0.f : best;
 #pragma unroll
@@ -314,17 +485,19 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_fwd_kernel(const RoutePar
       }
     }
     sum = lanes_sum<LPT>(sum);
-    if (!p.softmax && p.renorm && __any_sync(0xffffffffu, sum < 1e-30f && best > -CUDART_INF_F)) {
+    if (!p.softmax && p.renorm && __any_sync(0xffffffffu, sum < 1e-30f)) {
       // sigmoids that vanish in fp32 still have shares: s = e^z there
-      float far = 0.f;
+      const float peak = lanes_max<LPT>(best), around = peak == -CUDART_INF_F ? 0.f : peak;
+      float far = 0.f, share[PER];
 #pragma unroll
-      for (int n = 0; n < PER; ++n)
-        if (n * LPT + lane < p.k) far += expf(to_f32(row[s_pick[slot][n * LPT + lane]]) - from);
+      for (int n = 0; n < PER; ++n) {
+        share[n] = n * LPT + lane < p.k ? expf(to_f32(row[s_pick[slot][n * LPT + lane]]) - around) : 0.f;
+        far += share[n];
+      }
       far = lanes_sum<LPT>(far);
-      if (sum < 1e-30f && best > -CUDART_INF_F) {
+      if (sum < 1e-30f) {
 #pragma unroll
-        for (int n = 0; n < PER; ++n)
-          if (n * LPT + lane < p.k) chosen[n] = expf(to_f32(row[s_pick[slot][n * LPT + lane]]) - from);
+        for (int n = 0; n < PER; ++n) chosen[n] = share[n];
         sum = far;
       }
     }
@@ -347,7 +520,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_fwd_kernel(const RoutePar
       if (slot == who) {
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-          if (expert_of<LPT>(i, lane) < p.E) s_acc[expert_of<LPT>(i, lane)] += acc[i];
+          if (e0 + i < p.E) s_acc[e0 + i] += acc[i];
         if (lane == 0) s_acc[p.E] += acc_z;
       }
     }
@@ -532,12 +705,12 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_bwd_kernel(const RouteGra
 }
 
 template <typename T, int LPT, int VPL>
-int route_fwd_run(const RouteParams& p, int blocks, cudaStream_t stream) {
-  constexpr int TPB = ROUTE_THREADS / LPT;
-  const bool room = p.bias != nullptr || p.groups > 1;
-  const size_t smem = (room ? sizeof(double) * TPB * (p.E + p.groups) : 0) + sizeof(int) * (2 * p.E + 1);
+int route_fwd_run(RouteParams p, int blocks, cudaStream_t stream) {
+  constexpr int TPB = ROUTE_THREADS / LPT, BYTES = VPL * sizeof(T) < 16 ? VPL * sizeof(T) : 16;
+  // at most 8 (64 + 32) or 4 (512 + 32) values of 64 bits and two arrays of 512: with the static ones below 48 KB
+  const size_t smem = sizeof(double) * TPB * (p.E + p.groups) + sizeof(int) * (2 * p.E + 1);
+  p.vec = p.E % VPL == 0 && p.ld % VPL == 0 && reinterpret_cast<uintptr_t>(p.logits) % BYTES == 0;
   auto kernel = p.partial != nullptr ? route_fwd_kernel<T, LPT, VPL, true> : route_fwd_kernel<T, LPT, VPL, false>;
-  // at most 16 (256 + 32) or 8 (512 + 32) values of 64 bits: with the static arrays below the 48 KB that need no opting in
   return launch_pdl(kernel, dim3(blocks), dim3(ROUTE_THREADS), smem, stream, p) == cudaSuccess ? 0 : -3;
 }
 
@@ -549,8 +722,9 @@ template <typename T, int LPT, int VPL> int route_bwd_run(const RouteGrad& p, bo
   return e == cudaSuccess ? 0 : -3;
 }
 
-// lanes per token by the number of experts
-inline int route_lanes(int E) { return E <= 8 ? 1 : E <= 16 ? 2 : E <= 32 ? 4 : E <= 256 ? 8 : 16; }
+// Lanes per token in the forward pass: 8 where 8 experts for each hold them all (a warp then serves four tokens), up to a
+// warp beyond (its maximum over the lanes is one instruction).
+inline int route_lanes(int E) { return E <= 64 ? 8 : E <= 128 ? 16 : 32; }
 
 }  // namespace fmb
 
@@ -558,19 +732,29 @@ using namespace fmb;
 
 extern "C" int fmb_route_blocks(long long tokens, int E) {
   const int per = ROUTE_THREADS / route_lanes(E);
-  const long long need = (tokens + per - 1) / per, most = 4LL * sm_count();
+  const long long need = (tokens + per - 1) / per, most = (E <= 256 ? 5LL : 3LL) * sm_count();      // as many as are resident
   return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
 }
 
-#define FMB_ROUTE(T, RUN, ...)                                       \
+#define FMB_ROUTE_FWD(T, ...)                                        \
   do {                                                               \
-    if (E <= 8) return RUN<T, 1, 8>(__VA_ARGS__);                    \
-    if (E <= 16) return RUN<T, 2, 8>(__VA_ARGS__);                   \
-    if (E <= 32) return RUN<T, 4, 8>(__VA_ARGS__);                   \
-    if (E <= 64) return RUN<T, 8, 8>(__VA_ARGS__);                   \
-    if (E <= 128) return RUN<T, 8, 16>(__VA_ARGS__);                 \
-    if (E <= 256) return RUN<T, 8, 32>(__VA_ARGS__);                 \
-    return RUN<T, 16, 32>(__VA_ARGS__);                              \
+    if (E <= 8) return route_fwd_run<T, 8, 1>(__VA_ARGS__);          \
+    if (E <= 16) return route_fwd_run<T, 8, 2>(__VA_ARGS__);         \
+    if (E <= 32) return route_fwd_run<T, 8, 4>(__VA_ARGS__);         \
+    if (E <= 64) return route_fwd_run<T, 8, 8>(__VA_ARGS__);         \
+    if (E <= 128) return route_fwd_run<T, 16, 8>(__VA_ARGS__);       \
+    if (E <= 256) return route_fwd_run<T, 32, 8>(__VA_ARGS__);       \
+    return route_fwd_run<T, 32, 16>(__VA_ARGS__);                    \
+  } while (0)
+#define FMB_ROUTE_BWD(T, ...)                                        \
+  do {                                                               \
+    if (E <= 8) return route_bwd_run<T, 1, 8>(__VA_ARGS__);          \
+    if (E <= 16) return route_bwd_run<T, 2, 8>(__VA_ARGS__);         \
+    if (E <= 32) return route_bwd_run<T, 4, 8>(__VA_ARGS__);         \
+    if (E <= 64) return route_bwd_run<T, 8, 8>(__VA_ARGS__);         \
+    if (E <= 128) return route_bwd_run<T, 8, 16>(__VA_ARGS__);       \
+    if (E <= 256) return route_bwd_run<T, 8, 32>(__VA_ARGS__);       \
+    return route_bwd_run<T, 16, 32>(__VA_ARGS__);                    \
   } while (0)
 
 extern "C" int fmb_route_fwd(const void* logits, long long ld, int dtype, const float* bias, float* weights, int* idx,
@@ -586,10 +770,9 @@ extern "C" int fmb_route_fwd(const void* logits, long long ld, int dtype, const 
   p.logits = logits; p.ld = ld; p.tokens = tokens; p.bias = bias; p.weights = weights; p.idx = idx; p.counts = counts;
   p.partial = partial; p.E = E; p.k = k; p.softmax = softmax; p.groups = groups; p.gsize = E / groups; p.top_groups = top_groups;
   p.best = best; p.renorm = renorm; p.scale = scale;
-  p.vec = E % 4 == 0 && ld % 4 == 0 && aligned16(logits);
   int rc = -1;
-  if (dtype == FMB_BF16) rc = [&]() -> int { FMB_ROUTE(__nv_bfloat16, route_fwd_run, p, blocks, stream); }();
-  else if (dtype == FMB_F32) rc = [&]() -> int { FMB_ROUTE(float, route_fwd_run, p, blocks, stream); }();
+  if (dtype == FMB_BF16) rc = [&]() -> int { FMB_ROUTE_FWD(__nv_bfloat16, p, blocks, stream); }();
+  else if (dtype == FMB_F32) rc = [&]() -> int { FMB_ROUTE_FWD(float, p, blocks, stream); }();
   if (rc != 0 || partial == nullptr) return rc;
   return launch_pdl(route_aux_kernel, dim3(1), dim3(32, 32), 0, stream, partial, counts, aux, blocks, E, tokens, k, aux_coef,
                     z_coef) == cudaSuccess ? 0 : -3;
@@ -606,7 +789,7 @@ extern "C" int fmb_route_bwd(const void* logits, long long ld, int dtype, const 
   p.aux_coef = aux_coef; p.z_coef = z_coef;
   p.vec = E % 4 == 0 && ld % 4 == 0 && aligned16(logits) && aligned16(dlogits);
   const bool dense = daux != nullptr || (softmax && !renorm);
-  if (dtype == FMB_BF16) FMB_ROUTE(__nv_bfloat16, route_bwd_run, p, dense, stream);
-  if (dtype == FMB_F32) FMB_ROUTE(float, route_bwd_run, p, dense, stream);
+  if (dtype == FMB_BF16) FMB_ROUTE_BWD(__nv_bfloat16, p, dense, stream);
+  if (dtype == FMB_F32) FMB_ROUTE_BWD(float, p, dense, stream);
   return -1;
 }
