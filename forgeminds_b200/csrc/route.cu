@@ -201,8 +201,63 @@ template <typename T, int VPL> __device__ __forceinline__ void load_own(const T*
   }
 }
 
+// Whether expert b comes before expert a by their exact scores (sigmoids with their biases).
+__device__ __noinline__ bool sigmoid_ahead(float za, float zb, float bias_a, float bias_b, bool lower) {
+  const double a = 1.0 / (1.0 + exp(-static_cast<double>(za))) + static_cast<double>(bias_a);
+  const double b = 1.0 / (1.0 + exp(-static_cast<double>(zb))) + static_cast<double>(bias_b);
+  return b > a || (b == a && lower);
+}
+
+// The choice of a warp's tokens where some neighbours j, j + 1 of key[0, k + 2) are within `apart`, or a token is in doubt
+// already: pairs that stand alone are put in order, other tokens decided again. Writes pick[0, k).
+template <typename T, int LPT, int VPL>
+__device__ __noinline__ void settle(const RouteParams& p, const T* row, int lane, unsigned apart, bool doubt, bool flat_bias,
+                                    const unsigned* key, int* pick, double* c64, double* g64) {
+  const bool biased = p.bias != nullptr;
+  auto close = [&](int j) { return key[j] != 0 && key[j + 1] != 0 && key_score(key[j]) - key_score(key[j + 1]) <= apart; };
+  for (int j = lane; j < p.k; j += LPT) pick[j] = min(key_expert(key[j]), p.E - 1);
+  __syncwarp();
+  for (int j = lane; j < p.k; j += LPT) {
+    if (!close(j)) continue;
+    const int a = key_expert(key[j]), b = key_expert(key[j + 1]);
+    const float za = to_f32(row[a]), zb = to_f32(row[b]);
+    if (za == zb && (!biased || p.bias[a] == p.bias[b])) {
+      // equal in any precision, and the lower number is first; at the last choice the next one might belong before both
+      doubt |= j == p.k - 1 && close(j + 1);
+    } else if (p.softmax || !biased || (j > 0 && close(j - 1)) || close(j + 1)) {
+      doubt = true;
+    } else if (sigmoid_ahead(za, zb, p.bias[a], p.bias[b], b < a)) {
+      pick[j] = b;
+      if (j + 1 < p.k) pick[j + 1] = a;
+    }
+  }
+  __syncwarp();
+  unsigned who = __ballot_sync(0xffffffffu, doubt);
+  if (who == 0) return;
+  // a row of one logit throughout (an untrained router, a padded token) is in order as it is, with equal biases
+  bool flat = flat_bias;
+  for (int e = lane; e < p.E; e += LPT) flat &= to_f32(row[e]) == to_f32(row[0]);
+  who = __ballot_sync(0xffffffffu, !flat);
+  const unsigned seg = LPT == 32 ? 0xffffffffu : ((1u << LPT) - 1u) << (threadIdx.x % 32 / LPT * LPT);
+  flat = (who & seg) == 0;
+  who = __ballot_sync(0xffffffffu, doubt && !flat);
+  if (who == 0) return;
+  constexpr int MOST_K = LPT * VPL < FMB_ROUTE_MAX_K ? LPT * VPL : FMB_ROUTE_MAX_K, PER = (MOST_K + LPT - 1) / LPT;
+  int keep[PER];
+#pragma unroll
+  for (int n = 0; n < PER; ++n) keep[n] = n * LPT + lane < p.k ? pick[n * LPT + lane] : 0;
+  __syncwarp();
+  choose_exactly<T, LPT, VPL>(p, row, lane, c64, g64, pick);
+  if ((who & seg) == 0) {                                  // the other tokens keep theirs
+#pragma unroll
+    for (int n = 0; n < PER; ++n)
+      if (n * LPT + lane < p.k) pick[n * LPT + lane] = keep[n];
+  }
+  __syncwarp();
+}
+
 template <typename T, int LPT, int VPL, bool AUX>
-__global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kernel(const __grid_constant__ RouteParams p) {
+__global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kernel(const __grid_constant__ RouteParams p) {
   constexpr int TPB = ROUTE_THREADS / LPT;                 // tokens that a block has in hand
   constexpr int MOST_K = LPT * VPL < FMB_ROUTE_MAX_K ? LPT * VPL : FMB_ROUTE_MAX_K, PER = (MOST_K + LPT - 1) / LPT;
   extern __shared__ double s_mem[];                        // for the choice in 64 bits: scores [TPB, E], groups [TPB, groups]
@@ -222,6 +277,8 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
   // groups that are a power of two of whole lanes
   const int span = p.gsize / VPL;
   const bool whole_lanes = p.gsize % VPL == 0 && (span & (span - 1)) == 0 && span <= LPT;
+  const unsigned own_group = grouped && whole_lanes ? lane / span : 0;
+  const bool has_group = own_group < static_cast<unsigned>(p.groups), two_best = p.best > 1 && p.gsize > 1;
   for (int e = threadIdx.x; e < p.E; e += ROUTE_THREADS) s_count[e] = 0;
   if (AUX)
     for (int e = threadIdx.x; e <= p.E; e += ROUTE_THREADS) s_acc[e] = 0.f;
@@ -264,18 +321,23 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
 #pragma unroll
   for (int i = 0; i < (AUX ? VPL : 1); ++i) acc[i] = 0.f;
 
-  for (long long base = static_cast<long long>(blockIdx.x) * TPB; base < p.tokens; base += static_cast<long long>(gridDim.x) * TPB) {
-    const bool live = base + slot < p.tokens;
-    const long long token = live ? base + slot : p.tokens - 1;       // lanes without a token go along with the last one
-    const T* row = static_cast<const T*>(p.logits) + token * p.ld;
-    float z[VPL];
-    load_own<T, VPL>(row, e0, p.E, p.vec, z);
+  const int tokens = static_cast<int>(p.tokens);
+  const int stride = gridDim.x * TPB;                       // (fewer than 2^31 tokens)
+  float z[VPL];
+  auto row_of = [&](int base) {                       // lanes without a token go along with the last one
+    return static_cast<const T*>(p.logits) + static_cast<long long>(min(base + slot, tokens - 1)) * p.ld;
+  };
+  load_own<T, VPL>(row_of(blockIdx.x * TPB), e0, p.E, p.vec, z);
+  for (int base = blockIdx.x * TPB; base < tokens; base += stride) {
+    const bool live = base + slot < tokens;
+    const int token = min(base + slot, tokens - 1);
+    const T* row = row_of(base);
     float top = z[0], mass = 1.f;
 #pragma unroll
     for (int i = 1; i < VPL; ++i) top = max_or_nan(top, z[i]);
     bool doubt = bad_bias || !(top < CUDART_INF_F);         // NaN or +inf, or an order that fp32 leaves open
     if (p.softmax || AUX || !biased) top = lanes_max<LPT>(top);
-    const float high = top;
+    const float high = top;                                 // (of this lane alone where nothing needs the row's)
     if (p.softmax || AUX) {
       if (top == -CUDART_INF_F) top = 0.f;                  // a row of nothing but -inf: scores of 0
       mass = 0.f;
@@ -301,65 +363,65 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
         if (lane == 0) acc_z += lse * lse;
       }
     }
-    // fixed-point scores and keys; group_n: scores for the groups' sums, where the keys are of logits
-    unsigned key[VPL], group_n[VPL];
+    // fixed-point scores and keys; first, second: the lane's two largest for its group
+    unsigned key[VPL], first = 0, second = 0;
+    auto see = [&](unsigned v, int e) {
+      if (e < p.E) {
+        second = max(second, min(first, v));
+        first = max(first, v);
+        if (!whole_lanes) s_n[e] = key_score(v);
+      }
+    };
+    if (grouped && !whole_lanes) __syncwarp();              // the scores of the token before have been read
     if (by_score) {
       const float inv_mass = __fdividef(1.f, mass);
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
         const float c = p.softmax ? exp2_unit((z[i] - top) * 1.4426950408889634f) * inv_mass : sigmoid_near(z[i]);
-        group_n[i] = key[i] = route_key(fmaf(c, unit, bias[i]), e0 + i);
+        key[i] = route_key(fmaf(c, unit, bias[i]), e0 + i);
+      }
+      if (grouped) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
       }
     }
     if (!biased) {                                          // 32 units of logit below the largest one in 23 bits
 #pragma unroll
       for (int i = 0; i < VPL; ++i) key[i] = route_key(fmaf(z[i] - high, 262144.f, 16777215.f), e0 + i);
-      if (!by_score)
+      if (grouped && !by_score) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i) group_n[i] = key[i];
+        for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
+      }
     }
+    if (base + stride < tokens) load_own<T, VPL>(row_of(base + stride), e0, p.E, p.vec, z);      // the next token's
     if (e0 + VPL > p.E) {                                   // the last expert's key is above 0: its number is
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
-        if (e0 + i >= p.E) key[i] = group_n[i] = 0;
+        if (e0 + i >= p.E) key[i] = 0;
     }
     if (grouped) {
       unsigned low = 0, out = 0;                            // the lowest group kept and the highest left out
       if (whole_lanes) {
-        unsigned a = 0, b = 0;                              // the two largest of the lane, then of the group
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) {
-          const unsigned v = group_n[i];
-          b = max(b, min(a, v));
-          a = max(a, v);
-        }
+        unsigned a = first, b = second;                     // of the lane, then of the group
         for (int o = 1; o < span; o *= 2) {
           const unsigned oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
           b = max(max(b, ob), min(a, oa));
           a = max(a, oa);
         }
         // the group's score above 31 - its number, the same in all its lanes
-        const unsigned at = lane / span;
-        unsigned mine = at < static_cast<unsigned>(p.groups)
-                            ? (key_score(a) + (p.best > 1 && p.gsize > 1 ? key_score(b) : 0u)) << 5 | (31 - at) : 0u;
-        bool kept = false;
+        unsigned mine = has_group ? (key_score(a) + (two_best ? key_score(b) : 0u)) << 5 | (31 - own_group) : 0u;
+        const unsigned whole = mine;
+#pragma unroll 1
         for (int n = 0; n < p.top_groups; ++n) {
           low = lanes_umax<LPT>(mine);
-          if (mine == low) {
-            kept = true;
-            mine = 0;
-          }
+          mine = mine == low ? 0 : mine;
         }
         out = lanes_umax<LPT>(mine);
-        if (!kept || at >= static_cast<unsigned>(p.groups)) {
+        if (whole < low || !has_group) {                    // a group that is left out
 #pragma unroll
           for (int i = 0; i < VPL; ++i) key[i] = 0;
         }
       } else {
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (e0 + i < p.E) s_n[e0 + i] = key_score(group_n[i]);
         __syncwarp();
         unsigned* s_g = reinterpret_cast<unsigned*>(g64);
         for (int n = lane; n < p.groups; n += LPT) {
@@ -369,7 +431,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
             b = max(b, min(a, v));
             a = max(a, v);
           }
-          s_g[n] = (a + (p.best > 1 && p.gsize > 1 ? b : 0u)) << 5 | (31 - n);
+          s_g[n] = (a + (two_best ? b : 0u)) << 5 | (31 - n);
         }
         __syncwarp();
         unsigned kept = 0;
@@ -393,77 +455,59 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
       doubt |= p.top_groups < p.groups && (low >> 5) - (out >> 5) <= apart;
     }
     sort_falling(key);
-    // k rounds of the largest first key, and one more to see how far behind the next one is
-    auto round = [&](int j) {
+    // k rounds of the largest first key, each kept by a lane of its own, and one more to see how far behind the next one is
+    auto round = [&]() {
       const unsigned w = lanes_umax<LPT>(key[0]);
-      if (lane == 0) s_key[slot][j] = w;
       if (key[0] == w) {
 #pragma unroll
         for (int i = 0; i + 1 < VPL; ++i) key[i] = key[i + 1];
         key[VPL - 1] = 0;
       }
+      return w;
     };
-    for (int j = 0; j <= p.k; ++j) round(j);
-    __syncwarp();
+    unsigned mine[PER];
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      mine[n] = 0;
+#pragma unroll 1
+      for (int j = n * LPT; j < (n + 1) * LPT && j < p.k; ++j) {
+        const unsigned w = round();
+        if (lane == j - n * LPT) mine[n] = w;
+      }
+    }
+    const unsigned next = round();
     const unsigned apart = biased ? near : 3;
-    // neighbours j, j + 1 of the order that are too near to tell
-    auto close = [&](int j) {
-      const unsigned ka = s_key[slot][j], kb = s_key[slot][j + 1];
-      return ka != 0 && kb != 0 && key_score(ka) - key_score(kb) <= apart;
-    };
-    bool hit = false;
-    for (int j = lane; j < p.k; j += LPT) {
-      const unsigned ka = s_key[slot][j];
-      s_pick[slot][j] = min(key_expert(ka), p.E - 1);       // (a token in doubt may have fewer keys than choices)
-      doubt |= ka == 0;
-      hit |= close(j);
+    int pick[PER];
+    bool hit = false;                                       // neighbours of the order that are too near to tell
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      const int j = n * LPT + lane;
+      unsigned after = __shfl_down_sync(0xffffffffu, mine[n], 1, LPT);
+      if (n + 1 < PER) {
+        const unsigned turn = __shfl_sync(0xffffffffu, mine[n + 1 < PER ? n + 1 : n], 0, LPT);
+        if (lane == LPT - 1) after = turn;
+      }
+      if (j == p.k - 1) after = next;
+      pick[n] = min(key_expert(mine[n]), p.E - 1);          // (a token in doubt may have fewer keys than choices)
+      if (j < p.k) {
+        doubt |= mine[n] == 0;
+        hit |= after != 0 && key_score(mine[n]) - key_score(after) <= apart;
+      }
     }
-    if (__any_sync(0xffffffffu, hit)) {
-      round(p.k + 1);
-      __syncwarp();
-      for (int j = lane; j < p.k; j += LPT) {
-        if (!close(j)) continue;
-        const int a = key_expert(s_key[slot][j]), b = key_expert(s_key[slot][j + 1]);
-        const float za = to_f32(row[a]), zb = to_f32(row[b]);
-        if (za == zb && (!biased || p.bias[a] == p.bias[b])) {
-          // equal in any precision, and the lower number is first; at the last choice the next one might belong before both
-          doubt |= j == p.k - 1 && close(j + 1);
-        } else if (p.softmax || !biased || (j > 0 && close(j - 1)) || close(j + 1)) {
-          doubt = true;
-        } else {                                            // a pair alone: in order by its exact scores
-          const double ca = 1.0 / (1.0 + exp(-static_cast<double>(za))) + static_cast<double>(p.bias[a]);
-          const double cb = 1.0 / (1.0 + exp(-static_cast<double>(zb))) + static_cast<double>(p.bias[b]);
-          if (cb > ca || (cb == ca && b < a)) {
-            s_pick[slot][j] = b;
-            if (j + 1 < p.k) s_pick[slot][j + 1] = a;
-          }
-        }
+    if (__any_sync(0xffffffffu, hit || doubt)) {            // one token of this warp, or more: all its lanes go
+      const unsigned then = round();
+#pragma unroll
+      for (int n = 0; n < PER; ++n)
+        if (n * LPT + lane < p.k) s_key[slot][n * LPT + lane] = mine[n];
+      if (lane == 0) {
+        s_key[slot][p.k] = next;
+        s_key[slot][p.k + 1] = then;
       }
       __syncwarp();
-    }
-    {
-      const unsigned who = __ballot_sync(0xffffffffu, doubt);
-      if (who) {                                            // some token of this warp: all its lanes go, the others keep theirs
-        const unsigned seg = LPT == 32 ? 0xffffffffu : ((1u << LPT) - 1u) << (threadIdx.x % 32 / LPT * LPT);
-        // a row of one logit throughout (an untrained router, a padded token) is in order as it is, with equal biases
-        float floor = CUDART_INF_F;
+      settle<T, LPT, VPL>(p, row, lane, apart, doubt, !biased || flat_bias, s_key[slot], s_pick[slot], c64, g64);
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (e0 + i < p.E) floor = fminf(floor, z[i]);
-        floor = -lanes_max<LPT>(-floor);
-        const bool mine = (who & seg) != 0 && !(floor == high && (!biased || flat_bias));
-        int keep[PER];
-        __syncwarp();
-#pragma unroll
-        for (int n = 0; n < PER; ++n) keep[n] = n * LPT + lane < p.k ? s_pick[slot][n * LPT + lane] : 0;
-        __syncwarp();
-        if (__any_sync(0xffffffffu, mine)) choose_exactly<T, LPT, VPL>(p, row, lane, c64, g64, s_pick[slot]);
-        if (!mine) {
-#pragma unroll
-          for (int n = 0; n < PER; ++n)
-            if (n * LPT + lane < p.k) s_pick[slot][n * LPT + lane] = keep[n];
-        }
-      }
+      for (int n = 0; n < PER; ++n)
+        if (n * LPT + lane < p.k) pick[n] = s_pick[slot][n * LPT + lane];
       __syncwarp();
     }
     // weights of the chosen, each by a lane of its own
@@ -471,7 +515,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
 #pragma unroll
     for (int n = 0; n < PER; ++n) {
       const int j = n * LPT + lane;
-      chosen[n] = j < p.k ? to_f32(row[s_pick[slot][j]]) : -CUDART_INF_F;
+      chosen[n] = j < p.k ? to_f32(row[pick[n]]) : -CUDART_INF_F;
       best = fmaxf(best, chosen[n]);
     }
     if (p.softmax) best = lanes_max<LPT>(best);
@@ -491,7 +535,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
       float far = 0.f, share[PER];
 #pragma unroll
       for (int n = 0; n < PER; ++n) {
-        share[n] = n * LPT + lane < p.k ? expf(to_f32(row[s_pick[slot][n * LPT + lane]]) - around) : 0.f;
+        share[n] = n * LPT + lane < p.k ? expf(to_f32(row[pick[n]]) - around) : 0.f;
         far += share[n];
       }
       far = lanes_sum<LPT>(far);
@@ -506,9 +550,9 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 5) route_fwd_kern
     for (int n = 0; n < PER; ++n) {
       const int j = n * LPT + lane;
       if (j < p.k && live) {
-        const int e = s_pick[slot][j];
-        p.weights[token * p.k + j] = chosen[n] * by;
-        p.idx[token * p.k + j] = e;
+        const int e = pick[n];
+        p.weights[static_cast<long long>(token) * p.k + j] = chosen[n] * by;
+        p.idx[static_cast<long long>(token) * p.k + j] = e;
         atomicAdd(&s_count[e], 1);
       }
     }
@@ -732,7 +776,7 @@ using namespace fmb;
 
 extern "C" int fmb_route_blocks(long long tokens, int E) {
   const int per = ROUTE_THREADS / route_lanes(E);
-  const long long need = (tokens + per - 1) / per, most = (E <= 256 ? 5LL : 3LL) * sm_count();      // as many as are resident
+  const long long need = (tokens + per - 1) / per, most = (E <= 256 ? 6LL : 3LL) * sm_count();      // as many as are resident
   return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
 }
 
@@ -766,6 +810,7 @@ extern "C" int fmb_route_fwd(const void* logits, long long ld, int dtype, const 
     return -2;
   if (cudaMemsetAsync(counts, 0, E * sizeof(int), stream) != cudaSuccess) return -3;
   if (tokens <= 0) return 0;
+  if (tokens > 0x7fff0000LL) return -2;                    // steps over the tokens stay within 31 bits
   RouteParams p = {};
   p.logits = logits; p.ld = ld; p.tokens = tokens; p.bias = bias; p.weights = weights; p.idx = idx; p.counts = counts;
   p.partial = partial; p.E = E; p.k = k; p.softmax = softmax; p.groups = groups; p.gsize = E / groups; p.top_groups = top_groups;
