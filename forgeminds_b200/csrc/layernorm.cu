@@ -12,6 +12,11 @@
 
 namespace fmb {
 
+__device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+// Rows of a block's ring in the backward pass: 512 threads with two chunks of three tensors are 48 KB each.
+template <int VPL> struct BwdStages { static constexpr int N = VPL == 1 ? 3 : 2; };
+
 // How a thread of a row's TPR threads sees it: chunk i of N values. VEC: 16 contiguous bytes; otherwise N single
 // values TPR apart (widths, pitches or addresses that are no multiple of 16 bytes), still coalesced.
 template <typename T, int TPR, bool VEC> struct RowMap {
@@ -183,7 +188,9 @@ layernorm_fwd_wide_kernel(const T* __restrict__ x, long long ldx, const T* __res
 
 // ------------------------------------------------------------------ backward
 // Blocks walk over the rows. A thread keeps its columns' sums of dy xh and dy in registers; a block leaves them as
-// one row of `partial` [blocks, 2, d], which the column kernel below adds in a fixed order.
+// one row of `partial` [blocks, 2, d], which the column kernel below adds in a fixed order. With 16-byte chunks the rows
+// come through a ring of shared memory, copied STAGES - 1 rows ahead, each thread its own chunks (no barrier guards them):
+// with loads into registers a block waited out the memory's latency at every row.
 template <typename T, typename WT, int TPR, int VPL, bool VEC>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
 layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
@@ -191,11 +198,14 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
                      T* __restrict__ dx, float* __restrict__ partial, long long rows, int d, float inv_d) {
   using M = RowMap<T, TPR, VEC>;
   constexpr int N = M::N, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
+  constexpr int STAGES = BwdStages<VPL>::N;
   __shared__ float2 scratch[2][THREADS / 32];
-  extern __shared__ float s_fold[];                       // [2, d], when several rows share a block
+  extern __shared__ uint4 s_ring[];                       // [stage][dy, x, dres][chunk][thread]; the fold below takes its place
+  float* s_fold = reinterpret_cast<float*>(s_ring);       // [2, d], when several rows share a block
   pdl_wait();
   pdl_launch_dependents();
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+  const int tensors = dres != nullptr ? 3 : 2;
   float wv[VPL][N], dwa[VPL][N], dba[VPL][N];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
@@ -203,18 +213,51 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
 #pragma unroll
     for (int j = 0; j < N; ++j) { dwa[i][j] = 0.f; dba[i][j] = 0.f; }
   }
-  int turn = 0;
-  for (long long base = static_cast<long long>(blockIdx.x) * RPB; base < rows; base += static_cast<long long>(gridDim.x) * RPB) {
+  const long long step = static_cast<long long>(gridDim.x) * RPB, start = static_cast<long long>(blockIdx.x) * RPB + sub;
+  auto place = [&](int stage, int tensor, int i) { return s_ring + ((stage * tensors + tensor) * VPL + i) * THREADS + threadIdx.x; };
+  auto copy = [&](const T* from, long long ld, long long row, int stage, int tensor) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (M::col(i, 0, t) < d)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(place(stage, tensor, i))),
+                     "l"(from + row * ld + M::col(i, 0, t)) : "memory");
+  };
+  auto fetch = [&](long long row, int stage) {            // one group for each row, an empty one behind the last
+    if (VEC && row < rows) {
+      copy(dy, ldy, row, stage, 0);
+      copy(x, ldx, row, stage, 1);
+      if (dres != nullptr) copy(dres, ldr, row, stage, 2);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  if constexpr (VEC) {
+#pragma unroll
+    for (int n = 0; n < STAGES - 1; ++n) fetch(start + n * step, n);
+  }
+  int turn = 0, stage = 0;
+  float2 st = stats[start < rows ? start : 0];
+  for (long long base = static_cast<long long>(blockIdx.x) * RPB; base < rows; base += step) {
     const long long row = base + sub;
     const int width = row < rows ? d : 0;
     const long long at = row < rows ? row : 0;
-    const float2 st = stats[at];
+    const float2 next_st = stats[row + step < rows ? row + step : 0];
     uint4 rx[VPL], rg[VPL], rr[VPL];
+    if constexpr (VEC) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      rg[i] = M::load(dy + at * ldy, i, t, width);
-      rx[i] = M::load(x + at * ldx, i, t, width);
-      if (dres != nullptr) rr[i] = M::load(dres + at * ldr, i, t, width);
+      for (int i = 0; i < VPL; ++i) {
+        const bool here = M::col(i, 0, t) < width;
+        rg[i] = here ? *place(stage, 0, i) : make_uint4(0, 0, 0, 0);
+        rx[i] = here ? *place(stage, 1, i) : make_uint4(0, 0, 0, 0);
+        if (dres != nullptr) rr[i] = here ? *place(stage, 2, i) : make_uint4(0, 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        rg[i] = M::load(dy + at * ldy, i, t, width);
+        rx[i] = M::load(x + at * ldx, i, t, width);
+        if (dres != nullptr) rr[i] = M::load(dres + at * ldr, i, t, width);
+      }
     }
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
@@ -231,6 +274,10 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
         s1 += g[j];
         s2 += g[j] * xh[j];
       }
+    }
+    if constexpr (VEC) {                                  // into the place of the row before, which was used a row ago
+      fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
     }
     const float2 sums = row_sum2<TPR>(s1, s2, scratch[turn]);
     turn ^= 1;
@@ -253,7 +300,9 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
       }
       M::store(dx + at * d, o, i, t, width);
     }
+    st = next_st;
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (partial == nullptr) return;
   float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * d;
   if constexpr (RPB > 1) {
@@ -329,24 +378,31 @@ layernorm_bwd_cols_kernel(const T* __restrict__ dy, long long ldy, const T* __re
   mine[d + c] = b;
 }
 
-// Sums of the columns of partial [n, 2d] in a fixed order: 32 columns x 32 groups of rows per block.
+// Sums of the columns of partial [n, 2d] in a fixed order: 8 columns (one sector of 32 bytes) x 128 groups of rows per
+// block, so that even 1024 columns are work for 256 blocks.
 template <typename WT>
 __global__ void __launch_bounds__(1024)
 layernorm_cols_kernel(const float* __restrict__ partial, WT* __restrict__ dw, WT* __restrict__ db, int n, int d) {
-  __shared__ float red[32][33];
+  __shared__ float red[32][9];
   pdl_wait();
   pdl_launch_dependents();
-  const int c = blockIdx.x * 32 + threadIdx.x;
+  const int c = blockIdx.x * 8 + threadIdx.x % 8;
   float s = 0.f;
-  if (c < 2 * d)
-    for (int r = threadIdx.y; r < n; r += 32) s += partial[static_cast<long long>(r) * 2 * d + c];
-  red[threadIdx.y][threadIdx.x] = s;
+  if (c < 2 * d) {
+#pragma unroll 4
+    for (int r = threadIdx.x / 8; r < n; r += 128) s += partial[static_cast<long long>(r) * 2 * d + c];
+  }
+  s += __shfl_xor_sync(0xffffffffu, s, 8);
+  s += __shfl_xor_sync(0xffffffffu, s, 16);
+  if (threadIdx.x % 32 < 8) red[threadIdx.x / 32][threadIdx.x % 8] = s;
   __syncthreads();
-  s = lanes_sum<32>(red[threadIdx.x][threadIdx.y]);       // warp y adds column y's 32 groups
-  const int out = blockIdx.x * 32 + threadIdx.y;
-  if (threadIdx.x == 0 && out < 2 * d) {
-    WT* to = out < d ? dw : db;
-    if (to != nullptr) to[out < d ? out : out - d] = from_f32<WT>(s);
+  if (threadIdx.x < 256) {                                // warp y adds column y's 32 warps
+    s = lanes_sum<32>(red[threadIdx.x % 32][threadIdx.x / 32]);
+    const int out = blockIdx.x * 8 + threadIdx.x / 32;
+    if (threadIdx.x % 32 == 0 && out < 2 * d) {
+      WT* to = out < d ? dw : db;
+      if (to != nullptr) to[out < d ? out : out - d] = from_f32<WT>(s);
+    }
   }
 }
 
@@ -398,15 +454,27 @@ int fwd_run(const void* x, long long ldx, const void* delta, long long ldd, cons
   return e == cudaSuccess ? 0 : -3;
 }
 
+// Opts a kernel in to 100 KB of shared memory (beyond 48 KB with the static part; the call costs a tenth of a microsecond).
+inline bool more_shared(const void* kernel) {
+  return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024) == cudaSuccess;
+}
+
 template <typename T, typename WT, bool VEC>
 cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, const WT* w, const float2* stats, const T* dres,
                        long long ldr, T* dx, float* partial, long long rows, int d, int nblocks, cudaStream_t stream) {
   const int chunks = (d + Vec16<T>::N - 1) / Vec16<T>::N;
   const float inv_d = 1.f / static_cast<float>(d);
 #define FMB_LN_BWD(TPR, VPL)                                                                                             \
-  return launch_pdl(layernorm_bwd_kernel<T, WT, TPR, VPL, VEC>, dim3(nblocks), dim3(TPR > 256 ? TPR : 256),              \
-                    TPR < 256 && partial != nullptr ? 2 * d * sizeof(float) : 0, stream, dy, ldy, x, ldx, w, stats, dres, ldr, \
-                    dx, partial, rows, d, inv_d)
+  do {                                                                                                                   \
+    constexpr int THREADS = TPR > 256 ? TPR : 256;                                                                       \
+    const size_t ring = VEC ? sizeof(uint4) * BwdStages<VPL>::N * (dres != nullptr ? 3 : 2) * VPL * THREADS : 0;         \
+    const size_t fold = TPR < 256 && partial != nullptr ? 2 * d * sizeof(float) : 0;                                     \
+    const size_t smem = ring > fold ? ring : fold;                                                                       \
+    auto kernel = layernorm_bwd_kernel<T, WT, TPR, VPL, VEC>;                                                            \
+    if (smem > 46 * 1024 && !more_shared(reinterpret_cast<const void*>(kernel))) return cudaErrorInvalidValue;           \
+    return launch_pdl(kernel, dim3(nblocks), dim3(THREADS), smem, stream, dy, ldy, x, ldx, w, stats, dres, ldr, dx,      \
+                      partial, rows, d, inv_d);                                                                          \
+  } while (0)
   if (chunks <= 32) FMB_LN_BWD(32, 1);
   if (chunks <= 64) FMB_LN_BWD(64, 1);
   if (chunks <= 128) FMB_LN_BWD(128, 1);
@@ -435,7 +503,7 @@ int bwd_run(const void* dy, long long ldy, const void* x, long long ldx, const v
   cudaError_t e = vec ? bwd_launch<T, WT, true>(gp, ldy, xp, ldx, wp, st, rp, ldr, op, partial, rows, d, nblocks, stream)
                       : bwd_launch<T, WT, false>(gp, ldy, xp, ldx, wp, st, rp, ldr, op, partial, rows, d, nblocks, stream);
   if (e == cudaSuccess && partial != nullptr)
-    e = launch_pdl(layernorm_cols_kernel<WT>, dim3((2 * d + 31) / 32), dim3(32, 32), 0, stream, partial, static_cast<WT*>(dw),
+    e = launch_pdl(layernorm_cols_kernel<WT>, dim3((2 * d + 7) / 8), dim3(1024), 0, stream, partial, static_cast<WT*>(dw),
                    static_cast<WT*>(db), nblocks, d);
   return e == cudaSuccess ? 0 : -3;
 }

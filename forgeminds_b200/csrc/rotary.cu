@@ -30,7 +30,9 @@ struct RotaryParams {
   float sign;
 };
 
-// One item: unit `u` of a token (a vector of VEC pairs, or a vector of VEC copied values) in `per_group` heads.
+constexpr int BATCH = 4;
+
+// One item: unit `u` of a token (VEC pairs, or two vectors of VEC copied values) in `per_group` heads.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
   pdl_wait();
@@ -69,47 +71,76 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
       for (int j = 0; j < VEC; ++j) s[j] *= p.sign;
     }
   }
-  // where the two vectors of pairs, or the one that is copied, lie in a head
-  const int first = turn ? (INTER ? 2 * VEC * unit : VEC * unit) : p.R + VEC * (unit - p.rot_units);
-  const int second = INTER ? first + VEC : first + p.R / 2;
+  // where the two vectors of pairs, or the two that are copied (the second may not be there), lie in a head
+  const int first = turn ? (INTER ? 2 * VEC * unit : VEC * unit) : p.R + 2 * VEC * (unit - p.rot_units);
+  const int second = INTER || !turn ? first + VEC : first + p.R / 2;
+  const bool two = turn || second < p.D;
   const int h_end = min((group + 1) * p.per_group, p.q.heads + p.k.heads);
-#pragma unroll 4
-  for (int h = group * p.per_group; h < h_end; ++h) {
+  auto place = [&](int h, const T*& src, T*& dst) {
     const bool is_k = h >= p.q.heads;
     const RotaryTensor& x = is_k ? p.k : p.q;
     const int hh = is_k ? h - p.q.heads : h;
-    const T* src = static_cast<const T*>(x.src) + b * x.sb + t * x.st + hh * x.sh;
-    T* dst = static_cast<T*>(x.dst) + (static_cast<long long>(token) * x.heads + hh) * p.D;
-    if constexpr (VEC == Vec16<T>::N) {
-      const uint4 ra = *reinterpret_cast<const uint4*>(src + first);
-      if (!turn) { *reinterpret_cast<uint4*>(dst + first) = ra; continue; }
-      const uint4 rb = *reinterpret_cast<const uint4*>(src + second);
-      float x0[VEC], x1[VEC], y0[VEC], y1[VEC];
-      Vec16<T>::unpack(ra, x0);
-      Vec16<T>::unpack(rb, x1);
-      if constexpr (INTER) {
+    src = static_cast<const T*>(x.src) + b * x.sb + t * x.st + hh * x.sh;
+    dst = static_cast<T*>(x.dst) + (static_cast<long long>(token) * x.heads + hh) * p.D;
+  };
+  if constexpr (VEC == Vec16<T>::N) {
+    // BATCH heads are loaded before the first of them is stored: a thread has 128 bytes on their way
+    for (int h = group * p.per_group; h < h_end; h += BATCH) {
+      uint4 ra[BATCH], rb[BATCH];
+      T* dst[BATCH];
 #pragma unroll
-        for (int j = 0; j < VEC / 2; ++j) {
-          y0[2 * j] = x0[2 * j] * c[j] - x0[2 * j + 1] * s[j];
-          y0[2 * j + 1] = x0[2 * j] * s[j] + x0[2 * j + 1] * c[j];
-          y1[2 * j] = x1[2 * j] * c[VEC / 2 + j] - x1[2 * j + 1] * s[VEC / 2 + j];
-          y1[2 * j + 1] = x1[2 * j] * s[VEC / 2 + j] + x1[2 * j + 1] * c[VEC / 2 + j];
+      for (int i = 0; i < BATCH; ++i)
+        if (h + i < h_end) {
+          const T* src;
+          place(h + i, src, dst[i]);
+          ra[i] = *reinterpret_cast<const uint4*>(src + first);
+          if (two) rb[i] = *reinterpret_cast<const uint4*>(src + second);
         }
-      } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          y0[j] = x0[j] * c[j] - x1[j] * s[j];
-          y1[j] = x0[j] * s[j] + x1[j] * c[j];
+      for (int i = 0; i < BATCH; ++i) {
+        if (h + i >= h_end) break;
+        if (turn) {
+          float x0[VEC], x1[VEC], y0[VEC], y1[VEC];
+          Vec16<T>::unpack(ra[i], x0);
+          Vec16<T>::unpack(rb[i], x1);
+          if constexpr (INTER) {
+#pragma unroll
+            for (int j = 0; j < VEC / 2; ++j) {
+              y0[2 * j] = x0[2 * j] * c[j] - x0[2 * j + 1] * s[j];
+              y0[2 * j + 1] = x0[2 * j] * s[j] + x0[2 * j + 1] * c[j];
+              y1[2 * j] = x1[2 * j] * c[VEC / 2 + j] - x1[2 * j + 1] * s[VEC / 2 + j];
+              y1[2 * j + 1] = x1[2 * j] * s[VEC / 2 + j] + x1[2 * j + 1] * c[VEC / 2 + j];
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+              y0[j] = x0[j] * c[j] - x1[j] * s[j];
+              y1[j] = x0[j] * s[j] + x1[j] * c[j];
+            }
+          }
+          ra[i] = Vec16<T>::pack(y0);
+          rb[i] = Vec16<T>::pack(y1);
         }
+        *reinterpret_cast<uint4*>(dst[i] + first) = ra[i];
+        if (two) *reinterpret_cast<uint4*>(dst[i] + second) = rb[i];
       }
-      *reinterpret_cast<uint4*>(dst + first) = Vec16<T>::pack(y0);
-      *reinterpret_cast<uint4*>(dst + second) = Vec16<T>::pack(y1);
-    } else {
-      static_assert(VEC == 1, "single values otherwise");
-      if (!turn) { dst[first] = src[first]; continue; }
-      const float a = to_f32(src[first]), e = to_f32(src[second]);
-      dst[first] = from_f32<T>(a * c[0] - e * s[0]);
-      dst[second] = from_f32<T>(a * s[0] + e * c[0]);
+    }
+  } else {
+    static_assert(VEC == 1, "single values otherwise");
+#pragma unroll 2
+    for (int h = group * p.per_group; h < h_end; ++h) {
+      const T* src;
+      T* dst;
+      place(h, src, dst);
+      const T va = src[first], vb = two ? src[second] : va;
+      if (turn) {
+        const float a = to_f32(va), e = to_f32(vb);
+        dst[first] = from_f32<T>(a * c[0] - e * s[0]);
+        dst[second] = from_f32<T>(a * s[0] + e * c[0]);
+      } else {
+        dst[first] = va;
+        if (two) dst[second] = vb;
+      }
     }
   }
 }
@@ -118,7 +149,7 @@ template <typename T, bool INTER>
 cudaError_t rotary_launch(RotaryParams p, bool vec, cudaStream_t stream) {
   const int n = vec ? Vec16<T>::N : 1, heads = p.q.heads + p.k.heads;
   p.rot_units = p.R / 2 / n;
-  p.units = p.rot_units + (p.D - p.R) / n;
+  p.units = p.rot_units + ((p.D - p.R) / n + 1) / 2;
   // Few tokens: a thread per head, for latency. Many: up to eight heads per thread, for the tables' sake.
   const long long lanes = static_cast<long long>(p.tokens) * p.units;
   const long long room = static_cast<long long>(sm_count()) * 2048;
