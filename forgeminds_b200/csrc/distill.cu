@@ -280,34 +280,6 @@ template <typename T> struct KlRow {
   __device__ __forceinline__ int single(int t) const { return t < head ? t : nv * N + t; }       // of thread t
 };
 
-// two fp32 values in one register pair, and the instructions that take both at once
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float lo, float hi) {
-  F2 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ float2 f2_parts(F2 v) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
-  return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-  F2 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-  F2 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 m = __hmax2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
   return *reinterpret_cast<const uint32_t*>(&m);
@@ -438,24 +410,24 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     load_slot(next);
     // sums: exponentials of the student, e = exp(t - ref) of the teacher, and e (t - ref - x / tau) where x is held here
     const float mc = m == -CUDART_INF_F ? 0.f : m * c;
-    F2 sums = 0;
+    F2 sums = f2(0.f, 0.f);
     {
       const F2 mc2 = f2(-mc, -mc);
-      F2 more = 0;
+      F2 more = f2(0.f, 0.f);
 #pragma unroll 2
       for (int i = threadIdx.x; i < n; i += THREADS) {
         float f[N];
         Vec16<T>::unpack(s_row[i], f);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
-          const float2 o = f2_parts(f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, mc2));
+          const float2 o = (f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, mc2));
           if (j % 2) more = f2_add(more, f2(exp2_unit(o.x), exp2_unit(o.y)));
           else sums = f2_add(sums, f2(exp2_unit(o.x), exp2_unit(o.y)));
         }
       }
       sums = f2_add(sums, more);
     }
-    float s = f2_parts(sums).x + f2_parts(sums).y + exp2_unit(fmaf(single, c, -mc)), e = 0.f, a = 0.f, xk = 0.f;
+    float s = sums.x + sums.y + exp2_unit(fmaf(single, c, -mc)), e = 0.f, a = 0.f, xk = 0.f;
     bool mine = false, twice = false;                      // whether the student's logit at the index is held here
     int mark = -1;
     if (at >= 0) {
@@ -533,8 +505,8 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
           Vec16<T>::unpack(s_row[i], f);
 #pragma unroll
           for (int j = 0; j < H; ++j) {
-            float2 o = f2_parts(f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, gmc2));
-            o = f2_parts(f2_mul(f2(exp2_unit(o.x), exp2_unit(o.y)), by2));
+            float2 o = (f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, gmc2));
+            o = (f2_mul(f2(exp2_unit(o.x), exp2_unit(o.y)), by2));
             f[2 * j] = o.x;
             f[2 * j + 1] = o.y;
           }

@@ -14,8 +14,8 @@ namespace fmb {
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
-// Rows of a block's ring in the backward pass: 512 threads with two chunks of three tensors are 48 KB each.
-template <int VPL> struct BwdStages { static constexpr int N = VPL == 1 ? 3 : 2; };
+// Rows of a block's ring in the backward pass: 1024 chunks of three tensors are 48 KB each.
+template <int CHUNKS> struct BwdStages { static constexpr int N = CHUNKS <= 512 ? 3 : 2; };
 
 // How a thread of a row's TPR threads sees it: chunk i of N values. VEC: 16 contiguous bytes; otherwise N single
 // values TPR apart (widths, pitches or addresses that are no multiple of 16 bytes), still coalesced.
@@ -190,15 +190,18 @@ layernorm_fwd_wide_kernel(const T* __restrict__ x, long long ldx, const T* __res
 // Blocks walk over the rows. A thread keeps its columns' sums of dy xh and dy in registers; a block leaves them as
 // one row of `partial` [blocks, 2, d], which the column kernel below adds in a fixed order. With 16-byte chunks the rows
 // come through a ring of shared memory, copied STAGES - 1 rows ahead, each thread its own chunks (no barrier guards them):
-// with loads into registers a block waited out the memory's latency at every row.
+// with loads into registers a block waited out the memory's latency at every row. Two chunks per thread from 65 on: what a
+// row costs beside its columns (two sums over its threads, statistics, addresses) is as much as 130 instructions a thread.
+// dx, dw and db of bf16 rows with dres, the column sums included: 16384 x 4096 in 96 us (5.6 TB/s; with one chunk per
+// thread 112, from registers 125), 65536 x 1024 in 88 us (6.1 TB/s; one chunk 96).
 template <typename T, typename WT, int TPR, int VPL, bool VEC>
-__global__ void __launch_bounds__(TPR > 256 ? TPR : 256)
+__global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : VPL > 1 ? 2 : 4)
 layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
                      const WT* __restrict__ w, const float2* __restrict__ stats, const T* __restrict__ dres, long long ldr,
                      T* __restrict__ dx, float* __restrict__ partial, long long rows, int d, float inv_d) {
   using M = RowMap<T, TPR, VEC>;
   constexpr int N = M::N, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
-  constexpr int STAGES = BwdStages<VPL>::N;
+  constexpr int STAGES = BwdStages<VPL * THREADS>::N;
   __shared__ float2 scratch[2][THREADS / 32];
   extern __shared__ uint4 s_ring[];                       // [stage][dy, x, dres][chunk][thread]; the fold below takes its place
   float* s_fold = reinterpret_cast<float*>(s_ring);       // [2, d], when several rows share a block
@@ -206,100 +209,118 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
   pdl_launch_dependents();
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int tensors = dres != nullptr ? 3 : 2;
-  float wv[VPL][N], dwa[VPL][N], dba[VPL][N];
+  constexpr int H = N / 2;
+  F2 wv[VPL][H], dwa[VPL][H], dba[VPL][H];
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
-    M::weights(w, wv[i], i, t, d, 1.f);
+    float f[N];
+    M::weights(w, f, i, t, d, 1.f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) { dwa[i][j] = 0.f; dba[i][j] = 0.f; }
+    for (int j = 0; j < H; ++j) { wv[i][j] = f2(f[2 * j], f[2 * j + 1]); dwa[i][j] = dba[i][j] = f2(0.f, 0.f); }
   }
-  const long long step = static_cast<long long>(gridDim.x) * RPB, start = static_cast<long long>(blockIdx.x) * RPB + sub;
-  auto place = [&](int stage, int tensor, int i) { return s_ring + ((stage * tensors + tensor) * VPL + i) * THREADS + threadIdx.x; };
-  auto copy = [&](const T* from, long long ld, long long row, int stage, int tensor) {
+  // Everything a row needs moves on by one step: pointers, not products, and rows in 31 bits.
+  const int n_rows = static_cast<int>(rows), step = gridDim.x * RPB, start = blockIdx.x * RPB + sub;
+  const int row_bytes = tensors * VPL * THREADS * 16;
+  const char* ring = reinterpret_cast<const char*>(s_ring + threadIdx.x);
+  const uint32_t ring_at = smem_at(ring);
+  const long long step_dy = step * ldy, step_x = step * ldx, step_res = step * ldr, step_out = static_cast<long long>(step) * d;
+  const int own = VEC ? M::col(0, 0, t) : 0;              // this thread's first column, where its chunks are contiguous
+  const T *next_dy = dy + start * ldy + own, *next_x = x + start * ldx + own, *next_res = dres + start * ldr + own;
+  T* out = dx + static_cast<long long>(start) * d;
+  int next_row = start;
+  int put = 0, get = 0;                                   // bytes from the ring's start
+  auto copy = [&](const T* from, int tensor) {
 #pragma unroll
     for (int i = 0; i < VPL; ++i)
       if (M::col(i, 0, t) < d)
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(place(stage, tensor, i))),
-                     "l"(from + row * ld + M::col(i, 0, t)) : "memory");
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring_at + put + (tensor * VPL + i) * THREADS * 16),
+                     "l"(from + i * TPR * N) : "memory");
   };
-  auto fetch = [&](long long row, int stage) {            // one group for each row, an empty one behind the last
-    if (VEC && row < rows) {
-      copy(dy, ldy, row, stage, 0);
-      copy(x, ldx, row, stage, 1);
-      if (dres != nullptr) copy(dres, ldr, row, stage, 2);
+  auto fetch = [&]() {                                    // one group for each row, an empty one behind the last
+    if (next_row < n_rows) {
+      copy(next_dy, 0);
+      copy(next_x, 1);
+      if (dres != nullptr) copy(next_res, 2);
+      next_dy += step_dy;
+      next_x += step_x;
+      next_res += step_res;
+      next_row += step;                                   // stays within 31 bits: it was below the number of rows
     }
+    put = put == (STAGES - 1) * row_bytes ? 0 : put + row_bytes;
     asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto held = [&](int tensor, int i) { return *reinterpret_cast<const uint4*>(ring + get + (tensor * VPL + i) * THREADS * 16); };
+  auto pairs = [](const uint4& u, F2 (&v)[H]) {
+    float f[N];
+    Vec16<T>::unpack(u, f);
+#pragma unroll
+    for (int j = 0; j < H; ++j) v[j] = f2(f[2 * j], f[2 * j + 1]);
   };
   if constexpr (VEC) {
 #pragma unroll
-    for (int n = 0; n < STAGES - 1; ++n) fetch(start + n * step, n);
+    for (int n = 0; n < STAGES - 1; ++n) fetch();
   }
-  int turn = 0, stage = 0;
-  float2 st = stats[start < rows ? start : 0];
-  for (long long base = static_cast<long long>(blockIdx.x) * RPB; base < rows; base += step) {
-    const long long row = base + sub;
-    const int width = row < rows ? d : 0;
-    const long long at = row < rows ? row : 0;
-    const float2 next_st = stats[row + step < rows ? row + step : 0];
-    uint4 rx[VPL], rg[VPL], rr[VPL];
-    if constexpr (VEC) {
-      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+  int turn = 0;
+  float2 st = stats[min(start, n_rows - 1)];
+  for (int base = blockIdx.x * RPB; base < n_rows; base += step, out += step_out) {
+    const int row = base + sub;
+    const int width = RPB == 1 || row < n_rows ? d : 0;   // rows beyond the last take part in the sums with nothing
+    const float2 next_st = stats[min(row + step, n_rows - 1)];
+    const F2 mean2 = f2(-st.x, -st.x), r2 = f2(st.y, st.y);
+    if constexpr (VEC) asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory");
+    F2 s1 = f2(0.f, 0.f), s2 = s1;
+    uint4 rg[VEC ? 1 : VPL], rx[VEC ? 1 : VPL], rr[VEC ? 1 : VPL];
+    if constexpr (!VEC) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i) {
-        const bool here = M::col(i, 0, t) < width;
-        rg[i] = here ? *place(stage, 0, i) : make_uint4(0, 0, 0, 0);
-        rx[i] = here ? *place(stage, 1, i) : make_uint4(0, 0, 0, 0);
-        if (dres != nullptr) rr[i] = here ? *place(stage, 2, i) : make_uint4(0, 0, 0, 0);
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        rg[i] = M::load(dy + at * ldy, i, t, width);
-        rx[i] = M::load(x + at * ldx, i, t, width);
-        if (dres != nullptr) rr[i] = M::load(dres + at * ldr, i, t, width);
+        rg[i] = M::load(dy + row * ldy, i, t, width);
+        rx[i] = M::load(x + row * ldx, i, t, width);
+        if (dres != nullptr) rr[i] = M::load(dres + row * ldr, i, t, width);
       }
     }
-    float s1 = 0.f, s2 = 0.f;
+    // both halves of the row's work take the chunk from the ring: held in registers it would cost the second block of an SM
+    auto take = [&](int tensor, int i) {
+      if constexpr (VEC) return M::col(i, 0, t) < width ? held(tensor, i) : make_uint4(0, 0, 0, 0);
+      else return tensor == 0 ? rg[i] : tensor == 1 ? rx[i] : rr[i];
+    };
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      float g[N], xh[N];
-      Vec16<T>::unpack(rg[i], g);
-      Vec16<T>::unpack(rx[i], xh);
+      F2 g[H], xh[H];
+      pairs(take(0, i), g);
+      pairs(take(1, i), xh);
 #pragma unroll
-      for (int j = 0; j < N; ++j) {                       // where there is no column dy is 0 and nothing is added
-        xh[j] = (xh[j] - st.x) * st.y;
-        dwa[i][j] += g[j] * xh[j];
-        dba[i][j] += g[j];
-        g[j] *= wv[i][j];
-        s1 += g[j];
-        s2 += g[j] * xh[j];
+      for (int j = 0; j < H; ++j) {                       // where there is no column dy is 0 and nothing is added
+        xh[j] = f2_mul(f2_add(xh[j], mean2), r2);
+        dwa[i][j] = f2_fma(g[j], xh[j], dwa[i][j]);
+        dba[i][j] = f2_add(dba[i][j], g[j]);
+        g[j] = f2_mul(g[j], wv[i][j]);
+        s1 = f2_add(s1, g[j]);
+        s2 = f2_fma(g[j], xh[j], s2);
       }
     }
-    if constexpr (VEC) {                                  // into the place of the row before, which was used a row ago
-      fetch(row + (STAGES - 1) * step, stage == 0 ? STAGES - 1 : stage - 1);
-      stage = stage + 1 == STAGES ? 0 : stage + 1;
-    }
-    const float2 sums = row_sum2<TPR>(s1, s2, scratch[turn]);
+    if constexpr (VEC) fetch();                           // into the place of the row before
+    
+    const float2 sums = row_sum2<TPR>(s1.x + s1.y, s2.x + s2.y, scratch[turn]);
     turn ^= 1;
-    const float c1 = sums.x * inv_d, c2 = sums.y * inv_d;
+    const F2 c1 = f2(-sums.x * inv_d, -sums.x * inv_d), c2 = f2(-sums.y * inv_d, -sums.y * inv_d);
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
-      float g[N], xh[N], o[N];
-      Vec16<T>::unpack(rg[i], g);
-      Vec16<T>::unpack(rx[i], xh);
+      F2 g[H], xh[H], add[H];
+      pairs(take(0, i), g);
+      pairs(take(1, i), xh);
+      if (dres != nullptr) pairs(take(2, i), add);
+      float o[N];
 #pragma unroll
-      for (int j = 0; j < N; ++j) {
-        xh[j] = (xh[j] - st.x) * st.y;
-        o[j] = st.y * (g[j] * wv[i][j] - c1 - xh[j] * c2);
+      for (int j = 0; j < H; ++j) {
+        xh[j] = f2_mul(f2_add(xh[j], mean2), r2);
+        const F2 inner = f2_add(f2_fma(xh[j], c2, f2_mul(g[j], wv[i][j])), c1);
+        const float2 v = (dres != nullptr ? f2_fma(inner, r2, add[j]) : f2_mul(inner, r2));
+        o[2 * j] = v.x;
+        o[2 * j + 1] = v.y;
       }
-      if (dres != nullptr) {
-        float e[N];
-        Vec16<T>::unpack(rr[i], e);
-#pragma unroll
-        for (int j = 0; j < N; ++j) o[j] += e[j];
-      }
-      M::store(dx + at * d, o, i, t, width);
+      M::store(out, o, i, t, width);
     }
+    if constexpr (VEC) get = get == (STAGES - 1) * row_bytes ? 0 : get + row_bytes;
     st = next_st;
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
@@ -314,9 +335,10 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
 #pragma unroll
           for (int j = 0; j < N; ++j) {
             const int c = M::col(i, j, t);
+            const float2 a = dwa[i][j / 2], b = dba[i][j / 2];
             if (c < d) {
-              s_fold[c] = (who ? s_fold[c] : 0.f) + dwa[i][j];
-              s_fold[d + c] = (who ? s_fold[d + c] : 0.f) + dba[i][j];
+              s_fold[c] = (who ? s_fold[c] : 0.f) + (j % 2 ? a.y : a.x);
+              s_fold[d + c] = (who ? s_fold[d + c] : 0.f) + (j % 2 ? b.y : b.x);
             }
           }
       }
@@ -329,7 +351,11 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const int c = M::col(i, j, t);
-        if (c < d) { mine[c] = dwa[i][j]; mine[d + c] = dba[i][j]; }
+        const float2 a = dwa[i][j / 2], b = dba[i][j / 2];
+        if (c < d) {
+          mine[c] = j % 2 ? a.y : a.x;
+          mine[d + c] = j % 2 ? b.y : b.x;
+        }
       }
   }
 }
@@ -467,7 +493,7 @@ cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, co
 #define FMB_LN_BWD(TPR, VPL)                                                                                             \
   do {                                                                                                                   \
     constexpr int THREADS = TPR > 256 ? TPR : 256;                                                                       \
-    const size_t ring = VEC ? sizeof(uint4) * BwdStages<VPL>::N * (dres != nullptr ? 3 : 2) * VPL * THREADS : 0;         \
+    const size_t ring = VEC ? sizeof(uint4) * BwdStages<VPL * THREADS>::N * (dres != nullptr ? 3 : 2) * VPL * THREADS : 0;         \
     const size_t fold = TPR < 256 && partial != nullptr ? 2 * d * sizeof(float) : 0;                                     \
     const size_t smem = ring > fold ? ring : fold;                                                                       \
     auto kernel = layernorm_bwd_kernel<T, WT, TPR, VPL, VEC>;                                                            \
@@ -477,9 +503,9 @@ cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, co
   } while (0)
   if (chunks <= 32) FMB_LN_BWD(32, 1);
   if (chunks <= 64) FMB_LN_BWD(64, 1);
-  if (chunks <= 128) FMB_LN_BWD(128, 1);
-  if (chunks <= 256) FMB_LN_BWD(256, 1);
-  if (chunks <= 512) FMB_LN_BWD(512, 1);
+  if (chunks <= 128) FMB_LN_BWD(64, 2);
+  if (chunks <= 256) FMB_LN_BWD(128, 2);
+  if (chunks <= 512) FMB_LN_BWD(256, 2);
   if (chunks <= BWD_CHUNKS) FMB_LN_BWD(512, 2);
 #undef FMB_LN_BWD
   layernorm_bwd_wide_kernel<T, WT><<<static_cast<unsigned>(rows), 1024, 0, stream>>>(dy, ldy, x, ldx, w, stats, dres, ldr, dx,
@@ -530,9 +556,9 @@ extern "C" int fmb_layernorm_bwd_blocks(long long rows, int d, int dtype) {
   const int n = dtype == FMB_BF16 ? 8 : 4;
   const int chunks = (d + n - 1) / n;
   if (chunks > BWD_CHUNKS) return static_cast<int>(rows < 32 ? (rows < 1 ? 1 : rows) : 32);
-  const int per_row = chunks <= 32 ? 32 : chunks <= 64 ? 64 : chunks <= 128 ? 128 : 256;
+  const int per_row = chunks <= 32 ? 32 : chunks <= 128 ? 64 : chunks <= 256 ? 128 : 256;
   const long long need = (rows + 256 / per_row - 1) / (256 / per_row);
-  const long long most = static_cast<long long>(sm_count()) * (chunks <= 256 ? 4 : 2);
+  const long long most = static_cast<long long>(sm_count()) * (chunks <= 64 ? 4 : chunks <= 512 ? 2 : 1);      // as many as are resident
   return static_cast<int>(need < 1 ? 1 : need < most ? need : most);
 }
 
@@ -540,7 +566,7 @@ extern "C" int fmb_layernorm_bwd(const void* dy, long long ldy, const void* x, l
                                  const void* dres, long long ldr, void* dx, float* partial, void* dw, void* db, long long rows,
                                  int d, int dtype, int w_dtype, int nblocks, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (d <= 0 || rows > 0x7fffffffLL || nblocks < 1) return -2;
+  if (d <= 0 || rows > 0x7fff0000LL || nblocks < 1) return -2;      // steps over the rows stay within 31 bits
   if (dtype == FMB_BF16 && w_dtype == FMB_BF16)
     return bwd_run<__nv_bfloat16, __nv_bfloat16>(dy, ldy, x, ldx, w, stats, dres, ldr, dx, partial, dw, db, rows, d, nblocks, stream);
   if (dtype == FMB_BF16 && w_dtype == FMB_F32)

@@ -85,6 +85,13 @@ __device__ __forceinline__ float exp2_unit(float x) {
   return y;
 }
 
+// two fp32 values in one register pair, for the instructions that take both at once
+using F2 = float2;
+__device__ __forceinline__ F2 f2(float lo, float hi) { return make_float2(lo, hi); }
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) { return __ffma2_rn(a, b, c); }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) { return __fadd2_rn(a, b); }
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) { return __fmul2_rn(a, b); }
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 // SMs of the current device (asked once per device)

@@ -301,8 +301,11 @@ def _check_layer_norm(name: str, x, w, b) -> None:
     _one_device(name, x, w, b)
 
 
+_MOST_ROWS = 2 ** 31 - 2 ** 16        # rows that the kernels number in 31 bits
+
+
 def _ln_fast(x, *rest) -> bool:
-    return x.shape[-1] <= 2 ** 24 and x.numel() // x.shape[-1] < 2 ** 31 and fast_ok(x, *rest)
+    return x.shape[-1] <= 2 ** 24 and x.numel() // x.shape[-1] < _MOST_ROWS and fast_ok(x, *rest)
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor | None = None, b: torch.Tensor | None = None,
@@ -556,7 +559,7 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
         _one_device("route_experts", logits, bias)
         bias = bias.detach()
     args = (n_groups, top_groups, group_best, bool(renormalise), float(scale), float(aux_coef), float(z_coef))
-    if E <= ROUTE_MAX_EXPERTS and k <= ROUTE_MAX_K and n_groups <= ROUTE_MAX_GROUPS and logits.shape[0] * k < 2 ** 31 \
+    if E <= ROUTE_MAX_EXPERTS and k <= ROUTE_MAX_K and n_groups <= ROUTE_MAX_GROUPS and logits.shape[0] * k < _MOST_ROWS \
             and fast_ok(logits):
         if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
             bias = bias.to(torch.float32).contiguous()
