@@ -16,16 +16,22 @@
 namespace fmb {
 
 constexpr int KL_THREADS = 512;
+constexpr int KL_COUNT_BLOCKS = 256;
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <typename TT> __device__ __forceinline__ bool slot_counts(long long at, TT value, int V) {
   return at >= 0 && at < V && !(to_f32(value) == -CUDART_INF_F);
 }
 
+// Scratch of a forward pass: rows that count, the ticket, rows given out, then the blocks' parts of the count. Nothing has to
+// be cleared before the count kernel, which leaves one part per block and clears the two counters.
+constexpr int WS_COUNT = 0, WS_TICKET = 1, WS_TAKEN = 2, WS_PARTS = 4;
+static_assert(WS_PARTS + KL_COUNT_BLOCKS == FMB_KL_SCRATCH, "the caller's scratch");
+
 // Rows that have a slot that counts. One warp per row.
 template <typename TT>
 __global__ void __launch_bounds__(256)
-kl_topk_count_kernel(const TT* __restrict__ values, const long long* __restrict__ index, int* __restrict__ count,
+kl_topk_count_kernel(const TT* __restrict__ values, const long long* __restrict__ index, int* __restrict__ ws,
                      long long rows, int V, int K) {
   __shared__ int s_n;
   if (threadIdx.x == 0) s_n = 0;
@@ -41,7 +47,10 @@ kl_topk_count_kernel(const TT* __restrict__ values, const long long* __restrict_
   }
   if (lane == 0 && n) atomicAdd(&s_n, n);
   __syncthreads();
-  if (threadIdx.x == 0 && s_n) atomicAdd(count, s_n);      // whole numbers: the order does not matter
+  if (threadIdx.x == 0) {
+    ws[WS_PARTS + blockIdx.x] = s_n;
+    if (blockIdx.x == 0) ws[WS_TICKET] = ws[WS_TAKEN] = 0;
+  }
 }
 
 struct KlParams {
@@ -55,6 +64,8 @@ struct KlParams {
   void* grad;                      // [rows, V] contiguous (its pitch is ldg), or null
   long long ldg;
   const int* count;                // rows that count (mean), or null
+  int* parts;                      // scratch whose parts the count is the sum of, and where it is then left; or null
+  int n_parts;
   int* ticket;                     // 0 before the launch; the block that makes it `blocks` adds the rows' losses
   int* taken;                      // 0 before the launch: rows that have been given out
   float* loss;                     // the sum (mean) of row_loss, or null
@@ -80,6 +91,21 @@ __device__ __forceinline__ float block_max(float v, float* scratch) {
   __syncthreads();
   v = (threadIdx.x & 31) < (blockDim.x >> 5) ? scratch[threadIdx.x & 31] : -CUDART_INF_F;
   return lanes_max<32>(v);
+}
+
+// What the losses are divided by: 1, the count that is given, or the sum of the parts, which every block takes and leaves
+// beside them for the backward pass.
+__device__ __forceinline__ float rows_that_count(const KlParams& p, int* scratch) {
+  if (p.parts == nullptr) return p.count != nullptr ? static_cast<float>(max(*p.count, 1)) : 1.f;
+  int n = 0;
+  for (int i = threadIdx.x; i < p.n_parts; i += blockDim.x) n += p.parts[WS_PARTS + i];
+  n = __reduce_add_sync(0xffffffffu, n);
+  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = n;
+  __syncthreads();
+  n = 0;
+  for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) n += scratch[w];
+  if (threadIdx.x == 0) p.parts[WS_COUNT] = n;
+  return static_cast<float>(max(n, 1));
 }
 
 // Teacher's side of a row into shared memory: index (-1 where a slot does not count), p and log p. Returns sum p.
@@ -158,7 +184,9 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
   int* s_at = reinterpret_cast<int*>(s_logp + p.K);
   float* s_x = reinterpret_cast<float*>(s_at + p.K);
   const float c = LOG2E / p.tau, inv_tau = 1.f / p.tau;
-  const float per_row = p.count != nullptr ? 1.f / static_cast<float>(max(*p.count, 1)) : 1.f;
+  if (!FWD && p.skip_one && !p.upstream_rows && *p.upstream == 1.f) return;
+  __shared__ int s_parts[KL_THREADS / 32];
+  const float per_row = 1.f / rows_that_count(p, s_parts);
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x) {
     float up = 1.f;
     if constexpr (!FWD) {
@@ -321,7 +349,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     }
   };
   const float c = LOG2E / p.tau, inv_tau = 1.f / p.tau;
-  const float scale = (p.count != nullptr ? 1.f / static_cast<float>(max(*p.count, 1)) : 1.f) * inv_tau;
+  const float counted = rows_that_count(p, s_at), scale = inv_tau / counted;
   const int first = rank * per_cta;                        // this CTA's first vector
   const bool slot = threadIdx.x < p.K;
   const F2 c2 = f2(c, c);
@@ -551,7 +579,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
       float v = 0.f;
       for (long long i = threadIdx.x; i < p.rows; i += THREADS) v += __ldcg(p.row_loss + i);
       v = block_sum(v, scratch);
-      if (threadIdx.x == 0) *p.loss = p.count != nullptr ? v / static_cast<float>(max(*p.count, 1)) : v;
+      if (threadIdx.x == 0) *p.loss = v / counted;
     }
   }
 }
@@ -602,22 +630,19 @@ int kl_run(KlParams p, bool fwd, int* ws, bool mean, const int* count, cudaStrea
   const size_t smem = static_cast<size_t>(p.K) * 16;
   cudaError_t e = cudaSuccess;
   if (fwd) {
-    if (cudaMemsetAsync(ws, 0, 3 * sizeof(int), stream) != cudaSuccess) return -3;
-    p.ticket = ws + 1;
-    p.taken = ws + 2;
+    p.ticket = ws + WS_TICKET;
+    p.taken = ws + WS_TAKEN;
   }
-  if (mean) {
-    if (count == nullptr) {
-      count = ws;
-      if (fwd) {
-        const long long blocks = (p.rows + 7) / 8 < 4LL * sm_count() ? (p.rows + 7) / 8 : 4LL * sm_count();
-        e = launch_pdl(kl_topk_count_kernel<TT>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream,
-                       static_cast<const TT*>(p.values), p.index, ws, p.rows, p.V, p.K);
-        if (e != cudaSuccess) return -3;
-      }
-    }
-    p.count = count;
+  if (fwd && mean && count == nullptr) {
+    p.n_parts = static_cast<int>((p.rows + 7) / 8 < KL_COUNT_BLOCKS ? (p.rows + 7) / 8 : KL_COUNT_BLOCKS);
+    p.parts = ws;
+    e = launch_pdl(kl_topk_count_kernel<TT>, dim3(p.n_parts), dim3(256), 0, stream, static_cast<const TT*>(p.values), p.index, ws,
+                   p.rows, p.V, p.K);
+    if (e != cudaSuccess) return -3;
+  } else if (fwd && cudaMemsetAsync(ws, 0, WS_PARTS * sizeof(int), stream) != cudaSuccess) {
+    return -3;
   }
+  if (mean) p.count = count;
   if (fwd) {
     // the fewest CTAs (1, 2, 4 or 8) that hold a row, more while SMs would be left without one
     constexpr int N = Vec16<T>::N, MOST = KL_ROW_BYTES / 16;

@@ -87,6 +87,7 @@ int fmb_sum_f32(const float* x, float* out, long long n, float scale, int accumu
 
 // ---- distillation from a teacher's top logits (distill.cu)
 #define FMB_KL_MAX_KEEP 1024
+#define FMB_KL_SCRATCH 260
 // Row losses, row statistics (float2: maximum, sum of exponentials) and, when given, the gradient for an upstream
 // gradient of 1 (rows `ldg` apart; may be the student itself). values / index [rows, K]; lse [rows] may be null. ws: two
 // ints of scratch, ws[0] receives the number of rows that count when `mean` and no `count` is given. loss (may be null):

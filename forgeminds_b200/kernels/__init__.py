@@ -285,9 +285,10 @@ def _rw():
 
 
 def _one_device(name: str, first: torch.Tensor, *others) -> None:
+    device = first.device
     for t in others:
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name}: tensors on {first.device} and {t.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{name}: tensors on {device} and {t.device}")
 
 
 def _check_layer_norm(name: str, x, w, b) -> None:
@@ -437,15 +438,18 @@ def _kl_topk_args(name, rows_shape, vocab, values, index, temperature, lse):
     if index.dtype not in (torch.int32, torch.int64) or not values.is_floating_point():
         raise ValueError(f"{name}: teacher_values must be floating-point and teacher_index int32 or int64, got {values.dtype} "
                          f"and {index.dtype}")
-    if index.dim() < 1 or index.shape[-1] < 1 or index.shape != values.shape or tuple(index.shape[:-1]) != tuple(rows_shape):
+    shape = index.shape
+    if len(shape) < 1 or shape[-1] < 1 or shape != values.shape or shape[:-1] != rows_shape:
         raise ValueError(f"{name}: teacher_values {tuple(values.shape)} and teacher_index {tuple(index.shape)} for rows "
                          f"{tuple(rows_shape)}")
     if vocab < 1:
         raise ValueError(f"{name}: no logits")
-    K = index.shape[-1]
-    values, index = values.detach().reshape(-1, K), index.reshape(-1, K)
+    if index.dim() != 2:
+        values, index = values.reshape(-1, index.shape[-1]), index.reshape(-1, index.shape[-1])
+    if values.requires_grad:
+        values = values.detach()
     if lse is not None:
-        if tuple(lse.shape) != tuple(rows_shape) or not lse.is_floating_point():
+        if lse.shape != rows_shape or not lse.is_floating_point():
             raise ValueError(f"{name}: teacher_lse {tuple(lse.shape)} {lse.dtype} for rows {tuple(rows_shape)}")
         lse = lse.detach().reshape(-1)
     return values, index, lse
