@@ -24,7 +24,8 @@ import torch
 import torch.nn.functional as F
 
 DEFAULT_OPS = ["rms_norm", "add_rms_norm", "swiglu", "swiglu_split", "qk_norm_rope", "kl_div_logits",
-               "newton_schulz", "topk", "softmax", "gemm", "attention", "cross_entropy"]
+               "newton_schulz", "topk", "softmax", "gemm", "attention", "cross_entropy", "layer_norm", "add_layer_norm",
+               "rotary_qk", "kl_topk_logits", "route_experts"]
 
 
 def _peaks():
@@ -79,6 +80,27 @@ def build_case(op, a, device, dtype):
     if op == "topk":
         x = r(512, a.vocab)
         return (), lambda: torch.topk(x, 64, dim=-1), lambda: K.topk(x, 64), x.numel() * es, 0, False
+    if op in ("layer_norm", "add_layer_norm"):
+        x, d = r(tok, dim).requires_grad_(), r(tok, dim).requires_grad_()
+        w, b = torch.ones(dim, device=device, requires_grad=True), torch.zeros(dim, device=device, requires_grad=True)
+        if op == "layer_norm":
+            return (x, w, b), lambda: F.layer_norm(x, (dim,), w.to(dtype), b.to(dtype)), lambda: K.layer_norm(x, w, b), 2 * tok * dim * es, 0, True
+        return (x, d, w, b), lambda: R.add_layer_norm(x, d, w.to(dtype), b.to(dtype)), lambda: K.add_layer_norm(x, d, w, b), 4 * tok * dim * es, 0, True
+    if op == "rotary_qk":
+        B, T, H, D = a.batch, a.seq, a.heads, a.head_dim
+        q, k = r(B, T, H, D).requires_grad_(), r(B, T, max(1, H // 4), D).requires_grad_()
+        cos, sin = K.rotary_tables(T, D, device=device)
+        return (q, k), lambda: (R.rotary(q, cos, sin), R.rotary(k, cos, sin)), lambda: K.rotary_qk(q, k, cos, sin), \
+            2 * (q.numel() + k.numel()) * es, 0, True
+    if op == "kl_topk_logits":
+        n = min(tok, 4096)
+        s = r(n, a.vocab).requires_grad_()
+        v, i = torch.randn(n, a.vocab, device=device).topk(64, dim=-1)
+        return (s,), lambda: R.kl_topk(s, v, i).mean(), lambda: K.kl_topk_logits(s, v, i), s.numel() * es, 0, True
+    if op == "route_experts":
+        z, bias = torch.randn(tok, 64, device=device).requires_grad_(), torch.zeros(64, device=device)
+        return (z,), lambda: R.route_experts(z, 6, False, bias)[0], \
+            lambda: K.route_experts(z, 6, score="sigmoid", bias=bias)[0], z.numel() * 4, 0, True
     if op == "softmax":
         x = r(tok, 128).requires_grad_()
         return (x,), lambda: torch.softmax(x, -1), lambda: K.softmax(x), 2 * x.numel() * es, 0, True

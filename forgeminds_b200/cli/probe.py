@@ -37,6 +37,8 @@ def _cases(dev, dt):
     T, hd = 37, 48
     ang = torch.outer(torch.arange(T, dtype=torch.float32), 10000.0 ** (-torch.arange(0, hd, 2, dtype=torch.float32) / hd))
     cos, sin = ang.cos().to(dev)[None, :, None, :], ang.sin().to(dev)[None, :, None, :]
+    kept, kept_at = rnd(65, 5001, dtype=torch.float32).topk(9, dim=-1)
+    bias, groups = rnd(40, scale=0.1, dtype=torch.float32), dict(score="sigmoid", n_groups=5, top_groups=3)
     out = [
         ("rms_norm 1003x1032", lambda a: K.rms_norm(a[0], a[1], 1e-6), lambda a: R.rms_norm(a[0], a[1], 1e-6),
          [rnd(1003, 1032), rnd(1032, dtype=torch.float32)], 3e-2),
@@ -51,6 +53,16 @@ def _cases(dev, dt):
         ("kl_div_logits 65x5000", lambda a: K.kl_div_logits(a[0], a[1].detach()),       # the teacher is a constant
          lambda a: R.kl_div_logits(a[0], a[1].detach())[0],
          [rnd(65, 5000), rnd(65, 5000)], 3e-2),
+        ("layer_norm 1003x1030", lambda a: K.layer_norm(*a), lambda a: R.layer_norm(*a),
+         [rnd(1003, 1030), rnd(1030, dtype=torch.float32), rnd(1030, dtype=torch.float32)], 3e-2),
+        ("add_layer_norm 517x2056", lambda a: K.add_layer_norm(*a), lambda a: R.add_layer_norm(*a),
+         [rnd(517, 2056), rnd(517, 2056), rnd(2056, dtype=torch.float32), rnd(2056, dtype=torch.float32)], 3e-2),
+        ("rotary 3x37x5x48, 20 of 48 interleaved", lambda a: K.rotary(a[0], cos[0, :, 0, :10], sin[0, :, 0, :10], None, True),
+         lambda a: R.rotary(a[0], cos[0, :, 0, :10], sin[0, :, 0, :10], None, True), [rnd(3, T, 5, hd)], 2e-2),
+        ("kl_topk_logits 65x5001", lambda a: K.kl_topk_logits(a[0], kept, kept_at),
+         lambda a: R.kl_topk(a[0], kept, kept_at).mean(), [rnd(65, 5001)], 3e-2),
+        ("route_experts 61x40, 3 of 5 groups", lambda a: K.route_experts(a[0], 6, bias=bias, **groups)[0],
+         lambda a: R.route_experts(a[0], 6, False, bias, 5, 3)[0], [rnd(61, 40)], 2e-2),
     ]
     return out
 

@@ -533,6 +533,17 @@ def kl_topk_distill_loss(hs: torch.Tensor, w: torch.Tensor, teacher_values: torc
 ROUTE_MAX_EXPERTS, ROUTE_MAX_K, ROUTE_MAX_GROUPS = 512, 32, 32
 
 
+def check_route(E: int, k: int, score: str, n_groups: int, top_groups: int, group_best: int) -> None:
+    """Raises ``ValueError`` for a choice of ``k`` of ``E`` experts that :func:`route_experts` refuses."""
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"score must be softmax|sigmoid, got {score!r}")
+    if n_groups < 1 or E % n_groups or not 1 <= top_groups <= n_groups or group_best not in (1, 2):
+        raise ValueError(f"{E} experts in {n_groups} groups of which {top_groups} are kept by their {group_best} best: the "
+                         "groups must be equal, 1 <= top_groups <= n_groups, group_best 1 or 2")
+    if not 1 <= k <= E // n_groups * top_groups:
+        raise ValueError(f"k must be from 1 to the {E // n_groups * top_groups} experts of the kept groups, got {k}")
+
+
 def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias: torch.Tensor | None = None, n_groups: int = 1,
                   top_groups: int = 1, group_best: int = 2, renormalise: bool = True, scale: float = 1.0,
                   aux_coef: float = 0.0, z_coef: float = 0.0):
@@ -550,13 +561,7 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
     if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
         raise ValueError(f"route_experts needs floating-point [tokens, experts], got {tuple(logits.shape)} {logits.dtype}")
     E = logits.shape[1]
-    if score not in ("softmax", "sigmoid"):
-        raise ValueError(f"score must be softmax|sigmoid, got {score!r}")
-    if n_groups < 1 or E % n_groups or not 1 <= top_groups <= n_groups or group_best not in (1, 2):
-        raise ValueError(f"{E} experts in {n_groups} groups of which {top_groups} are kept by their {group_best} best: the "
-                         "groups must be equal, 1 <= top_groups <= n_groups, group_best 1 or 2")
-    if not 1 <= k <= E // n_groups * top_groups:
-        raise ValueError(f"k must be from 1 to the {E // n_groups * top_groups} experts of the kept groups, got {k}")
+    check_route(E, k, score, n_groups, top_groups, group_best)
     if bias is not None:
         if tuple(bias.shape) != (E,) or not bias.is_floating_point():
             raise ValueError(f"route_experts: bias {tuple(bias.shape)} {bias.dtype} for {E} experts")

@@ -32,6 +32,10 @@ def _looks_like_swiglu(m: nn.Module) -> bool:
     return all(isinstance(getattr(m, n, None), nn.Linear) for n in ("w1", "w2", "w3"))
 
 
+def _is_layer_norm(m: nn.Module) -> bool:
+    return isinstance(m, nn.LayerNorm) and len(m.normalized_shape) == 1
+
+
 def _eps_of(m: nn.Module, x: torch.Tensor) -> float:
     eps = getattr(m, "eps", None)
     return float(torch.finfo(x.dtype).eps if eps is None else eps)     # nn.RMSNorm(eps=None) semantics
@@ -48,6 +52,14 @@ def _fuse_norm(m: nn.Module) -> None:
     def forward(self, x):
         w = self.weight
         return rms_norm(x, w if w.dtype in (x.dtype, torch.float32) else w.to(x.dtype), _eps_of(self, x))
+    _swap_forward(m, forward)
+
+
+def _fuse_layer_norm(m: nn.Module) -> None:
+    from . import layer_norm
+
+    def forward(self, x):
+        return layer_norm(x, self.weight, self.bias, self.eps)
     _swap_forward(m, forward)
 
 
@@ -81,12 +93,18 @@ def _fuse_mlp_split(m: nn.Module) -> None:
 
 def patch(module: nn.Module, split: bool = False, kind: "str | None" = None) -> bool:
     """Fuse one module in place. Returns True if it was recognised (or already patched), False if
-    it was left alone. ``kind="norm"`` / ``kind="mlp"`` validate the structure and raise
-    ``TypeError`` when it does not fit."""
+    it was left alone. ``kind="norm"`` / ``kind="mlp"`` / ``kind="layer_norm"`` validate the structure and raise
+    ``TypeError`` when it does not fit; a ``torch.nn.LayerNorm`` is only taken when it is named."""
     if getattr(module, "_fm_norm", False) or getattr(module, "_fm_mlp", False):
         return True
-    if kind not in (None, "norm", "mlp"):
-        raise ValueError(f"kind must be 'norm', 'mlp' or None, got {kind!r}")
+    if kind not in (None, "norm", "mlp", "layer_norm"):
+        raise ValueError(f"kind must be 'norm', 'mlp', 'layer_norm' or None, got {kind!r}")
+    if kind == "layer_norm":
+        if not _is_layer_norm(module):
+            raise TypeError(f"patch(kind='layer_norm') needs a torch.nn.LayerNorm of one dimension, got {type(module).__name__}")
+        _fuse_layer_norm(module)
+        module._fm_norm = True
+        return True
     if kind == "norm":
         if not _norm_weight_ok(module):
             raise TypeError(f"patch(kind='norm') needs a 1-D weight Parameter on {type(module).__name__}")
@@ -109,13 +127,20 @@ def patch(module: nn.Module, split: bool = False, kind: "str | None" = None) -> 
     return False
 
 
-def enable(model: nn.Module, norm: bool = True, swiglu_mlp: bool = True, split: bool = False) -> nn.Module:
-    """Patch every recognised norm / gated MLP under ``model``; counts land on ``model._fm_fused``."""
+def enable(model: nn.Module, norm: bool = True, swiglu_mlp: bool = True, split: bool = False,
+           layer_norm: bool = False) -> nn.Module:
+    """Patch every recognised norm / gated MLP under ``model``, and with ``layer_norm`` every ``torch.nn.LayerNorm`` of one
+    dimension; counts land on ``model._fm_fused``."""
     counts = {"norm": 0, "mlp": 0}
+    if layer_norm:
+        counts["layer_norm"] = 0
     for m in list(model.modules()):
         if getattr(m, "_fm_norm", False) or getattr(m, "_fm_mlp", False):
             continue
-        if norm and _looks_like_rmsnorm(m):
+        if layer_norm and _is_layer_norm(m):
+            patch(m, kind="layer_norm")
+            counts["layer_norm"] += 1
+        elif norm and _looks_like_rmsnorm(m):
             patch(m)
             counts["norm"] += 1
         elif swiglu_mlp and _looks_like_swiglu(m):

@@ -15,6 +15,11 @@ Three execution paths share those semantics:
 * **sm_100a, expert parallel**: the dispatch writes routed rows straight into the owning rank's
   symmetric buffer and the combine reads them back over NVLink (:mod:`forgeminds_b200.parallel.ep`).
 
+The router's choice can also be made by sigmoid scores, with a bias that balances the load without a loss
+(``balance_bias=True``, :meth:`Router.rebalance`), within the best groups of experts, and with weights that are
+not renormalised or are scaled: :func:`forgeminds_b200.kernels.route_experts` states the formulas, and every
+path above takes its choice.
+
 ``capacity_factor > 0`` bounds every expert to ``ceil(cf * tokens * top_k / E)`` rows and drops the
 overflow (the reference is dropless; 0 keeps that behaviour).
 """
@@ -55,13 +60,46 @@ class _AllToAll(torch.autograd.Function):
 
 
 class Router(nn.Module):
-    def __init__(self, dim: int, n_experts: int, top_k: int):
+    """Gate and choice of experts. The options beyond ``top_k`` are those of ``fm.kernels.route_experts``;
+    ``balance_bias=True`` adds the buffer ``bias [n_experts]`` (zeros), which :meth:`rebalance` moves."""
+
+    def __init__(self, dim: int, n_experts: int, top_k: int, score: str = "softmax", balance_bias: bool = False,
+                 n_groups: int = 1, top_groups: int = 1, group_best: int = 2, renormalise: bool = True,
+                 scale: float = 1.0):
         super().__init__()
         self.gate = nn.Linear(dim, n_experts, bias=False)
         self.n_experts, self.top_k = n_experts, top_k
+        self.plain = score == "softmax" and not balance_bias and n_groups == 1 and renormalise and scale == 1.0
+        if not self.plain:
+            from .kernels import check_route
+            check_route(n_experts, top_k, score, n_groups, top_groups, group_best)
+        self.options = dict(score=score, n_groups=n_groups, top_groups=top_groups, group_best=group_best,
+                            renormalise=bool(renormalise), scale=float(scale))
+        self.register_buffer("bias", torch.zeros(n_experts) if balance_bias else None)
+        self.last_counts: Optional[torch.Tensor] = None
+
+    def choose(self, logits, aux_coef: float, z_coef: float):
+        """``logits [N, E]`` -> ``(weights fp32 [N, k], idx int32 [N, k], aux)`` by the options; keeps the counts."""
+        from . import kernels as K
+        w, idx, self.last_counts, aux = K.route_experts(logits, self.top_k, bias=self.bias, aux_coef=aux_coef,
+                                                        z_coef=z_coef, **self.options)
+        return w, idx, logits.new_zeros((), dtype=torch.float32) if aux is None else aux
+
+    @torch.no_grad()
+    def rebalance(self, rate: float, group=None) -> None:
+        """``bias += rate * sign(mean load - load)`` by the last forward pass's counts, summed over the ranks of ``group``
+        when it is given: experts with less than their share become easier to choose."""
+        if self.bias is None:
+            raise RuntimeError("rebalance needs a router with balance_bias=True")
+        if self.last_counts is None:
+            raise RuntimeError("rebalance needs the counts of a forward pass")
+        load = self.last_counts.float()
+        if group is not None:
+            dist.all_reduce(load, group=group)
+        self.bias += (rate * torch.sign(load.mean() - load)).to(self.bias.dtype)
 
     def forward(self, x):
-        """``x [N, d]`` -> ``(weights [N, k] in x.dtype, idx [N, k], aux, z)``"""
+        """``x [N, d]`` -> ``(weights [N, k] in x.dtype, idx [N, k], aux, z)`` of the plain softmax choice"""
         logits = self.gate(x).float()
         probs = logits.softmax(dim=-1)
         w, idx = probs.topk(self.top_k, dim=-1)
@@ -133,14 +171,17 @@ class Experts(nn.Module):
 
 class MoE(nn.Module):
     def __init__(self, dim, hidden, n_experts, top_k, n_shared=0, ep_size=1, ep_group=None, ep_rank=0,
-                 offload_experts=False, grouped_mm=False, aux_coef=1e-2, z_coef=1e-3, capacity_factor=0.0):
+                 offload_experts=False, grouped_mm=False, aux_coef=1e-2, z_coef=1e-3, capacity_factor=0.0,
+                 score="softmax", balance_bias=False, n_groups=1, top_groups=1, group_best=2, renormalise=True,
+                 route_scale=1.0):
         super().__init__()
         assert n_experts % ep_size == 0, "n_experts must be divisible by ep_size"
         self.dim, self.hidden = dim, hidden
         self.n_experts, self.top_k = n_experts, top_k
         self.ep_size, self.ep_group, self.ep_rank = ep_size, ep_group, ep_rank
         self.n_local = n_experts // ep_size
-        self.router = Router(dim, n_experts, top_k)
+        self.router = Router(dim, n_experts, top_k, score=score, balance_bias=balance_bias, n_groups=n_groups,
+                             top_groups=top_groups, group_best=group_best, renormalise=renormalise, scale=route_scale)
         self.experts = Experts(self.n_local, dim, hidden, offload=offload_experts, grouped_mm=grouped_mm)
         self.shared = None
         if n_shared:
@@ -180,8 +221,12 @@ class MoE(nn.Module):
             from .ops.moe import moe_forward_native
             out = moe_forward_native(self, flat)
             return out.reshape(shape)
-        w, idx, aux, z = self.router(flat)
-        self.last_aux = self.aux_coef * aux + self.z_coef * z
+        if self.router.plain:
+            w, idx, aux, z = self.router(flat)
+            self.last_aux = self.aux_coef * aux + self.z_coef * z
+        else:
+            w, idx, self.last_aux = self.router.choose(self.router.gate(flat), self.aux_coef, self.z_coef)
+            w, idx = w.to(flat.dtype), idx.long()
         out = self._dispatch_torch(flat, w, idx)
         if self.shared is not None:
             out = out + self.shared(flat)

@@ -1,11 +1,13 @@
-"""Building blocks for user architectures that run on the fused kernels: :class:`RMSNorm`, :class:`SwiGLU`.
+"""Building blocks for user architectures that run on the fused kernels: :class:`RMSNorm`, :class:`LayerNorm`,
+:class:`SwiGLU`.
 
 Drop-in ``nn.Module``s: on a B200 their forward goes through :mod:`forgeminds_b200.kernels` (hand-written
 sm_100a kernels, fp32 accumulation, one rounding at the store), anywhere else through the PyTorch
 statement of the same arithmetic. State-dict contract (the reference's ``forgemind/nn.py:82-217``):
 ``RMSNorm`` has the single parameter ``weight [dim]`` of ``torch.nn.RMSNorm`` and loads from / into one;
 ``SwiGLU`` has ``w1, w3, w2`` (``nn.Linear`` layout) or, when ``split=True``, ``gate_up, w2`` with
-``gate_up.weight = cat(w1.weight, w3.weight)``.
+``gate_up.weight = cat(w1.weight, w3.weight)``. ``LayerNorm`` has the parameters ``weight`` and ``bias`` of
+``torch.nn.LayerNorm``.
 """
 from __future__ import annotations
 
@@ -16,7 +18,7 @@ import torch.nn as nn
 
 from . import kernels as K
 
-__all__ = ["RMSNorm", "SwiGLU"]
+__all__ = ["RMSNorm", "LayerNorm", "SwiGLU"]
 
 
 def _positive(name: str, value) -> int:
@@ -63,6 +65,49 @@ class RMSNorm(nn.Module):
         if tuple(residual.shape) != tuple(x.shape):
             raise ValueError(f"residual {tuple(residual.shape)} and input {tuple(x.shape)} must have the same shape")
         total, normed = K.add_rms_norm(x, residual, gain, self.eps)
+        return normed, total
+
+
+class LayerNorm(nn.Module):
+    """Layer normalisation of the last dimension, ``y = (x - mean) / sqrt(var + eps) * weight + bias``.
+
+    ``forward_with_residual(x, r)`` returns ``(norm(x + r), x + r)`` from a single pass over the row.
+    """
+
+    def __init__(self, dim: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True, device=None,
+                 dtype=None):
+        super().__init__()
+        self.dim = _positive("LayerNorm dim", dim)
+        self.eps = float(eps)
+        self.elementwise_affine = bool(elementwise_affine)
+        affine = self.elementwise_affine
+        self.register_parameter("weight", nn.Parameter(torch.ones(self.dim, device=device, dtype=dtype)) if affine else None)
+        self.register_parameter("bias", nn.Parameter(torch.zeros(self.dim, device=device, dtype=dtype)) if affine and bias else None)
+
+    def extra_repr(self) -> str:
+        parts = [f"dim={self.dim}", f"eps={self.eps:g}"]
+        if self.weight is None:
+            parts.append("no weight")
+        elif self.bias is None:
+            parts.append("no bias")
+        return ", ".join(parts)
+
+    def _fits(self, x: torch.Tensor) -> None:
+        if x.shape[-1] != self.dim:
+            raise ValueError(f"input of shape {tuple(x.shape)} cannot be normalised by LayerNorm(dim={self.dim}): "
+                             "the last dimension must equal dim")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        self._fits(x)
+        return K.layer_norm(x, self.weight, self.bias, self.eps)
+
+    def forward_with_residual(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        self._fits(x)
+        if residual is None:
+            return K.layer_norm(x, self.weight, self.bias, self.eps), x
+        if tuple(residual.shape) != tuple(x.shape):
+            raise ValueError(f"residual {tuple(residual.shape)} and input {tuple(x.shape)} must have the same shape")
+        total, normed = K.add_layer_norm(x, residual, self.weight, self.bias, self.eps)
         return normed, total
 
 

@@ -153,6 +153,15 @@ def plan(idx, n_experts: int, capacity: int = 0):
     return slot_of, token_of, region, tile_group, limit
 
 
+def choose(moe, logits):
+    """``logits [N, E]`` -> ``(weights fp32 [N, k], idx int32 [N, k])`` by the layer's router; sets ``moe.last_aux``."""
+    if moe.router.plain:
+        route_w, idx, moe.last_aux, _counts = _Route.apply(logits, moe.top_k, moe.aux_coef, moe.z_coef)
+    else:
+        route_w, idx, moe.last_aux = moe.router.choose(logits, moe.aux_coef, moe.z_coef)
+    return route_w, idx
+
+
 def moe_forward_native(moe, x):
     """``x [N, d]`` bf16 -> MoE output ``[N, d]``; sets ``moe.last_aux``."""
     from .functional import linear
@@ -165,8 +174,7 @@ def moe_forward_native(moe, x):
         logits = linear(x, gate)
     else:       # the GEMM epilogue stores 16-byte vectors: an odd expert count takes the library matmul
         logits = torch.nn.functional.linear(x, gate.to(x.dtype))
-    route_w, idx, aux, _counts = _Route.apply(logits, moe.top_k, moe.aux_coef, moe.z_coef)
-    moe.last_aux = aux
+    route_w, idx = choose(moe, logits)
     slot_of, token_of, region, tile_group, limit = plan(idx, moe.n_experts, moe.capacity(x.shape[0]))
     ex = moe.experts
     out = _Experts.apply(x, route_w, ex.w1, ex.w3, ex.w2, slot_of, token_of, region, tile_group, moe.top_k, limit)

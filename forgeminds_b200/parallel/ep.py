@@ -87,14 +87,13 @@ class EPEngine:
     def forward(self, moe, x):
         """``x [N, d]`` bf16 -> ``[N, d]``; sets ``moe.last_aux``."""
         from ..ops.functional import linear
-        from ..ops.moe import _Route
+        from ..ops.moe import choose
         gate = moe.router.gate.weight
         if gate.shape[0] % 8 == 0:
             logits = linear(x, gate)
         else:
             logits = torch.nn.functional.linear(x, gate.to(x.dtype))
-        route_w, idx, aux, _counts = _Route.apply(logits, moe.top_k, moe.aux_coef, moe.z_coef)
-        moe.last_aux = aux
+        route_w, idx = choose(moe, logits)
         ex = moe.experts
         out = _EPExperts.apply(x, route_w, idx, ex.w1, ex.w3, ex.w2, self, moe.n_experts, moe.capacity(x.shape[0]))
         if moe.shared is not None:
