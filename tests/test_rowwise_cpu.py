@@ -245,3 +245,101 @@ def test_route_refuses():
     for bad in (z[0], z.long(), z[:, :0]):
         with pytest.raises(ValueError):
             K.route_experts(bad, 1)
+
+
+# ------------------------------------------------------------------------------ modules that take them
+def test_layer_norm_module():
+    mine, theirs = fm.nn.LayerNorm(24), torch.nn.LayerNorm(24)
+    torch.nn.init.normal_(theirs.weight)
+    torch.nn.init.normal_(theirs.bias)
+    mine.load_state_dict(theirs.state_dict())
+    theirs.load_state_dict(mine.state_dict())
+    x, r = _randn(3, 5, 24, seed=30), _randn(3, 5, 24, seed=31)
+    assert torch.allclose(mine(x), theirs(x), atol=1e-6)
+    y, total = mine.forward_with_residual(x, r)
+    assert torch.equal(total, x + r) and torch.allclose(y, theirs(x + r), atol=1e-6)
+    assert mine.forward_with_residual(x)[1] is x
+    assert [n for n, _ in fm.nn.LayerNorm(8, bias=False).named_parameters()] == ["weight"]
+    assert not list(fm.nn.LayerNorm(8, elementwise_affine=False).parameters())
+    assert "eps=1e-05" in repr(mine) and "no bias" in repr(fm.nn.LayerNorm(8, bias=False))
+    for bad in (lambda: fm.nn.LayerNorm(0), lambda: mine(x[..., :8]), lambda: mine.forward_with_residual(x, r[:1])):
+        with pytest.raises(ValueError):
+            bad()
+
+
+def test_patching_a_layer_norm_has_to_be_asked_for():
+    model = torch.nn.Sequential(torch.nn.LayerNorm(16), torch.nn.Linear(16, 16), torch.nn.LayerNorm((4, 4)))
+    K.enable(model)
+    assert model._fm_fused == {"norm": 0, "mlp": 0} and not K.patch(model[0])
+    x = _randn(3, 16, seed=32)
+    before = model[0](x)
+    K.enable(model, layer_norm=True)
+    assert model._fm_fused == {"norm": 0, "mlp": 0, "layer_norm": 1} and "forward" in model[0].__dict__
+    assert torch.allclose(model[0](x), before, atol=1e-6)
+    K.revert(model)
+    assert "forward" not in model[0].__dict__
+    assert K.patch(model[0], kind="layer_norm") and K.patch(model[0], kind="layer_norm")
+    for m in (model[1], model[2]):
+        with pytest.raises(TypeError):
+            K.patch(m, kind="layer_norm")
+
+
+@pytest.mark.parametrize("opts", [dict(score="sigmoid"), dict(balance_bias=True), dict(n_groups=2, top_groups=1),
+                                  dict(renormalise=False), dict(score="sigmoid", balance_bias=True, n_groups=2, top_groups=2, route_scale=2.5)])
+def test_moe_takes_the_routing_options(opts):
+    torch.manual_seed(5)
+    moe = fm.MoE(16, 32, 8, 3, **opts)
+    if moe.router.bias is not None:
+        assert "router.bias" in moe.state_dict()
+        moe.router.bias.copy_(0.1 * _randn(8, seed=33))
+    else:
+        assert "router.bias" not in moe.state_dict()
+    x = _randn(4, 6, 16, seed=34).requires_grad_()
+    y = moe(x)
+    names = dict(opts)
+    names["scale"] = names.pop("route_scale", 1.0)
+    names.pop("balance_bias", None)
+    flat = x.reshape(-1, 16)
+    w, idx, counts, aux = K.route_experts(moe.router.gate(flat), 3, bias=moe.router.bias, aux_coef=1e-2, z_coef=1e-3, **names)
+    want = torch.zeros_like(flat)
+    for e in range(8):
+        h = (F.silu(flat @ moe.experts.w1[e]) * (flat @ moe.experts.w3[e])) @ moe.experts.w2[e]
+        want = want + h * (w * (idx == e)).sum(-1, keepdim=True)
+    assert torch.allclose(y.reshape(-1, 16), want, atol=1e-6) and torch.allclose(moe.last_aux, aux)
+    assert torch.equal(moe.router.last_counts, counts)
+    for a, b in zip(torch.autograd.grad(y.sum() + moe.last_aux, (x, moe.router.gate.weight)),
+                    torch.autograd.grad(want.sum() + aux, (x, moe.router.gate.weight))):
+        assert torch.allclose(a, b, atol=1e-5)
+
+
+def test_moe_balance():
+    torch.manual_seed(6)
+    moe = fm.MoE(16, 32, 4, 1, score="sigmoid", balance_bias=True, aux_coef=0.0, z_coef=0.0)
+    with pytest.raises(RuntimeError):
+        moe.router.rebalance(0.1)                            # no forward pass yet
+    with torch.no_grad():
+        moe.router.gate.weight[2] += 0.5                     # a favourite
+    x = _randn(200, 16, seed=35).abs()
+    moe(x)
+    assert float(moe.last_aux) == 0.0 and moe.router.last_counts.argmax() == 2
+    first = moe.router.last_counts.clone()
+    for _ in range(40):
+        moe.router.rebalance(0.02)
+        moe(x)
+    assert moe.router.last_counts.max() < first.max() and moe.router.bias[2] < 0
+    with pytest.raises(RuntimeError):
+        fm.MoE(16, 32, 4, 1).router.rebalance(0.1)
+    for bad in (dict(score="tanh"), dict(n_groups=3), dict(n_groups=2, top_groups=3), dict(n_groups=4, top_groups=1, score="sigmoid")):
+        with pytest.raises(ValueError):
+            fm.MoE(16, 32, 4, 2, **bad)
+
+
+def test_moe_defaults_route_as_before():
+    torch.manual_seed(7)
+    moe = fm.MoE(16, 32, 4, 2)
+    assert moe.router.plain and set(moe.state_dict()) == {"router.gate.weight", "experts.w1", "experts.w3", "experts.w2"}
+    x = _randn(9, 16, seed=36)
+    w, idx, aux, z = moe.router(x)
+    probs = moe.router.gate(x).softmax(-1)
+    v, i = probs.topk(2, dim=-1)
+    assert torch.equal(idx, i) and torch.allclose(w, v / v.sum(-1, keepdim=True))
