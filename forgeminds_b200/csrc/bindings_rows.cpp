@@ -33,6 +33,12 @@ void ok(int rc, const char* what, int kernels) {
   fmb_count_launches(kernels);
 }
 
+// What a user may get wrong raises ValueError, like the checks of the PyTorch path; the C++ side makes them for the kernels'
+// path because they cost it a microsecond less per argument.
+template <typename... P> void refuse(bool when, const P&... parts) {
+  if (when) throw pybind11::value_error(c10::str(parts...));
+}
+
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
 const void* ptr(const OptTensor& t) { return given(t) ? t->data_ptr() : nullptr; }
 
@@ -46,8 +52,11 @@ void beside(const Tensor& t, const Tensor& like, int64_t n, at::ScalarType type,
 void rows_of(const Tensor& t, const char* name) {
   TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor");
   TORCH_CHECK(t.dim() == 2 && (t.numel() == 0 || t.size(1) <= 1 || t.stride(1) == 1), name, " must be 2-D with contiguous rows");
-  TORCH_CHECK(t.size(1) >= 1 && t.size(1) <= (1 << 24), name, ": rows of 1 to 2^24 values");
+  TORCH_CHECK(t.size(1) >= 1 && (t.size(1) <= (1 << 24) || t.numel() == 0), name, ": rows of 1 to 2^24 values");
 }
+
+// elements between rows; what a single row says about it means nothing (and may be odd, which costs the wide loads)
+int64_t pitch(const Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
 
 void rows_like(const Tensor& t, const Tensor& like, const char* name) {
   rows_of(t, name);
@@ -70,7 +79,7 @@ std::vector<Tensor> layernorm_fwd(const Tensor& x, const OptTensor& delta, const
   Tensor y = at::empty({rows, d}, x.options()), sum, stats;
   if (given(delta)) sum = at::empty({rows, d}, x.options());
   if (need_stats) stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
-  ok(fmb_layernorm_fwd(x.data_ptr(), x.stride(0), ptr(delta), given(delta) ? delta->stride(0) : 0, ptr(w), ptr(b),
+  ok(fmb_layernorm_fwd(x.data_ptr(), pitch(x), ptr(delta), given(delta) ? pitch(*delta) : 0, ptr(w), ptr(b),
                        given(delta) ? sum.data_ptr() : nullptr, y.data_ptr(), need_stats ? stats.data_ptr<float>() : nullptr, rows,
                        static_cast<int>(d), static_cast<float>(eps), dt(x, "x"), wt == at::kFloat ? FMB_F32 : FMB_BF16,
                        cur_stream()), "layernorm_fwd", rows > 0);
@@ -96,8 +105,8 @@ std::vector<Tensor> layernorm_bwd(const Tensor& dy, const Tensor& x, const OptTe
   if (need_db) db = cols ? at::empty({d}, wopt) : at::zeros({d}, wopt);
   const int nb = fmb_layernorm_bwd_blocks(rows, static_cast<int>(d), dt(x, "x"));
   if (cols) partial = at::empty({nb, 2, d}, x.options().dtype(at::kFloat));
-  ok(fmb_layernorm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), ptr(w), stats.data_ptr<float>(), ptr(dres),
-                       given(dres) ? dres->stride(0) : 0, dx.data_ptr(), cols ? partial.data_ptr<float>() : nullptr,
+  ok(fmb_layernorm_bwd(dy.data_ptr(), pitch(dy), x.data_ptr(), pitch(x), ptr(w), stats.data_ptr<float>(), ptr(dres),
+                       given(dres) ? pitch(*dres) : 0, dx.data_ptr(), cols ? partial.data_ptr<float>() : nullptr,
                        need_dw ? dw.data_ptr() : nullptr, need_db ? db.data_ptr() : nullptr, rows, static_cast<int>(d), dt(x, "x"),
                        w_fp32 ? FMB_F32 : FMB_BF16, nb, cur_stream()), "layernorm_bwd", rows > 0 ? 1 + cols : 0);
   return {dx, dw, db};
@@ -114,6 +123,7 @@ std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& co
     TORCH_CHECK(t.dim() == 4 && (t.numel() == 0 || t.size(3) <= 1 || t.stride(3) == 1), name, " must be [B, T, H, D] with contiguous heads");
     TORCH_CHECK(t.size(0) == q.size(0) && t.size(1) == q.size(1) && t.size(3) == q.size(3), name,
                 " must share q's batch, sequence and head dimensions");
+    TORCH_CHECK(t.size(2) <= (1 << 24), name, ": more than 2^24 heads");
   };
   check(q, "q");
   if (given(k)) check(*k, "k");
@@ -137,10 +147,11 @@ std::vector<Tensor> rotary(const Tensor& q, const OptTensor& k, const Tensor& co
   }
   c10::cuda::CUDAGuard guard(q.device());
   Tensor qo = at::empty({B, T, q.size(2), D}, q.options()), ko;
-  FmbRotaryTensor qa = {q.data_ptr(), qo.data_ptr(), q.stride(0), q.stride(1), q.stride(2), static_cast<int>(q.size(2))}, ka = {};
+  auto step = [](const Tensor& t, int dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; };       // (of one: it may be odd)
+  FmbRotaryTensor qa = {q.data_ptr(), qo.data_ptr(), step(q, 0), step(q, 1), step(q, 2), static_cast<int>(q.size(2))}, ka = {};
   if (given(k)) {
     ko = at::empty({B, T, k->size(2), D}, q.options());
-    ka = {k->data_ptr(), ko.data_ptr(), k->stride(0), k->stride(1), k->stride(2), static_cast<int>(k->size(2))};
+    ka = {k->data_ptr(), ko.data_ptr(), step(*k, 0), step(*k, 1), step(*k, 2), static_cast<int>(k->size(2))};
   }
   if (B * T == 0 || D == 0 || qa.heads + ka.heads == 0) return {qo, ko};
   ok(fmb_rotary(&qa, &ka, cos.data_ptr<float>(), sin.data_ptr<float>(), cos.stride(0), table, ptr(positions), wide, pos_b, B,
@@ -171,13 +182,13 @@ std::vector<Tensor> kl_topk_fwd(const Tensor& student, const Tensor& values, con
   c10::cuda::CUDAGuard guard(student.device());
   auto f32 = student.options().dtype(at::kFloat);
   Tensor row_loss = at::empty({rows}, f32), stats = at::empty({rows, 2}, f32), grad, loss;
-  Tensor ws = at::empty({2}, student.options().dtype(at::kInt));
+  Tensor ws = at::empty({FMB_KL_SCRATCH}, student.options().dtype(at::kInt));
   if (need_grad) grad = in_place ? student : at::empty({rows, V}, student.options());
   if (total) loss = rows > 0 ? at::empty({}, f32) : at::zeros({}, f32);
-  ok(fmb_kl_topk_fwd(student.data_ptr(), student.stride(0), values.data_ptr(),
+  ok(fmb_kl_topk_fwd(student.data_ptr(), pitch(student), values.data_ptr(),
                      reinterpret_cast<const long long*>(index.data_ptr<int64_t>()), static_cast<const float*>(ptr(lse)),
                      row_loss.data_ptr<float>(), stats.data_ptr<float>(), need_grad ? grad.data_ptr() : nullptr,
-                     need_grad ? grad.stride(0) : 0, static_cast<const int*>(ptr(count)), ws.data_ptr<int>(),
+                     need_grad ? pitch(grad) : 0, static_cast<const int*>(ptr(count)), ws.data_ptr<int>(), static_cast<int>(ws.numel()),
                      total ? loss.data_ptr<float>() : nullptr, rows, static_cast<int>(V), static_cast<int>(K),
                      static_cast<float>(tau), mean, dt(student, "student"), dt(values, "values"), cur_stream()),
      "kl_topk_fwd", rows > 0 ? 1 + (mean && !given(count)) : 0);
@@ -196,9 +207,9 @@ Tensor kl_topk_bwd(const Tensor& student, const Tensor& values, const Tensor& in
   if (given(done)) rows_like(*done, student, "done");
   c10::cuda::CUDAGuard guard(student.device());
   Tensor grad = given(done) ? *done : at::empty({rows, V}, student.options());
-  ok(fmb_kl_topk_bwd(student.data_ptr(), student.stride(0), values.data_ptr(),
+  ok(fmb_kl_topk_bwd(student.data_ptr(), pitch(student), values.data_ptr(),
                      reinterpret_cast<const long long*>(index.data_ptr<int64_t>()), static_cast<const float*>(ptr(lse)),
-                     stats.data_ptr<float>(), grad.data_ptr(), grad.stride(0), static_cast<const int*>(ptr(count)),
+                     stats.data_ptr<float>(), grad.data_ptr(), pitch(grad), static_cast<const int*>(ptr(count)),
                      upstream.data_ptr<float>(), upstream.dim() > 0 && upstream.numel() == rows, given(done), rows,
                      static_cast<int>(V), static_cast<int>(K), static_cast<float>(tau), dt(student, "student"),
                      dt(values, "values"), cur_stream()), "kl_topk_bwd", rows > 0);
@@ -224,7 +235,7 @@ std::vector<Tensor> route_fwd(const Tensor& logits, const OptTensor& bias, int64
     partial = at::empty({nb, E + 1}, f32);
     aux = N > 0 ? at::empty({}, f32) : at::zeros({}, f32);
   }
-  ok(fmb_route_fwd(logits.data_ptr(), logits.stride(0), dt(logits, "logits"), static_cast<const float*>(ptr(bias)),
+  ok(fmb_route_fwd(logits.data_ptr(), pitch(logits), dt(logits, "logits"), static_cast<const float*>(ptr(bias)),
                    weights.data_ptr<float>(), idx.data_ptr<int>(), counts.data_ptr<int>(),
                    need_aux ? partial.data_ptr<float>() : nullptr, need_aux ? aux.data_ptr<float>() : nullptr, N,
                    static_cast<int>(E), static_cast<int>(k), softmax, static_cast<int>(groups), static_cast<int>(top_groups),
@@ -246,7 +257,7 @@ Tensor route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& idx,
   if (given(daux)) beside(*daux, logits, 1, at::kFloat, "daux");
   c10::cuda::CUDAGuard guard(logits.device());
   Tensor out = at::empty({N, E}, logits.options());
-  ok(fmb_route_bwd(logits.data_ptr(), logits.stride(0), dt(logits, "logits"), weights.data_ptr<float>(), idx.data_ptr<int>(),
+  ok(fmb_route_bwd(logits.data_ptr(), pitch(logits), dt(logits, "logits"), weights.data_ptr<float>(), idx.data_ptr<int>(),
                    static_cast<const float*>(ptr(dweights)), static_cast<const float*>(ptr(daux)), counts.data_ptr<int>(),
                    out.data_ptr(), N, static_cast<int>(E), static_cast<int>(k), softmax, renorm, static_cast<float>(scale),
                    static_cast<float>(aux_coef), static_cast<float>(z_coef), cur_stream()), "route_bwd", N > 0);
@@ -291,12 +302,27 @@ Tensor heads4(const Tensor& x) { return x.size(3) <= 1 || x.stride(3) == 1 ? x :
 Tensor f32_flat(const Tensor& t, int64_t n) { return t.to(at::kFloat).reshape({n}).contiguous(); }
 
 // weight and bias in one type that the kernels take: fp32, or the input's
-std::pair<Tensor, Tensor> gain(const Tensor& x, const OptTensor& w, const OptTensor& b) {
+std::pair<OptTensor, OptTensor> gain(const Tensor& x, const OptTensor& w, const OptTensor& b) {
   at::ScalarType type = at::kFloat;
   const at::ScalarType first = given(w) ? w->scalar_type() : given(b) ? b->scalar_type() : at::kFloat;
   if (first == x.scalar_type() && (!given(w) || !given(b) || b->scalar_type() == first)) type = first;
-  auto fit = [&](const OptTensor& t) { return given(t) ? t->detach().to(type).contiguous() : Tensor(); };
+  auto fit = [&](const OptTensor& t) {
+    return !given(t) || (t->scalar_type() == type && t->is_contiguous()) ? t : OptTensor(t->to(type).contiguous());
+  };
   return {fit(w), fit(b)};
+}
+Tensor shaped(const Tensor& t, const Tensor& like) { return like.dim() == 2 ? t : t.view(like.sizes()); }
+
+void check_norm(const char* op, const Tensor& x, const OptTensor& delta, const OptTensor& w, const OptTensor& b) {
+  refuse(x.dim() < 1 || x.size(-1) < 1, op, " normalises the last dimension; the input is ", x.sizes());
+  if (given(delta))
+    refuse(delta->sizes() != x.sizes() || delta->scalar_type() != x.scalar_type() || delta->device() != x.device(), op,
+           " needs two tensors of one shape, type and device, got ", x.sizes(), " ", x.scalar_type(), " on ", x.device(), " and ",
+           delta->sizes(), " ", delta->scalar_type(), " on ", delta->device());
+  for (const OptTensor* t : {&w, &b})
+    if (given(*t))
+      refuse((*t)->dim() != 1 || (*t)->size(0) != x.size(-1) || (*t)->device() != x.device(), op, ": a weight or bias ", (*t)->sizes(),
+             " on ", (*t)->device(), " does not fit rows of ", x.size(-1), " on ", x.device());
 }
 Tensor as_type(const Tensor& t, int64_t type) { return t.defined() ? t.to(static_cast<at::ScalarType>(type)) : t; }
 int64_t type_of(const OptTensor& t) { return given(t) ? static_cast<int64_t>(t->scalar_type()) : 0; }
@@ -309,50 +335,48 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     const bool add = given(delta);
     const Tensor x2 = rows2(x.detach());
     auto [wd, bd] = gain(x, w, b);
-    auto out = layernorm_fwd(x2, add ? OptTensor(rows2(delta->detach())) : OptTensor(), as_opt(wd), as_opt(bd), eps, true);
-    Tensor y = out[0].view(x.sizes());
-    Tensor sum = add ? out[1].view(x.sizes()) : Tensor();
-    if (add) ctx->save_for_backward({sum, wd, out[2]});
-    else ctx->save_for_backward({x2.is_alias_of(x) && x2.sizes() == x.sizes() ? x : x2, wd, out[2]});
-    ctx->saved_data["fp32"] = (!wd.defined() || wd.scalar_type() == at::kFloat) && (!bd.defined() || bd.scalar_type() == at::kFloat);
-    ctx->saved_data["w"] = type_of(w);
-    ctx->saved_data["b"] = type_of(b);
-    ctx->saved_data["add"] = add;
-    ctx->saved_data["edges"] = static_cast<int64_t>(given(w)) | static_cast<int64_t>(given(b)) << 1;
+    auto out = layernorm_fwd(x2, add ? OptTensor(rows2(delta->detach())) : OptTensor(), wd, bd, eps, true);
+    Tensor y = shaped(out[0], x);
+    Tensor sum = add ? shaped(out[1], x) : Tensor();
+    const Tensor weight = given(wd) ? (given(w) && wd->is_same(*w) ? *w : wd->detach()) : Tensor();
+    if (add) ctx->save_for_backward({sum, weight, out[2]});
+    else ctx->save_for_backward({x2.is_alias_of(x) && x2.sizes() == x.sizes() ? x : x2, weight, out[2]});
+    const bool fp32 = (!given(wd) || wd->scalar_type() == at::kFloat) && (!given(bd) || bd->scalar_type() == at::kFloat);
+    ctx->saved_data["how"] = static_cast<int64_t>(given(w)) | static_cast<int64_t>(given(b)) << 1 | static_cast<int64_t>(fp32) << 2 |
+                             static_cast<int64_t>(add) << 3 | type_of(w) << 8 | type_of(b) << 16;
     return add ? variable_list{sum, y} : variable_list{y};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const bool add = ctx->saved_data["add"].toBool();
+    const int64_t how = ctx->saved_data["how"].toInt();
+    const bool has_w = how & 1, has_b = how & 2, add = how & 8;
     const Tensor gy = add ? g[1] : g[0], gsum = add ? g[0] : Tensor();
-    if (!gy.defined()) return {gsum, gsum, Tensor(), Tensor(), Tensor()};
+    if (!gy.defined()) return {gsum, add ? gsum : Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
-    const int64_t edges = ctx->saved_data["edges"].toInt();
     const size_t first = add ? 2 : 1;
-    const bool need_w = (edges & 1) && ctx->needs_input_grad(first);
-    const bool need_b = (edges & 2) && ctx->needs_input_grad(first + (edges & 1));
+    const bool need_w = has_w && ctx->needs_input_grad(first), need_b = has_b && ctx->needs_input_grad(first + has_w);
     auto out = layernorm_bwd(rows2(gy), rows2(saved[0]), as_opt(saved[1]), saved[2],
-                             gsum.defined() ? OptTensor(rows2(gsum)) : OptTensor(), need_w, need_b, ctx->saved_data["fp32"].toBool());
-    const Tensor dx = out[0].view(gy.sizes());
-    return once({dx, add ? dx : Tensor(), as_type(out[1], ctx->saved_data["w"].toInt()), as_type(out[2], ctx->saved_data["b"].toInt()),
-                 Tensor()});
+                             gsum.defined() ? OptTensor(rows2(gsum)) : OptTensor(), need_w, need_b, how & 4);
+    const Tensor dx = shaped(out[0], gy);
+    return once({dx, add ? dx : Tensor(), as_type(out[1], how >> 8 & 255), as_type(out[2], how >> 16 & 255), Tensor()});
   }
 };
 
 Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  check_norm("layer_norm", x, OptTensor(), w, b);
   if (wants_grad({&x, opt(w), opt(b)})) return LayerNormNode::apply(x, OptTensor(), w, b, eps)[0];
   auto [wd, bd] = gain(x, w, b);
-  return layernorm_fwd(rows2(x), OptTensor(), as_opt(wd), as_opt(bd), eps, false)[0].view(x.sizes());
+  return shaped(layernorm_fwd(rows2(x), OptTensor(), wd, bd, eps, false)[0], x);
 }
 
 std::tuple<Tensor, Tensor> add_layer_norm(const Tensor& x, const Tensor& delta, const OptTensor& w, const OptTensor& b, double eps) {
-  TORCH_CHECK(x.sizes() == delta.sizes(), "add_layer_norm: one shape required");
+  check_norm("add_layer_norm", x, delta, w, b);
   if (wants_grad({&x, &delta, opt(w), opt(b)})) {
     auto out = LayerNormNode::apply(x, OptTensor(delta), w, b, eps);
     return {out[0], out[1]};
   }
   auto [wd, bd] = gain(x, w, b);
-  auto out = layernorm_fwd(rows2(x), rows2(delta), as_opt(wd), as_opt(bd), eps, false);
-  return {out[1].view(x.sizes()), out[0].view(x.sizes())};
+  auto out = layernorm_fwd(rows2(x), rows2(delta), wd, bd, eps, false);
+  return {shaped(out[1], x), shaped(out[0], x)};
 }
 
 struct RotaryNode : public torch::autograd::Function<RotaryNode> {
@@ -375,14 +399,58 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
   }
 };
 
+struct RotaryTables {
+  Tensor cos, sin;
+  OptTensor positions;
+};
+
+// The arguments of a rotation as its kernel takes them: tables [positions, R / 2] (or [1, positions, 1, R / 2]) in fp32
+RotaryTables rotary_args(const char* op, const Tensor& q, const OptTensor& k, Tensor cos, Tensor sin, const OptTensor& positions) {
+  refuse(q.dim() != 4 || (given(k) && k->dim() != 4), op, " needs [batch, tokens, heads, head_dim], got ", q.sizes());
+  const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
+  if (given(k))
+    refuse(k->size(0) != B || k->size(1) != T || k->size(3) != D || k->scalar_type() != q.scalar_type() || k->device() != q.device(), op,
+           ": q ", q.sizes(), " ", q.scalar_type(), " on ", q.device(), " and k ", k->sizes(), " ", k->scalar_type(), " on ", k->device(),
+           " differ in more than their heads");
+  refuse(cos.device() != q.device() || sin.device() != q.device() || (given(positions) && positions->device() != q.device()), op,
+         ": q is on ", q.device(), ", its tables or positions are not");
+  refuse(cos.requires_grad() || sin.requires_grad(), op, ": the tables are constants, but one of them requires a gradient");
+  if (cos.dim() == 4 && cos.size(0) == 1 && cos.size(2) == 1) {
+    cos = cos.select(0, 0).select(1, 0);
+    if (sin.dim() == 4) sin = sin.reshape({sin.size(1), sin.size(3)});
+  }
+  refuse(cos.dim() != 2 || cos.sizes() != sin.sizes() || !cos.is_floating_point(), op, ": cos and sin must be [positions, rotated / 2], got ",
+         cos.sizes(), " and ", sin.sizes());
+  refuse(2 * cos.size(1) > D, op, ": tables for ", 2 * cos.size(1), " values of heads of ", D);
+  OptTensor at = positions;
+  if (given(positions)) {
+    const auto type = positions->scalar_type();
+    refuse(type != at::kInt && type != at::kLong, op, ": positions must be int32 or int64, got ", type);
+    const bool one = positions->dim() == 1 && positions->size(0) == T;
+    const bool all = positions->dim() == 2 && positions->size(1) == T && (positions->size(0) == B || positions->size(0) == 1);
+    refuse(!one && !all, op, ": positions ", positions->sizes(), " for ", B, " sequences of ", T, " tokens");
+    refuse(cos.size(0) < 1, op, ": empty tables");
+    if (!positions->is_contiguous()) at = positions->contiguous();
+  } else {
+    refuse(T > cos.size(0), op, ": tables of ", cos.size(0), " positions for sequences of ", T, " tokens");
+  }
+  if (cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat || cos.strides() != sin.strides() || cos.stride(1) != 1) {
+    cos = cos.to(at::kFloat).contiguous();
+    sin = sin.to(at::kFloat).contiguous();
+  }
+  return {cos, sin, at};
+}
+
 Tensor rotary_one(const Tensor& q, const Tensor& cos, const Tensor& sin, const OptTensor& positions, bool interleaved) {
-  if (wants_grad({&q})) return RotaryNode::apply(q, OptTensor(), cos, sin, positions, interleaved)[0];
-  return rotary(heads4(q), OptTensor(), cos, sin, positions, interleaved, 1.0)[0];
+  const auto a = rotary_args("rotary", q, OptTensor(), cos, sin, positions);
+  if (wants_grad({&q})) return RotaryNode::apply(q, OptTensor(), a.cos, a.sin, a.positions, interleaved)[0];
+  return rotary(heads4(q), OptTensor(), a.cos, a.sin, a.positions, interleaved, 1.0)[0];
 }
 std::tuple<Tensor, Tensor> rotary_qk(const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin,
                                      const OptTensor& positions, bool interleaved) {
-  auto out = wants_grad({&q, &k}) ? RotaryNode::apply(q, OptTensor(k), cos, sin, positions, interleaved)
-                                  : rotary(heads4(q), heads4(k), cos, sin, positions, interleaved, 1.0);
+  const auto a = rotary_args("rotary_qk", q, k, cos, sin, positions);
+  auto out = wants_grad({&q, &k}) ? RotaryNode::apply(q, OptTensor(k), a.cos, a.sin, a.positions, interleaved)
+                                  : rotary(heads4(q), heads4(k), a.cos, a.sin, a.positions, interleaved, 1.0);
   return {out[0], out[1]};
 }
 
@@ -420,13 +488,32 @@ struct KlTopkNode : public torch::autograd::Function<KlTopkNode> {
 
 // reduction: 0 mean, 1 sum, 2 none
 Tensor kl_topk(const Tensor& student, const Tensor& values, const Tensor& index, const OptTensor& lse, double tau, int64_t reduction) {
+  refuse(student.dim() < 1 || student.size(-1) < 1, "kl_topk_logits: student must be [.., V], got ", student.sizes());
+  refuse(!(tau >= 1e-20 && tau <= 1e20), "kl_topk_logits: temperature must be from 1e-20 to 1e20, got ", tau);
+  refuse((index.scalar_type() != at::kInt && index.scalar_type() != at::kLong) || !values.is_floating_point(),
+         "kl_topk_logits: teacher_values must be floating-point and teacher_index int32 or int64, got ", values.scalar_type(), " and ",
+         index.scalar_type());
+  const auto rows = student.sizes().slice(0, student.dim() - 1);
+  refuse(index.dim() != student.dim() || index.size(-1) < 1 || index.sizes() != values.sizes() ||
+         index.sizes().slice(0, index.dim() - 1) != rows, "kl_topk_logits: teacher_values ", values.sizes(), " and teacher_index ",
+         index.sizes(), " for rows ", rows);
+  refuse(values.device() != student.device() || index.device() != student.device() || (given(lse) && lse->device() != student.device()),
+         "kl_topk_logits: the student is on ", student.device(), ", the teacher is not");
+  if (given(lse))
+    refuse(lse->sizes() != rows || !lse->is_floating_point(), "kl_topk_logits: teacher_lse ", lse->sizes(), " ", lse->scalar_type(),
+           " for rows ", rows);
+  const int64_t K = index.size(-1), n = K > 0 ? index.numel() / K : 0;
+  auto flat = [&](const Tensor& t) { return (t.dim() == 2 ? t : t.reshape({n, K})).contiguous(); };
+  const bool taken = values.scalar_type() == at::kFloat || values.scalar_type() == at::kBFloat16;
+  const Tensor v = flat(taken ? values : values.to(at::kFloat)), i = flat(index.scalar_type() == at::kLong ? index : index.to(at::kLong));
+  const OptTensor l = given(lse) ? OptTensor(f32_flat(*lse, n)) : OptTensor();
   if (wants_grad({&student})) {
-    const Tensor flat = student.dim() == 2 ? student : student.reshape({-1, student.size(-1)});
-    Tensor out = KlTopkNode::apply(flat, values, index, lse, tau, reduction);
-    return reduction == 2 ? out.view(student.sizes().slice(0, student.dim() - 1)) : out;
+    const Tensor s2 = student.dim() == 2 ? student : student.reshape({n, student.size(-1)});
+    Tensor out = KlTopkNode::apply(s2, v, i, l, tau, reduction);
+    return reduction == 2 && student.dim() != 2 ? out.view(rows) : out;
   }
-  auto out = kl_topk_fwd(rows2(student), values, index, lse, tau, reduction != 2, reduction == 0, OptTensor(), false, false);
-  return reduction == 2 ? out[1].view(student.sizes().slice(0, student.dim() - 1)) : out[0];
+  auto out = kl_topk_fwd(rows2(student), v, i, l, tau, reduction != 2, reduction == 0, OptTensor(), false, false);
+  return reduction == 2 ? out[1].view(rows) : out[0];
 }
 
 struct RouteNode : public torch::autograd::Function<RouteNode> {
@@ -463,10 +550,18 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
 std::tuple<Tensor, Tensor, Tensor, OptTensor> route(const Tensor& logits, const OptTensor& bias, int64_t k, bool softmax, int64_t groups,
                                                     int64_t top_groups, int64_t best, bool renorm, double scale, double aux_coef,
                                                     double z_coef) {
+  refuse(logits.dim() != 2 || logits.size(1) < 1, "route_experts needs [tokens, experts], got ", logits.sizes());
+  OptTensor steer = bias;
+  if (given(bias)) {
+    refuse(bias->dim() != 1 || bias->size(0) != logits.size(1) || !bias->is_floating_point() || bias->device() != logits.device(),
+           "route_experts: bias ", bias->sizes(), " ", bias->scalar_type(), " on ", bias->device(), " for ", logits.size(1), " experts on ",
+           logits.device());
+    if (bias->scalar_type() != at::kFloat || !bias->is_contiguous()) steer = bias->to(at::kFloat).contiguous();
+  }
   const bool need_aux = aux_coef != 0.0 || z_coef != 0.0;
   auto out = wants_grad({&logits})
-                 ? RouteNode::apply(logits, bias, k, softmax, groups, top_groups, best, renorm, scale, aux_coef, z_coef)
-                 : route_fwd(rows2(logits), bias, k, softmax, groups, top_groups, best, renorm, scale, need_aux, aux_coef, z_coef);
+                 ? RouteNode::apply(logits, steer, k, softmax, groups, top_groups, best, renorm, scale, aux_coef, z_coef)
+                 : route_fwd(rows2(logits), steer, k, softmax, groups, top_groups, best, renorm, scale, need_aux, aux_coef, z_coef);
   return {out[0], out[1], out[2], need_aux ? OptTensor(out[3]) : OptTensor()};
 }
 

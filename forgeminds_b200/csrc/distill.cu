@@ -672,10 +672,11 @@ int kl_dispatch(const KlParams& p, int dtype, int t_dtype, bool fwd, int* ws, bo
 using namespace fmb;
 
 extern "C" int fmb_kl_topk_fwd(const void* student, long long ld, const void* values, const long long* index, const float* lse,
-                               float* row_loss, float* stats, void* grad, long long ldg, const int* count, int* ws, float* loss,
-                               long long rows, int V, int K, float tau, int mean, int dtype, int t_dtype, cudaStream_t stream) {
+                               float* row_loss, float* stats, void* grad, long long ldg, const int* count, int* ws, int ws_ints,
+                               float* loss, long long rows, int V, int K, float tau, int mean, int dtype, int t_dtype, cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || K <= 0 || K > FMB_KL_MAX_KEEP || !(tau > 0.f)) return -2;
+  if (V <= 0 || K <= 0 || K > FMB_KL_MAX_KEEP || !(tau > 0.f) || ws == nullptr || ws_ints < FMB_KL_SCRATCH) return -2;
+  if (rows > 0x7fff0000LL) return -2;                      // rows are given out by a counter of 32 bits
   KlParams p = {};
   p.student = student; p.ld = ld; p.values = values; p.index = index; p.lse = lse; p.row_loss = row_loss;
   p.stats = reinterpret_cast<float2*>(stats); p.grad = grad; p.ldg = ldg; p.loss = loss; p.rows = rows; p.V = V; p.K = K;
@@ -688,7 +689,7 @@ extern "C" int fmb_kl_topk_bwd(const void* student, long long ld, const void* va
                                int upstream_rows, int skip_one, long long rows, int V, int K, float tau, int dtype, int t_dtype,
                                cudaStream_t stream) {
   if (rows <= 0) return 0;
-  if (V <= 0 || K <= 0 || K > FMB_KL_MAX_KEEP || !(tau > 0.f) || upstream == nullptr) return -2;
+  if (V <= 0 || K <= 0 || K > FMB_KL_MAX_KEEP || !(tau > 0.f) || upstream == nullptr || rows > 0x7fff0000LL) return -2;
   KlParams p = {};
   p.student = student; p.ld = ld; p.values = values; p.index = index; p.lse = lse;
   p.stats = const_cast<float2*>(reinterpret_cast<const float2*>(stats)); p.grad = grad; p.ldg = ldg; p.upstream = upstream;

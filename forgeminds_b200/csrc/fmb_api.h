@@ -87,14 +87,14 @@ int fmb_sum_f32(const float* x, float* out, long long n, float scale, int accumu
 
 // ---- distillation from a teacher's top logits (distill.cu)
 #define FMB_KL_MAX_KEEP 1024
-#define FMB_KL_SCRATCH 260
+#define FMB_KL_SCRATCH 260            // ints
 // Row losses, row statistics (float2: maximum, sum of exponentials) and, when given, the gradient for an upstream
-// gradient of 1 (rows `ldg` apart; may be the student itself). values / index [rows, K]; lse [rows] may be null. ws: two
-// ints of scratch, ws[0] receives the number of rows that count when `mean` and no `count` is given. loss (may be null):
-// the sum of the rows, divided by the count when `mean`.
+// gradient of 1 (rows `ldg` apart; may be the student itself). values / index [rows, K]; lse [rows] may be null. ws:
+// scratch of `ws_ints` >= FMB_KL_SCRATCH ints, ws[0] receives the number of rows that count when `mean` and no `count` is
+// given. loss (may be null): the sum of the rows, divided by the count when `mean`.
 int fmb_kl_topk_fwd(const void* student, long long ld, const void* values, const long long* index, const float* lse,
-                    float* row_loss, float* stats, void* grad, long long ldg, const int* count, int* ws, float* loss,
-                    long long rows, int V, int K, float tau, int mean, int dtype, int t_dtype, cudaStream_t stream);
+                    float* row_loss, float* stats, void* grad, long long ldg, const int* count, int* ws, int ws_ints,
+                    float* loss, long long rows, int V, int K, float tau, int mean, int dtype, int t_dtype, cudaStream_t stream);
 // The gradient for `upstream` (one number, or one per row). skip_one: rows whose upstream is 1 are there already.
 int fmb_kl_topk_bwd(const void* student, long long ld, const void* values, const long long* index, const float* lse,
                     const float* stats, void* grad, long long ldg, const int* count, const float* upstream,

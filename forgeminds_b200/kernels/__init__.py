@@ -279,9 +279,19 @@ def softmax(x: torch.Tensor, dim: int = -1, dtype: torch.dtype | None = None) ->
 
 
 # ------------------------------------------------------------------------------ LayerNorm
+# The kernels' path of the functions below goes straight to the extension: its C++ side checks the arguments (ValueError, as
+# here) and holds the autograd nodes. SMALL: sizes within which every limit of the kernels holds.
+SMALL = 2 ** 24
+
+
 def _rw():
     from ..ops import rowwise
     return rowwise
+
+
+def _ext():
+    from .. import ops
+    return ops._mod or ops.require()
 
 
 def _one_device(name: str, first: torch.Tensor, *others) -> None:
@@ -306,7 +316,7 @@ _MOST_ROWS = 2 ** 31 - 2 ** 16        # rows that the kernels number in 31 bits
 
 
 def _ln_fast(x, *rest) -> bool:
-    return x.shape[-1] <= 2 ** 24 and x.numel() // x.shape[-1] < _MOST_ROWS and fast_ok(x, *rest)
+    return (x.numel() < SMALL or (x.shape[-1] <= 2 ** 24 and x.numel() // x.shape[-1] < _MOST_ROWS)) and fast_ok(x, *rest)
 
 
 def layer_norm(x: torch.Tensor, w: torch.Tensor | None = None, b: torch.Tensor | None = None,
@@ -314,9 +324,9 @@ def layer_norm(x: torch.Tensor, w: torch.Tensor | None = None, b: torch.Tensor |
     """``(x - mean) / sqrt(var + eps) * w + b`` over the last dimension (``var`` is the mean square deviation); ``w`` and
     ``b`` are fp32 or of ``x``'s type and may each be left out. Statistics and the gradients of ``w`` and ``b`` are summed
     in fp32, in an order that does not change from run to run."""
-    _check_layer_norm("layer_norm", x, w, b)
     if _ln_fast(x, w, b):
-        return _rw().layer_norm(x, w, b, float(eps))
+        return _ext().layer_norm(x, w, b, eps)
+    _check_layer_norm("layer_norm", x, w, b)
     return _ref.layer_norm(x, w, b, eps)
 
 
@@ -324,13 +334,13 @@ def add_layer_norm(x: torch.Tensor, delta: torch.Tensor, w: torch.Tensor | None 
                    eps: float = 1e-5):
     """Residual add and norm in one pass: returns ``(x + delta, layer_norm(x + delta, w, b))``. The norm is that of the sum
     as it is stored in ``x``'s type."""
+    if _ln_fast(x, delta, w, b):
+        return _ext().add_layer_norm(x, delta, w, b, eps)
     _check_layer_norm("add_layer_norm", x, w, b)
     if x.shape != delta.shape or x.dtype != delta.dtype:
         raise ValueError(f"add_layer_norm needs two tensors of one shape and type, got {tuple(x.shape)} {x.dtype} and "
                          f"{tuple(delta.shape)} {delta.dtype}")
     _one_device("add_layer_norm", x, delta)
-    if _ln_fast(x, delta, w, b):
-        return _rw().add_layer_norm(x, delta, w, b, float(eps))
     return _ref.add_layer_norm(x, delta, w, b, eps)
 
 
@@ -401,17 +411,21 @@ def _rotary_args(name, x, k, cos, sin, positions):
 
 
 def _rotary(name, x, k, cos, sin, positions, interleaved):
+    if cos.shape[-1:] != (0,) and _rotary_small(x, k) and fast_ok(x, k):
+        if k is None:
+            return _ext().rotary_one(x, cos, sin, positions, interleaved)
+        return _ext().rotary_qk(x, k, cos, sin, positions, interleaved)
     cos, sin = _rotary_args(name, x, k, cos, sin, positions)
-    if cos.shape[1] and x.numel() + (0 if k is None else k.numel()) and x.shape[-1] <= 2 ** 16 \
-            and x.shape[0] * x.shape[1] < 2 ** 31 and fast_ok(x, k):
-        if cos.dtype != torch.float32 or cos.stride() != sin.stride() or cos.stride(1) != 1:
-            cos, sin = cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
-        if positions is not None and not positions.is_contiguous():
-            positions = positions.contiguous()
-        return _rw().rotary(x, k, cos, sin, positions, bool(interleaved))
     if k is None:
         return _ref.rotary(x, cos, sin, positions, interleaved)
     return _ref.rotary(x, cos, sin, positions, interleaved), _ref.rotary(k, cos, sin, positions, interleaved)
+
+
+def _rotary_small(x, k) -> bool:
+    if 0 < x.numel() < 2 ** 16:
+        return True
+    heads = x.shape[2] + (0 if k is None else k.shape[2]) if x.dim() == 4 and (k is None or k.dim() == 4) else 0
+    return 0 < heads <= 2 ** 24 and 0 < x.shape[3] <= 2 ** 16 and 0 < x.shape[0] * x.shape[1] < 2 ** 31
 
 
 def rotary(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor | None = None,
@@ -433,8 +447,8 @@ def rotary_qk(q: torch.Tensor, k: torch.Tensor, cos: torch.Tensor, sin: torch.Te
 
 # ------------------------------------------------------------------------------ distillation from top logits
 def _kl_topk_args(name, rows_shape, vocab, values, index, temperature, lse):
-    if not temperature > 0 or math.isinf(temperature):
-        raise ValueError(f"{name}: temperature must be positive and finite, got {temperature}")
+    if not 1e-20 <= temperature <= 1e20:
+        raise ValueError(f"{name}: temperature must be from 1e-20 to 1e20, got {temperature}")
     if index.dtype not in (torch.int32, torch.int64) or not values.is_floating_point():
         raise ValueError(f"{name}: teacher_values must be floating-point and teacher_index int32 or int64, got {values.dtype} "
                          f"and {index.dtype}")
@@ -476,13 +490,13 @@ def kl_topk_logits(student: torch.Tensor, teacher_values: torch.Tensor, teacher_
     other rows. An index that stands twice counts twice."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean|sum|none, got {reduction!r}")
+    if _kl_small(student, teacher_index) and fast_ok(student):
+        return _ext().kl_topk(student, teacher_values, teacher_index, teacher_lse, temperature, _REDUCTIONS[reduction])
     if student.dim() < 1 or not student.is_floating_point():
         raise ValueError(f"kl_topk_logits: student must be floating-point [.., V], got {tuple(student.shape)} {student.dtype}")
     V = student.shape[-1]
     _one_device("kl_topk_logits", student, teacher_values, teacher_index, teacher_lse)
     values, index, lse = _kl_topk_args("kl_topk_logits", student.shape[:-1], V, teacher_values, teacher_index, temperature, teacher_lse)
-    if V <= 2 ** 24 and index.shape[1] <= _KL_MAX_KEEP and index.shape[0] < 2 ** 31 and fast_ok(student):
-        return _rw().kl_topk(student, *_kl_topk_native(values, index, lse), float(temperature), reduction)
     rows = _ref.kl_topk(student.reshape(-1, V), values, index, lse, temperature)
     if reduction == "none":
         return rows.view(student.shape[:-1])
@@ -495,6 +509,12 @@ def _wide_sum(t: torch.Tensor) -> torch.Tensor:
     return (t if t.dtype == torch.float64 else t.float()).sum()
 
 
+def _kl_small(student: torch.Tensor, index: torch.Tensor) -> bool:
+    return student.dim() > 0 and index.dim() > 0 and index.shape[-1] <= _KL_MAX_KEEP and \
+        (student.numel() < SMALL or (student.shape[-1] <= 2 ** 24 and student.numel() // student.shape[-1] < _MOST_ROWS))
+
+
+_REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 _KL_MAX_KEEP = 1024          # FMB_KL_MAX_KEEP: more kept logits than this take the PyTorch path
 
 
@@ -512,7 +532,7 @@ def kl_topk_distill_loss(hs: torch.Tensor, w: torch.Tensor, teacher_values: torc
                                        teacher_lse)
     s2 = hs.reshape(-1, hs.shape[-1])
     n = s2.shape[0]
-    native = V <= 2 ** 24 and index.shape[1] <= _KL_MAX_KEEP and n < 2 ** 31 and fast_ok(hs)
+    native = V <= 2 ** 24 and index.shape[1] <= _KL_MAX_KEEP and n < _MOST_ROWS and fast_ok(hs)
     if native:
         values, index, lse = _kl_topk_native(values, index, lse)
     counts = _ref.kl_topk_counts(values, index, V).any(dim=-1).sum().clamp(min=1)
@@ -523,7 +543,7 @@ def kl_topk_distill_loss(hs: torch.Tensor, w: torch.Tensor, teacher_values: torc
         part = slice(lo, lo + chunk)
         logits = s2[part] @ w.to(s2.dtype).t()
         some = None if lse is None else lse[part]
-        rows = _rw().kl_topk(logits, values[part], index[part], some, float(temperature), "sum") if native else \
+        rows = _ext().kl_topk(logits, values[part], index[part], some, float(temperature), _REDUCTIONS["sum"]) if native else \
             _ref.kl_topk(logits, values[part], index[part], some, temperature).sum()
         total = rows if total is None else total + rows
     return total / counts
@@ -560,19 +580,16 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
     coefficients are 0. A token whose logits are all ``-inf`` has scores of 0; weights of chosen scores that are all 0 are 0."""
     if logits.dim() != 2 or not logits.is_floating_point() or logits.shape[1] < 1:
         raise ValueError(f"route_experts needs floating-point [tokens, experts], got {tuple(logits.shape)} {logits.dtype}")
-    E = logits.shape[1]
+    N, E = logits.shape
     check_route(E, k, score, n_groups, top_groups, group_best)
+    args = (n_groups, top_groups, group_best, bool(renormalise), scale, aux_coef, z_coef)
+    if E <= ROUTE_MAX_EXPERTS and k <= ROUTE_MAX_K and n_groups <= ROUTE_MAX_GROUPS and N * k < _MOST_ROWS and fast_ok(logits):
+        return _ext().route(logits, bias, k, score == "softmax", *args)
     if bias is not None:
         if tuple(bias.shape) != (E,) or not bias.is_floating_point():
             raise ValueError(f"route_experts: bias {tuple(bias.shape)} {bias.dtype} for {E} experts")
         _one_device("route_experts", logits, bias)
         bias = bias.detach()
-    args = (n_groups, top_groups, group_best, bool(renormalise), float(scale), float(aux_coef), float(z_coef))
-    if E <= ROUTE_MAX_EXPERTS and k <= ROUTE_MAX_K and n_groups <= ROUTE_MAX_GROUPS and logits.shape[0] * k < _MOST_ROWS \
-            and fast_ok(logits):
-        if bias is not None and (bias.dtype != torch.float32 or not bias.is_contiguous()):
-            bias = bias.to(torch.float32).contiguous()
-        return _rw().route(logits, bias, int(k), score == "softmax", *args)
     return _ref.route_experts(logits, int(k), score == "softmax", bias, *args)
 
 

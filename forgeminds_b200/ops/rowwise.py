@@ -1,9 +1,9 @@
-"""LayerNorm, rotary positions, distillation from top logits and expert routing on the kernels (GPU only;
-:mod:`forgeminds_b200.kernels` checks arguments and picks the PyTorch path elsewhere).
+"""Output head and distillation from a teacher's top logits in one Function (GPU only; ``fm.kernels.kl_topk_distill_loss``
+checks arguments and picks the PyTorch path elsewhere).
 
-``layer_norm``, ``rotary_qk``, ``kl_topk`` and ``route`` are differentiable as they come out of the extension: their
-autograd nodes are C++ (``csrc/bindings_rows.cpp``), which keeps what their backward kernels read: row statistics instead
-of normalised values, the choice and its weights instead of scores.
+The row operators themselves (``layer_norm``, ``rotary_qk``, ``kl_topk``, ``route``) are differentiable as they come out of
+the extension: their autograd nodes are C++ (``csrc/bindings_rows.cpp``), which keeps what their backward kernels read: row
+statistics instead of normalised values, the choice and its weights instead of scores.
 """
 from __future__ import annotations
 
@@ -14,34 +14,8 @@ from . import require
 from .functional import BF16, bf16_of, gemm
 
 F32 = torch.float32
-REDUCTIONS = {"mean": 0, "sum": 1, "none": 2}
 
 
-def layer_norm(x, w, b, eps):
-    return require().layer_norm(x, w, b, eps)
-
-
-def add_layer_norm(x, delta, w, b, eps):
-    """``(x + delta, layer_norm(x + delta))`` from one pass over the row."""
-    return require().add_layer_norm(x, delta, w, b, eps)
-
-
-def rotary(q, k, cos, sin, positions, interleaved):
-    if k is None:
-        return require().rotary_one(q, cos, sin, positions, interleaved)
-    return require().rotary_qk(q, k, cos, sin, positions, interleaved)
-
-
-def kl_topk(student, values, index, lse, tau, reduction):
-    return require().kl_topk(student, values, index, lse, tau, REDUCTIONS[reduction])
-
-
-def route(logits, bias, k, softmax, groups, top_groups, best, renorm, scale, aux_coef, z_coef):
-    """``logits [N, E]`` -> ``(weights fp32 [N, k], idx int32 [N, k], counts int32 [E], aux fp32 or None)``."""
-    return require().route(logits, bias, k, softmax, groups, top_groups, best, renorm, scale, aux_coef, z_coef)
-
-
-# ------------------------------------------------------------------------------ head and distillation loss
 class _LinearKLTopK(torch.autograd.Function):
     """Mean top-logit KL of ``h @ W.T`` without fp32 logits: each chunk of bf16 logits becomes its gradient in place;
     the two gradient products run once in the backward pass, scaled by the incoming gradient on the device."""
