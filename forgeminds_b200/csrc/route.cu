@@ -8,10 +8,12 @@
 //
 // Forward: LPT lanes share a token, each with VPL neighbouring experts. The order must be that of the exact scores. What
 // is compared are whole numbers of 32 bits: 23 bits of the score in fixed point, 9 of the expert's number, so that one
-// maximum finds value and expert and no two are equal. Each lane sorts its own by a network once; a round of the choice is
-// then a maximum over the lanes' first ones. A token where two neighbours of the order are nearer than the errors of score
-// and fixed point, and not equal by their inputs, is decided again in 64 bits; so is one with NaN or +inf.
-// Bound by these instructions (about 350 per token of 256 experts and 8 choices), not by memory.
+// maximum finds value and expert and no two are equal. Each lane lists its four largest by a network once; a round of the
+// choice is then a maximum over the lanes' first ones. A token where two neighbours of the order are nearer than the errors
+// of score and fixed point, and not equal by their inputs, is decided again, in 64 bits where it must be; so is one with NaN
+// or +inf, and one of which a lane has given away its four.
+// Bound by these instructions (600 per token of 256 experts in 8 groups and 8 choices), not by memory: 65536 such tokens in
+// 56 us at two thirds of the issue slots, 17 us of memory traffic; their backward pass, all zeros but for 8 values, 18 us.
 #include "fmb_api.h"
 #include "launch.cuh"
 #include "rows.cuh"
@@ -53,9 +55,9 @@ __device__ __forceinline__ void load_logits(const T* row, int lane, int E, int v
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
 
 // A token's choice in 64 bits by its LPT lanes: writes the chosen experts to pick[0, k). c, g: shared memory for E scores
-// and the groups'. Rare, and 30000 cycles long: a pair of neighbours alone is put in order without it.
+// and the groups'. Rare, and tens of thousands of cycles long: a pair of neighbours alone is put in order without it.
 template <typename T, int LPT, int VPL>
-__device__ __noinline__ void choose_exactly(const RouteParams& p, const T* row, int lane, double* c, double* g, int* pick) {
+__device__ __forceinline__ void choose_exactly(const RouteParams& p, const T* row, int lane, double* c, double* g, int* pick) {
   const int e0 = lane * VPL;
   double own[VPL];
   double top = -CUDART_INF, sum = 0.0;
@@ -178,6 +180,34 @@ template <int N> __device__ __forceinline__ void sort_falling(unsigned (&v)[N]) 
           }
 }
 
+// The four largest (or all, of fewer) in falling order: fours sorted, then merged with the best four so far (32 minima and
+// maxima for 8, where the whole order takes 38; and the rounds move four registers, not eight).
+constexpr int LIST = 4;
+template <int N, int L> __device__ __forceinline__ void top_falling(const unsigned (&v)[N], unsigned (&list)[L]) {
+  static_assert(L == (N < LIST ? N : LIST) && (N <= LIST || N % LIST == 0), "whole fours");
+#pragma unroll
+  for (int i = 0; i < L; ++i) list[i] = v[i];
+  sort_falling(list);
+#pragma unroll
+  for (int from = L; from < N; from += L) {
+    unsigned more[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) more[i] = v[from + i];
+    sort_falling(more);
+#pragma unroll
+    for (int i = 0; i < L; ++i) list[i] = max(list[i], more[L - 1 - i]);
+#pragma unroll
+    for (int o = L / 2; o > 0; o >>= 1)
+#pragma unroll
+      for (int i = 0; i < L; ++i)
+        if (!(i & o)) {
+          const unsigned a = list[i], b = list[i + o];
+          list[i] = max(a, b);
+          list[i + o] = min(a, b);
+        }
+  }
+}
+
 // VPL neighbouring experts' logits; -inf where there is none
 template <typename T, int VPL> __device__ __forceinline__ void load_own(const T* row, int e0, int E, int vec, float (&z)[VPL]) {
   constexpr int BYTES = VPL * sizeof(T);
@@ -201,23 +231,61 @@ template <typename T, int VPL> __device__ __forceinline__ void load_own(const T*
   }
 }
 
+// Keys of a lane's experts by their scores, and by their logits (without a bias the order is the same). bias: in fixed
+// point. fp32 logits: 32 units below the largest one in 23 bits.
+template <int VPL>
+__device__ __forceinline__ void keys_by_score(bool softmax, const float (&z)[VPL], const float (&bias)[VPL], float top, float inv_mass,
+                                              float unit, int e0, unsigned (&key)[VPL]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    const float c = softmax ? exp2_unit((z[i] - top) * 1.4426950408889634f) * inv_mass : sigmoid_near(z[i]);
+    key[i] = route_key(fmaf(c, unit, bias[i]), e0 + i);
+  }
+}
+// bf16: the 16 bits themselves, turned so that their order is the numbers' (and -0 is 0): no two logits share a score.
+template <typename T, int VPL>
+__device__ __forceinline__ void keys_by_logit(const float (&z)[VPL], float high, int e0, unsigned (&key)[VPL]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    if constexpr (sizeof(T) == 2) {
+      const unsigned b = __float_as_uint(z[i] + 0.f);
+      key[i] = ((b ^ (static_cast<unsigned>(static_cast<int>(b) >> 31) | 0x80000000u)) >> 16 << NUMBER_BITS) + (NUMBER - (e0 + i));
+    } else {
+      key[i] = route_key(fmaf(z[i] - high, 262144.f, 16777215.f), e0 + i);
+    }
+  }
+}
+__device__ __forceinline__ float fixed_bias(float bias, float lo, float unit) { return fmaf(bias - lo, unit, 8388608.f); }
+
+// One round of a choice: the largest first key of LPT lanes, whose lane moves on to its next one.
+template <int LPT, int N> __device__ __forceinline__ unsigned take_largest(unsigned (&list)[N]) {
+  const unsigned w = lanes_umax<LPT>(list[0]);
+  if (list[0] == w) {
+#pragma unroll
+    for (int i = 0; i + 1 < N; ++i) list[i] = list[i + 1];
+    list[N - 1] = 0;
+  }
+  return w;
+}
+
 // Whether expert b comes before expert a by their exact scores (sigmoids with their biases).
-__device__ __noinline__ bool sigmoid_ahead(float za, float zb, float bias_a, float bias_b, bool lower) {
+__device__ __forceinline__ bool sigmoid_ahead(float za, float zb, float bias_a, float bias_b, bool lower) {
   const double a = 1.0 / (1.0 + exp(-static_cast<double>(za))) + static_cast<double>(bias_a);
   const double b = 1.0 / (1.0 + exp(-static_cast<double>(zb))) + static_cast<double>(bias_b);
   return b > a || (b == a && lower);
 }
 
-// The choice of a warp's tokens where some neighbours j, j + 1 of key[0, k + 2) are within `apart`, or a token is in doubt
-// already: pairs that stand alone are put in order, other tokens decided again. Writes pick[0, k).
+// The choice of a warp's tokens where some neighbours j, j + 1 of key[0, k + 2) are closer than `apart`, or a token is in
+// doubt already: pairs that stand alone are put in order, other tokens decided again. Writes pick[0, k).
 template <typename T, int LPT, int VPL>
-__device__ __noinline__ void settle(const RouteParams& p, const T* row, int lane, unsigned apart, bool doubt, bool flat_bias,
-                                    const unsigned* key, int* pick, double* c64, double* g64) {
+__device__ __forceinline__ void settle(const RouteParams& p, const T* row, int lane, unsigned apart, bool doubt, bool flat_bias,
+                                       const unsigned* key, int* pick, double* c64, double* g64) {
   const bool biased = p.bias != nullptr;
-  auto close = [&](int j) { return key[j] != 0 && key[j + 1] != 0 && key_score(key[j]) - key_score(key[j + 1]) <= apart; };
+  auto close = [&](int j) { return key[j] != 0 && key[j + 1] != 0 && key_score(key[j]) - key_score(key[j + 1]) < apart; };
   for (int j = lane; j < p.k; j += LPT) pick[j] = min(key_expert(key[j]), p.E - 1);
   __syncwarp();
   for (int j = lane; j < p.k; j += LPT) {
+    doubt |= key[j] == 0;                                  // fewer keys than choices
     if (!close(j)) continue;
     const int a = key_expert(key[j]), b = key_expert(key[j + 1]);
     const float za = to_f32(row[a]), zb = to_f32(row[b]);
@@ -256,307 +324,403 @@ __device__ __noinline__ void settle(const RouteParams& p, const T* row, int lane
   __syncwarp();
 }
 
+// What is the same for all tokens of a thread
+template <int LPT, int VPL> struct RouteLane {
+  int lane, e0;
+  bool biased, grouped, by_score;                          // by_score: else the order of the logits is the scores'
+  bool whole_lanes, has_group, two_best;                   // whole_lanes: groups are a power of two of whole lanes
+  int span;
+  unsigned own_group;
+  __device__ __forceinline__ explicit RouteLane(const RouteParams& p) {
+    lane = threadIdx.x % LPT;
+    e0 = lane * VPL;
+    biased = p.bias != nullptr;
+    grouped = p.groups > 1;
+    by_score = biased || (grouped && p.best > 1);
+    span = p.gsize / VPL;
+    whole_lanes = p.gsize % VPL == 0 && (span & (span - 1)) == 0 && span <= LPT;
+    own_group = grouped && whole_lanes ? lane / span : 0;
+    has_group = own_group < static_cast<unsigned>(p.groups);
+    two_best = p.best > 1 && p.gsize > 1;
+  }
+};
+
+// Shared memory of a token: for the choice in 64 bits scores [E] and groups' [groups], keys [k + 2] and choices [k]; and
+// the block's counts [E]
+struct RouteRoom {
+  double *c64, *g64;
+  unsigned* key;
+  int *pick, *count;
+};
+
+// The fixed point of biased scores: what 0 is, steps per score, and how near two scores may be without being told apart
+struct RouteScale {
+  float lo, unit;
+  unsigned near;
+  bool bad_bias, flat_bias;                                // NaN or +inf: every choice is made in 64 bits; one finite bias for all
+};
+
+// Chooses for the LPT lanes' token and writes its weights, choice and counts. Not EXACT: returns false, and writes nothing
+// for any token of the warp, if one of them is left open by 32 bits or by the lists of its lanes. `loaded` is called once
+// the logits are used up. acc, acc_z: sums for the auxiliary loss.
+template <typename T, int LPT, int VPL, bool EXACT, bool AUX, typename F>
+__device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT, VPL>& me, const RouteScale& scale, const RouteRoom& room,
+                                       int token, bool live, const T* row, const float (&z)[VPL], const float (&bias)[VPL],
+                                       float* acc, float& acc_z, F&& loaded) {
+  constexpr int MOST_K = LPT * VPL < FMB_ROUTE_MAX_K ? LPT * VPL : FMB_ROUTE_MAX_K, PER = (MOST_K + LPT - 1) / LPT;
+  constexpr int L = EXACT || VPL < LIST ? VPL : LIST;
+  const int lane = me.lane, e0 = me.e0;
+  float top = z[0], mass = 1.f;
+#pragma unroll
+  for (int i = 1; i < VPL; ++i) top = max_or_nan(top, z[i]);
+  bool doubt = scale.bad_bias || !(top < CUDART_INF_F);     // NaN or +inf, or an order that fp32 leaves open
+  if (p.softmax || AUX || !me.biased) top = lanes_max<LPT>(top);
+  const float high = top;                                   // (of this lane alone where nothing needs the row's)
+  if (p.softmax || AUX) {
+    if (top == -CUDART_INF_F) top = 0.f;                    // a row of nothing but -inf: scores of 0
+    mass = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) mass += e0 + i < p.E ? expf(z[i] - top) : 0.f;
+    mass = lanes_sum<LPT>(mass);
+    if (mass == 0.f) mass = 1.f;
+  }
+  if constexpr (AUX) {
+    float norm = mass;
+    if (!p.softmax) {
+      norm = 0.f;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) norm += e0 + i < p.E ? sigmoid(z[i]) : 0.f;
+      norm = lanes_sum<LPT>(norm);
+      if (norm == 0.f) norm = 1.f;
+    }
+    if (live) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (e0 + i < p.E) acc[i] += (p.softmax ? expf(z[i] - top) : sigmoid(z[i])) / norm;
+      const float lse = top + logf(mass);
+      if (lane == 0) acc_z += lse * lse;
+    }
+  }
+  // fixed-point scores and keys; first, second: the lane's two largest for its group where the lists do not hold them
+  unsigned key[VPL], list[L], first = 0, second = 0;
+  const bool lists_serve = me.biased || !me.by_score;
+  unsigned* s_n = reinterpret_cast<unsigned*>(room.c64);    // groups that are no whole lanes: the token's fixed-point scores
+  auto see = [&](unsigned v, int e) {
+    if (e < p.E) {
+      if (!lists_serve) {
+        second = max(second, min(first, v));
+        first = max(first, v);
+      }
+      if (!me.whole_lanes) s_n[e] = key_score(v);
+    }
+  };
+  if (me.grouped && !me.whole_lanes) __syncwarp();          // the scores of the token before have been read
+  if (me.by_score) {
+    keys_by_score<VPL>(p.softmax, z, bias, top, p.softmax ? __fdividef(1.f, mass) : 1.f, scale.unit, e0, key);
+    if (me.grouped && !(lists_serve && me.whole_lanes)) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
+    }
+  }
+  if (!me.biased) {
+    keys_by_logit<T, VPL>(z, high, e0, key);
+    if (me.grouped && !me.by_score && !me.whole_lanes) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
+    }
+  }
+  loaded();
+  if (e0 + VPL > p.E) {                                     // the last expert's key is above 0: its number is
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e0 + i >= p.E) key[i] = 0;
+  }
+  auto make_list = [&]() {
+    if constexpr (L == VPL) {
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) list[i] = key[i];
+      sort_falling(list);
+    } else {
+      top_falling(key, list);
+    }
+  };
+  const unsigned by_logit = sizeof(T) == 2 ? 0u : 4u;       // bf16 logits' keys are exact
+  if (me.grouped) {
+    unsigned low = 0, out = 0;                              // the lowest group kept and the highest left out
+    if (me.whole_lanes) {
+      make_list();
+      unsigned a = lists_serve ? list[0] : first, b = lists_serve ? (L > 1 ? list[L > 1 ? 1 : 0] : 0u) : second;
+      for (int o = 1; o < me.span; o *= 2) {                // the lane's two largest, then the group's
+        const unsigned oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+        b = max(max(b, ob), min(a, oa));
+        a = max(a, oa);
+      }
+      // the group's score above 31 - its number, the same in all its lanes
+      unsigned mine = me.has_group ? (key_score(a) + (me.two_best ? key_score(b) : 0u)) << 5 | (31 - me.own_group) : 0u;
+      const unsigned whole = mine;
+#pragma unroll 1
+      for (int n = 0; n < p.top_groups; ++n) {
+        low = lanes_umax<LPT>(mine);
+        mine = mine == low ? 0 : mine;
+      }
+      out = lanes_umax<LPT>(mine);
+      if (whole < low || !me.has_group) {                   // a group that is left out
+#pragma unroll
+        for (int i = 0; i < L; ++i) list[i] = 0;
+      }
+    } else {
+      __syncwarp();
+      unsigned* s_g = reinterpret_cast<unsigned*>(room.g64);
+      for (int n = lane; n < p.groups; n += LPT) {
+        unsigned a = 0, b = 0;
+        for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
+          const unsigned v = s_n[e];
+          b = max(b, min(a, v));
+          a = max(a, v);
+        }
+        s_g[n] = (a + (me.two_best ? b : 0u)) << 5 | (31 - n);
+      }
+      __syncwarp();
+      unsigned kept = 0;
+      for (int n = lane; n < p.groups; n += LPT) {
+        int ahead = 0;
+        for (int m = 0; m < p.groups; ++m) ahead += s_g[m] > s_g[n];
+        if (ahead < p.top_groups) kept |= 1u << n;
+        if (ahead == p.top_groups - 1) low = s_g[n];
+        if (ahead >= p.top_groups) out = max(out, s_g[n]);
+      }
+#pragma unroll
+      for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+      low = lanes_umax<LPT>(low);
+      out = lanes_umax<LPT>(out);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i)
+        if (e0 + i < p.E && !(kept >> ((e0 + i) / p.gsize) & 1)) key[i] = 0;
+      __syncwarp();
+      make_list();
+    }
+    const unsigned apart = me.by_score ? 2 * scale.near : by_logit;
+    doubt |= p.top_groups < p.groups && (low >> 5) - (out >> 5) < apart;
+  } else {
+    make_list();
+  }
+  const bool longer = L < VPL && list[L - 1] != 0;          // there may be more behind the list
+  // k rounds of the largest first key, each kept by a lane of its own, and one more to see how far behind the next one is
+  unsigned mine[PER];
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    mine[n] = 0;
+#pragma unroll 4
+    for (int j = n * LPT; j < (n + 1) * LPT && j < p.k; ++j) {
+      const unsigned w = take_largest<LPT>(list);
+      if (lane == j - n * LPT) mine[n] = w;
+    }
+  }
+  const unsigned next = take_largest<LPT>(list);
+  bool open = longer && list[0] == 0;                       // this lane has given away its whole list
+  const unsigned apart = me.biased ? scale.near : by_logit;
+  int pick[PER];
+  unsigned after[PER];
+  bool hit = false;                                         // neighbours of the order that are too near to tell
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int j = n * LPT + lane;
+    after[n] = __shfl_down_sync(0xffffffffu, mine[n], 1, LPT);
+    if (n + 1 < PER) {
+      const unsigned turn = __shfl_sync(0xffffffffu, mine[n + 1 < PER ? n + 1 : n], 0, LPT);
+      if (lane == LPT - 1) after[n] = turn;
+    }
+    if (j == p.k - 1) after[n] = next;
+    pick[n] = min(key_expert(mine[n]), p.E - 1);            // (a token in doubt may have fewer keys than choices)
+    if (j < p.k) {
+      open |= mine[n] == 0;
+      hit |= after[n] != 0 && key_score(mine[n]) - key_score(after[n]) < apart;
+    }
+  }
+  open |= doubt;
+  if (__any_sync(0xffffffffu, hit || open)) {               // one token of this warp, or more: all its lanes go
+    const unsigned then = take_largest<LPT>(list);
+    if constexpr (EXACT) {
+#pragma unroll
+      for (int n = 0; n < PER; ++n)
+        if (n * LPT + lane < p.k) room.key[n * LPT + lane] = mine[n];
+      if (lane == 0) {
+        room.key[p.k] = next;
+        room.key[p.k + 1] = then;
+      }
+      __syncwarp();
+      settle<T, LPT, VPL>(p, row, lane, apart, doubt, !me.biased || scale.flat_bias, room.key, room.pick, room.c64, room.g64);
+#pragma unroll
+      for (int n = 0; n < PER; ++n)
+        if (n * LPT + lane < p.k) pick[n] = room.pick[n * LPT + lane];
+      __syncwarp();
+    } else {
+      // neighbours that are equal by their inputs are in order; at the last choice the next one might belong before both
+      if (hit) {
+#pragma unroll
+        for (int n = 0; n < PER; ++n) {
+          const int j = n * LPT + lane;
+          if (j < p.k && after[n] != 0 && key_score(mine[n]) - key_score(after[n]) < apart) {
+            const int b = key_expert(after[n]);
+            open |= to_f32(row[pick[n]]) != to_f32(row[b]) || (me.biased && p.bias[pick[n]] != p.bias[b]);
+            open |= j == p.k - 1 && then != 0 && key_score(next) - key_score(then) < apart;
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, open)) return false;
+    }
+  }
+  // weights of the chosen, each by a lane of its own
+  float sum = 0.f, best = -CUDART_INF_F, chosen[PER];
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int j = n * LPT + lane;
+    chosen[n] = j < p.k ? to_f32(row[pick[n]]) : -CUDART_INF_F;
+    best = fmaxf(best, chosen[n]);
+  }
+  if (p.softmax) best = lanes_max<LPT>(best);
+  // shares of the chosen alone are taken around their own maximum: they may all lie far below the row's
+  const float from = !p.renorm ? top : best == -CUDART_INF_F ? 0.f : best;
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    if (n * LPT + lane < p.k) {
+      chosen[n] = p.softmax ? expf(chosen[n] - from) / (p.renorm ? 1.f : mass) : sigmoid(chosen[n]);
+      sum += chosen[n];
+    }
+  }
+  sum = lanes_sum<LPT>(sum);
+  if (!p.softmax && p.renorm && __any_sync(0xffffffffu, sum < 1e-30f)) {
+    // sigmoids that vanish in fp32 still have shares: s = e^z there
+    const float peak = lanes_max<LPT>(best), around = peak == -CUDART_INF_F ? 0.f : peak;
+    float far = 0.f, share[PER];
+#pragma unroll
+    for (int n = 0; n < PER; ++n) {
+      share[n] = n * LPT + lane < p.k ? expf(to_f32(row[pick[n]]) - around) : 0.f;
+      far += share[n];
+    }
+    far = lanes_sum<LPT>(far);
+    if (sum < 1e-30f) {
+#pragma unroll
+      for (int n = 0; n < PER; ++n) chosen[n] = share[n];
+      sum = far;
+    }
+  }
+  const float by = !p.renorm ? p.scale : sum == 0.f ? 0.f : p.scale / sum;      // nothing to share out: weights of 0
+#pragma unroll
+  for (int n = 0; n < PER; ++n) {
+    const int j = n * LPT + lane;
+    if (j < p.k && live) {
+      const int e = pick[n];
+      p.weights[static_cast<long long>(token) * p.k + j] = chosen[n] * by;
+      p.idx[static_cast<long long>(token) * p.k + j] = e;
+      atomicAdd(room.count + e, 1);
+    }
+  }
+  __syncwarp();
+  return true;
+}
+
+template <typename T> __device__ __forceinline__ const T* route_row(const RouteParams& p, int token) {
+  return static_cast<const T*>(p.logits) + static_cast<long long>(token) * p.ld;
+}
+template <int VPL>
+__device__ __forceinline__ void load_bias(const RouteParams& p, int e0, const RouteScale& scale, float (&bias)[VPL]) {
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) bias[i] = fixed_bias(p.bias != nullptr && e0 + i < p.E ? p.bias[e0 + i] : 0.f, scale.lo, scale.unit);
+}
+
+// A warp's tokens once more, with whole lists and what 64 bits take. Everything is loaded here again and the code stands
+// inline, in a loop of its own: as a call from the middle of the loop over the tokens it made that loop spill (67 us where
+// this takes 56, 65536 tokens of 256 experts).
+template <typename T, int LPT, int VPL>
+__device__ __forceinline__ void decide_again(const RouteParams& p, RouteScale scale, RouteRoom room, int token, bool live) {
+  const RouteLane<LPT, VPL> me(p);
+  const T* row = route_row<T>(p, token);
+  float z[VPL], bias[VPL], none = 0.f;
+  load_own<T, VPL>(row, me.e0, p.E, p.vec, z);
+  load_bias<VPL>(p, me.e0, scale, bias);
+  decide<T, LPT, VPL, true, false>(p, me, scale, room, token, live, row, z, bias, nullptr, none, [] {});
+}
+
 template <typename T, int LPT, int VPL, bool AUX>
 __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kernel(const __grid_constant__ RouteParams p) {
   constexpr int TPB = ROUTE_THREADS / LPT;                 // tokens that a block has in hand
-  constexpr int MOST_K = LPT * VPL < FMB_ROUTE_MAX_K ? LPT * VPL : FMB_ROUTE_MAX_K, PER = (MOST_K + LPT - 1) / LPT;
+  constexpr int MOST_K = LPT * VPL < FMB_ROUTE_MAX_K ? LPT * VPL : FMB_ROUTE_MAX_K;
   extern __shared__ double s_mem[];                        // for the choice in 64 bits: scores [TPB, E], groups [TPB, groups]
   __shared__ unsigned s_key[TPB][MOST_K + 2];
   __shared__ int s_pick[TPB][MOST_K];
   __shared__ float s_range[2][ROUTE_THREADS / 32];
-  double* c64 = s_mem + static_cast<size_t>(threadIdx.x / LPT) * p.E;
-  double* g64 = s_mem + static_cast<size_t>(TPB) * p.E + threadIdx.x / LPT * p.groups;
-  unsigned* s_n = reinterpret_cast<unsigned*>(c64);        // groups that are no whole lanes: the token's fixed-point scores
+  const int slot = threadIdx.x / LPT;
   int* s_count = reinterpret_cast<int*>(s_mem + static_cast<size_t>(TPB) * (p.E + p.groups));   // [E]
   float* s_acc = reinterpret_cast<float*>(s_count + p.E);                                       // [E + 1]
+  const RouteRoom room = {s_mem + static_cast<size_t>(slot) * p.E, s_mem + static_cast<size_t>(TPB) * p.E + slot * p.groups,
+                          s_key[slot], s_pick[slot], s_count};
   pdl_wait();
   pdl_launch_dependents();
-  const int lane = threadIdx.x % LPT, slot = threadIdx.x / LPT, e0 = lane * VPL;
-  const bool biased = p.bias != nullptr, grouped = p.groups > 1;
-  const bool by_score = biased || (grouped && p.best > 1); // else the order of the logits is the scores'
-  // groups that are a power of two of whole lanes
-  const int span = p.gsize / VPL;
-  const bool whole_lanes = p.gsize % VPL == 0 && (span & (span - 1)) == 0 && span <= LPT;
-  const unsigned own_group = grouped && whole_lanes ? lane / span : 0;
-  const bool has_group = own_group < static_cast<unsigned>(p.groups), two_best = p.best > 1 && p.gsize > 1;
+  const RouteLane<LPT, VPL> me(p);
+  const int e0 = me.e0;
   for (int e = threadIdx.x; e < p.E; e += ROUTE_THREADS) s_count[e] = 0;
   if (AUX)
     for (int e = threadIdx.x; e <= p.E; e += ROUTE_THREADS) s_acc[e] = 0.f;
   // the range of scores in fixed point: [0, 1] and what the finite biases add
-  float lo = 0.f, hi = 1.f;
-  bool bad_bias = false;                                   // NaN or +inf: every choice is then made in 64 bits
-  bool flat_bias = false;                                  // one finite bias for all
-  float bias[VPL];
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    bias[i] = biased && e0 + i < p.E ? p.bias[e0 + i] : 0.f;
-    bad_bias |= !(bias[i] < CUDART_INF_F);
-  }
-  if (biased) {
+  RouteScale scale = {0.f, 1.f, 0, false, false};
+  float hi = 1.f, bias[VPL];
+  if (me.biased) {
     float a = CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i)
+    for (int i = 0; i < VPL; ++i) {
+      bias[i] = e0 + i < p.E ? p.bias[e0 + i] : 0.f;
+      scale.bad_bias |= !(bias[i] < CUDART_INF_F);
       if (e0 + i < p.E && fabsf(bias[i]) < CUDART_INF_F) { a = fminf(a, bias[i]); b = fmaxf(b, bias[i]); }
+    }
     a = -lanes_max<32>(-a);
     b = lanes_max<32>(b);
     if (threadIdx.x % 32 == 0) { s_range[0][threadIdx.x / 32] = a; s_range[1][threadIdx.x / 32] = b; }
     __syncthreads();
     for (int w = 0; w < ROUTE_THREADS / 32; ++w) { a = fminf(a, s_range[0][w]); b = fmaxf(b, s_range[1][w]); }
-    if (a <= b) { lo = a; hi = 1.f + b; }
+    if (a <= b) { scale.lo = a; hi = 1.f + b; }
     bool same = a == b;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) same &= e0 + i >= p.E || bias[i] == a;
-    flat_bias = __all_sync(0xffffffffu, same);
+    scale.flat_bias = __all_sync(0xffffffffu, same);
   }
   __syncthreads();
   // steps per score, so few less that no rounding goes past the last one; what the bias adds to the fixed point
-  const float unit = static_cast<float>(FIXED - 16) / (hi - lo);
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) bias[i] = fmaf(bias[i] - lo, unit, 8388608.f);
+  scale.unit = static_cast<float>(FIXED - 16) / (hi - scale.lo);
+  load_bias<VPL>(p, e0, scale, bias);
   // How far a score may be from the exact one. Sigmoid: s (1 - s) <= 1/4 of the error of e^-z (2^-22, and its argument's
   // rounding, 3.3e-7 at |z| = 5.5 and less in s beyond), 1.8e-7 from addition and reciprocal: 3.4e-7. Softmax, divided by a
-  // sum of up to 512 terms some 30 roundings deep: 3e-6. Then a step of the fixed point. Two of those.
-  const unsigned near = static_cast<unsigned>(fminf((p.softmax ? 6e-6f : 6.8e-7f) * unit + 3.f, 1e6f));
+  // sum of up to 512 terms some 30 roundings deep: 3e-6. Then a step of the fixed point. Two of those, and one more: closer
+  // than that is too near.
+  scale.near = static_cast<unsigned>(fminf((p.softmax ? 6e-6f : 6.8e-7f) * scale.unit + 4.f, 1e6f));
   float acc[AUX ? VPL : 1], acc_z = 0.f;
 #pragma unroll
   for (int i = 0; i < (AUX ? VPL : 1); ++i) acc[i] = 0.f;
 
-  const int tokens = static_cast<int>(p.tokens);
-  const int stride = gridDim.x * TPB;                       // (fewer than 2^31 tokens)
-  float z[VPL];
-  auto row_of = [&](int base) {                       // lanes without a token go along with the last one
-    return static_cast<const T*>(p.logits) + static_cast<long long>(min(base + slot, tokens - 1)) * p.ld;
-  };
-  load_own<T, VPL>(row_of(blockIdx.x * TPB), e0, p.E, p.vec, z);
-  for (int base = blockIdx.x * TPB; base < tokens; base += stride) {
-    const bool live = base + slot < tokens;
-    const int token = min(base + slot, tokens - 1);
-    const T* row = row_of(base);
-    float top = z[0], mass = 1.f;
-#pragma unroll
-    for (int i = 1; i < VPL; ++i) top = max_or_nan(top, z[i]);
-    bool doubt = bad_bias || !(top < CUDART_INF_F);         // NaN or +inf, or an order that fp32 leaves open
-    if (p.softmax || AUX || !biased) top = lanes_max<LPT>(top);
-    const float high = top;                                 // (of this lane alone where nothing needs the row's)
-    if (p.softmax || AUX) {
-      if (top == -CUDART_INF_F) top = 0.f;                  // a row of nothing but -inf: scores of 0
-      mass = 0.f;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) mass += e0 + i < p.E ? expf(z[i] - top) : 0.f;
-      mass = lanes_sum<LPT>(mass);
-      if (mass == 0.f) mass = 1.f;
+  const int last = static_cast<int>(p.tokens) - 1;          // (fewer than 2^31 tokens)
+  const int stride = gridDim.x * TPB;
+  float z[VPL];                                             // lanes without a token go along with the last one
+  load_own<T, VPL>(route_row<T>(p, min(static_cast<int>(blockIdx.x) * TPB + slot, last)), e0, p.E, p.vec, z);
+  for (int base = blockIdx.x * TPB; base <= last;) {
+    // 32 steps, of which those with an undecided token are taken again afterwards
+    const int begin = base;
+    unsigned again = 0;
+    for (unsigned bit = 1; bit != 0 && base <= last; bit <<= 1, base += stride) {
+      const int token = min(base + slot, last);
+      const bool done = decide<T, LPT, VPL, false, AUX>(p, me, scale, room, token, base + slot <= last, route_row<T>(p, token), z, bias, acc,
+                                                        acc_z, [&] {
+        if (base + stride <= last) load_own<T, VPL>(route_row<T>(p, min(base + stride + slot, last)), e0, p.E, p.vec, z);
+      });
+      if (!done) again |= bit;
     }
-    if constexpr (AUX) {
-      float norm = mass;
-      if (!p.softmax) {
-        norm = 0.f;
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) norm += e0 + i < p.E ? sigmoid(z[i]) : 0.f;
-        norm = lanes_sum<LPT>(norm);
-        if (norm == 0.f) norm = 1.f;
+    if (again != 0) {
+      for (; again != 0; again &= again - 1) {
+        const int at = begin + (__ffs(again) - 1) * stride + slot;
+        decide_again<T, LPT, VPL>(p, scale, room, min(at, last), at <= last);
       }
-      if (live) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (e0 + i < p.E) acc[i] += (p.softmax ? expf(z[i] - top) : sigmoid(z[i])) / norm;
-        const float lse = top + logf(mass);
-        if (lane == 0) acc_z += lse * lse;
-      }
+      if (base <= last) load_own<T, VPL>(route_row<T>(p, min(base + slot, last)), e0, p.E, p.vec, z);
+      load_bias<VPL>(p, e0, scale, bias);
     }
-    // fixed-point scores and keys; first, second: the lane's two largest for its group
-    unsigned key[VPL], first = 0, second = 0;
-    auto see = [&](unsigned v, int e) {
-      if (e < p.E) {
-        second = max(second, min(first, v));
-        first = max(first, v);
-        if (!whole_lanes) s_n[e] = key_score(v);
-      }
-    };
-    if (grouped && !whole_lanes) __syncwarp();              // the scores of the token before have been read
-    if (by_score) {
-      const float inv_mass = __fdividef(1.f, mass);
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const float c = p.softmax ? exp2_unit((z[i] - top) * 1.4426950408889634f) * inv_mass : sigmoid_near(z[i]);
-        key[i] = route_key(fmaf(c, unit, bias[i]), e0 + i);
-      }
-      if (grouped) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
-      }
-    }
-    if (!biased) {                                          // 32 units of logit below the largest one in 23 bits
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = route_key(fmaf(z[i] - high, 262144.f, 16777215.f), e0 + i);
-      if (grouped && !by_score) {
-#pragma unroll
-        for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
-      }
-    }
-    if (base + stride < tokens) load_own<T, VPL>(row_of(base + stride), e0, p.E, p.vec, z);      // the next token's
-    if (e0 + VPL > p.E) {                                   // the last expert's key is above 0: its number is
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (e0 + i >= p.E) key[i] = 0;
-    }
-    if (grouped) {
-      unsigned low = 0, out = 0;                            // the lowest group kept and the highest left out
-      if (whole_lanes) {
-        unsigned a = first, b = second;                     // of the lane, then of the group
-        for (int o = 1; o < span; o *= 2) {
-          const unsigned oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-          b = max(max(b, ob), min(a, oa));
-          a = max(a, oa);
-        }
-        // the group's score above 31 - its number, the same in all its lanes
-        unsigned mine = has_group ? (key_score(a) + (two_best ? key_score(b) : 0u)) << 5 | (31 - own_group) : 0u;
-        const unsigned whole = mine;
-#pragma unroll 1
-        for (int n = 0; n < p.top_groups; ++n) {
-          low = lanes_umax<LPT>(mine);
-          mine = mine == low ? 0 : mine;
-        }
-        out = lanes_umax<LPT>(mine);
-        if (whole < low || !has_group) {                    // a group that is left out
-#pragma unroll
-          for (int i = 0; i < VPL; ++i) key[i] = 0;
-        }
-      } else {
-        __syncwarp();
-        unsigned* s_g = reinterpret_cast<unsigned*>(g64);
-        for (int n = lane; n < p.groups; n += LPT) {
-          unsigned a = 0, b = 0;
-          for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
-            const unsigned v = s_n[e];
-            b = max(b, min(a, v));
-            a = max(a, v);
-          }
-          s_g[n] = (a + (two_best ? b : 0u)) << 5 | (31 - n);
-        }
-        __syncwarp();
-        unsigned kept = 0;
-        for (int n = lane; n < p.groups; n += LPT) {
-          int ahead = 0;
-          for (int m = 0; m < p.groups; ++m) ahead += s_g[m] > s_g[n];
-          if (ahead < p.top_groups) kept |= 1u << n;
-          if (ahead == p.top_groups - 1) low = s_g[n];
-          if (ahead >= p.top_groups) out = max(out, s_g[n]);
-        }
-#pragma unroll
-        for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
-        low = lanes_umax<LPT>(low);
-        out = lanes_umax<LPT>(out);
-#pragma unroll
-        for (int i = 0; i < VPL; ++i)
-          if (e0 + i < p.E && !(kept >> ((e0 + i) / p.gsize) & 1)) key[i] = 0;
-        __syncwarp();
-      }
-      const unsigned apart = by_score ? 2 * near : 3;
-      doubt |= p.top_groups < p.groups && (low >> 5) - (out >> 5) <= apart;
-    }
-    sort_falling(key);
-    // k rounds of the largest first key, each kept by a lane of its own, and one more to see how far behind the next one is
-    auto round = [&]() {
-      const unsigned w = lanes_umax<LPT>(key[0]);
-      if (key[0] == w) {
-#pragma unroll
-        for (int i = 0; i + 1 < VPL; ++i) key[i] = key[i + 1];
-        key[VPL - 1] = 0;
-      }
-      return w;
-    };
-    unsigned mine[PER];
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      mine[n] = 0;
-#pragma unroll 1
-      for (int j = n * LPT; j < (n + 1) * LPT && j < p.k; ++j) {
-        const unsigned w = round();
-        if (lane == j - n * LPT) mine[n] = w;
-      }
-    }
-    const unsigned next = round();
-    const unsigned apart = biased ? near : 3;
-    int pick[PER];
-    bool hit = false;                                       // neighbours of the order that are too near to tell
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      const int j = n * LPT + lane;
-      unsigned after = __shfl_down_sync(0xffffffffu, mine[n], 1, LPT);
-      if (n + 1 < PER) {
-        const unsigned turn = __shfl_sync(0xffffffffu, mine[n + 1 < PER ? n + 1 : n], 0, LPT);
-        if (lane == LPT - 1) after = turn;
-      }
-      if (j == p.k - 1) after = next;
-      pick[n] = min(key_expert(mine[n]), p.E - 1);          // (a token in doubt may have fewer keys than choices)
-      if (j < p.k) {
-        doubt |= mine[n] == 0;
-        hit |= after != 0 && key_score(mine[n]) - key_score(after) <= apart;
-      }
-    }
-    if (__any_sync(0xffffffffu, hit || doubt)) {            // one token of this warp, or more: all its lanes go
-      const unsigned then = round();
-#pragma unroll
-      for (int n = 0; n < PER; ++n)
-        if (n * LPT + lane < p.k) s_key[slot][n * LPT + lane] = mine[n];
-      if (lane == 0) {
-        s_key[slot][p.k] = next;
-        s_key[slot][p.k + 1] = then;
-      }
-      __syncwarp();
-      settle<T, LPT, VPL>(p, row, lane, apart, doubt, !biased || flat_bias, s_key[slot], s_pick[slot], c64, g64);
-#pragma unroll
-      for (int n = 0; n < PER; ++n)
-        if (n * LPT + lane < p.k) pick[n] = s_pick[slot][n * LPT + lane];
-      __syncwarp();
-    }
-    // weights of the chosen, each by a lane of its own
-    float sum = 0.f, best = -CUDART_INF_F, chosen[PER];
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      const int j = n * LPT + lane;
-      chosen[n] = j < p.k ? to_f32(row[pick[n]]) : -CUDART_INF_F;
-      best = fmaxf(best, chosen[n]);
-    }
-    if (p.softmax) best = lanes_max<LPT>(best);
-    // shares of the chosen alone are taken around their own maximum: they may all lie far below the row's
-    const float from = !p.renorm ? top : best == -CUDART_INF_F ? 0.f : best;
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      if (n * LPT + lane < p.k) {
-        chosen[n] = p.softmax ? expf(chosen[n] - from) / (p.renorm ? 1.f : mass) : sigmoid(chosen[n]);
-        sum += chosen[n];
-      }
-    }
-    sum = lanes_sum<LPT>(sum);
-    if (!p.softmax && p.renorm && __any_sync(0xffffffffu, sum < 1e-30f)) {
-      // sigmoids that vanish in fp32 still have shares: s = e^z there
-      const float peak = lanes_max<LPT>(best), around = peak == -CUDART_INF_F ? 0.f : peak;
-      float far = 0.f, share[PER];
-#pragma unroll
-      for (int n = 0; n < PER; ++n) {
-        share[n] = n * LPT + lane < p.k ? expf(to_f32(row[pick[n]]) - around) : 0.f;
-        far += share[n];
-      }
-      far = lanes_sum<LPT>(far);
-      if (sum < 1e-30f) {
-#pragma unroll
-        for (int n = 0; n < PER; ++n) chosen[n] = share[n];
-        sum = far;
-      }
-    }
-    const float by = !p.renorm ? p.scale : sum == 0.f ? 0.f : p.scale / sum;      // nothing to share out: weights of 0
-#pragma unroll
-    for (int n = 0; n < PER; ++n) {
-      const int j = n * LPT + lane;
-      if (j < p.k && live) {
-        const int e = pick[n];
-        p.weights[static_cast<long long>(token) * p.k + j] = chosen[n] * by;
-        p.idx[static_cast<long long>(token) * p.k + j] = e;
-        atomicAdd(&s_count[e], 1);
-      }
-    }
-    __syncwarp();
   }
   if constexpr (AUX) {
     for (int who = 0; who < TPB; ++who) {                   // tokens' sums one slot after another: a fixed order
@@ -565,7 +729,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
           if (e0 + i < p.E) s_acc[e0 + i] += acc[i];
-        if (lane == 0) s_acc[p.E] += acc_z;
+        if (me.lane == 0) s_acc[p.E] += acc_z;
       }
     }
   }

@@ -5,6 +5,7 @@ import torch
 
 import forgeminds_b200 as fm
 from forgeminds_b200 import ops
+from test_gpu_rowwise import check_route
 
 pytestmark = pytest.mark.gpu
 K = fm.kernels
@@ -180,3 +181,46 @@ def test_route_beyond_31_bits():
     tail = z.detach()[-64:].clone().requires_grad_()
     (want,) = torch.autograd.grad(K.route_experts(tail, 2, score="sigmoid")[0][:, 0].sum(), tail)
     assert torch.equal(g[-64:], want)
+
+
+# ------------------------------------------------------------------------------ orders that the fast choice leaves open
+@pytest.mark.parametrize("E,k,groups", [(64, 8, 1), (100, 20, 1), (128, 8, 4), (256, 8, 1), (256, 16, 8), (512, 12, 1), (384, 9, 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_when_neighbouring_experts_win(E, k, groups, dtype):
+    """All choices lie side by side: one lane has more of them than it keeps in its list."""
+    slope = torch.linspace(2, -2, E, device="cuda")
+    z = torch.stack([slope.roll(s) + 1e-3 * randn(E, seed=s) for s in range(0, E, 7)]).to(dtype)
+    bias = 0.01 * randn(E, seed=5)
+    for score in ("softmax", "sigmoid"):
+        for b in (None, bias):
+            check_route(z, k, score, b, groups, max(1, groups // 2))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_signed_zeros_and_equal_logits(dtype):
+    z = randn(50, 64, seed=6).round().to(dtype)
+    z[:, ::3] = 0.0
+    z[:, 1::3] = -0.0
+    z[10:20, 5:] = float("-inf")
+    z[20:30] = -z[20:30].abs()
+    for score in ("softmax", "sigmoid"):
+        for groups in (1, 8):
+            check_route(z[:10], 6, score, None, groups, max(1, groups // 2))
+            check_route(z[20:], 6, score, torch.zeros(64, device="cuda"), groups, max(1, groups // 2), best=1)
+        w, idx, _, _ = K.route_experts(z[10:20], 5, score=score)
+        assert torch.equal(idx.long(), z[10:20].double().sort(dim=1, descending=True, stable=True)[1][:, :5])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_route_many_tokens_that_are_decided_again(dtype):
+    """More steps per warp than it takes before it goes back to the undecided tokens; every order is the logits'."""
+    z = (randn(1200000, 64, seed=7) * 4).round().div(8).to(dtype)
+    z[5::997, 3] = float("inf")
+    z[7::501] = 0.25
+    want = z.sort(dim=1, descending=True, stable=True)[1][:, :6]
+    zeros = torch.zeros(64, device="cuda")
+    for opts in (dict(), dict(score="sigmoid"), dict(score="sigmoid", bias=zeros)):
+        w, idx, counts, _ = K.route_experts(z, 6, **opts)
+        keep = torch.ones(len(z), dtype=torch.bool, device="cuda") if not opts else torch.isfinite(z).all(1)
+        assert torch.equal(idx.long()[keep], want[keep])
+        assert torch.equal(counts.long(), torch.bincount(idx.flatten().long(), minlength=64))
