@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
 // A row is split over the CTAs of a cluster, at most 64 KB for each so that three of them share an SM: the logits are read
 // from memory once, and maximum, sum and gradient are taken from there. A thread keeps to its own 16-byte vectors, and as
 // soon as the gradient has used one, the same place receives the next row's: loads, exponentials and stores of the SM's
-// CTAs overlap. Few threads per row (256), because the reductions and the row's bookkeeping cost each warp as much as some
+// CTAs overlap. Few threads per row (256, or 128), because the reductions and the row's bookkeeping cost each warp as much as some
 // fifty vectors do. Kept logit k belongs to thread k, whose maximum and sums join the row's own reductions. The CTAs of a
 // row exchange (maximum, sum around it, loss) once. Rows are given out one by one: clusters that find no place at first,
 // while an earlier kernel still holds some SMs, would otherwise be a second wave.
@@ -313,14 +313,15 @@ __device__ __forceinline__ uint32_t max_bf16x2(uint32_t a, uint32_t b) {
   return *reinterpret_cast<const uint32_t*>(&m);
 }
 
-constexpr int KL_ROW_THREADS = 256;
-constexpr int KL_ROW_BYTES = 64 * 1024;                    // most of a row in one CTA
+constexpr int KL_ROW_THREADS = 256;                        // most of a CTA: the kept logits that it can take
 constexpr int KL_MARKS = 1024;                             // words of the marks by which an index that stands twice is found
+constexpr int KL_ROW_BYTES = 64 * 1024;                    // most of a row in one CTA, and
+constexpr int KL_ROW_MOST = 192 * 1024;                    // where eight CTAs of that do not hold it
 
-template <typename T, typename TT>
-__global__ void __launch_bounds__(KL_ROW_THREADS, 3)
+template <typename T, typename TT, int THREADS>
+__global__ void __launch_bounds__(THREADS, 3 * KL_ROW_THREADS / THREADS)
 kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
-  constexpr int N = Vec16<T>::N, H = N / 2, THREADS = KL_ROW_THREADS, WARPS = THREADS / 32;
+  constexpr int N = Vec16<T>::N, H = N / 2, WARPS = THREADS / 32;
   extern __shared__ uint4 s_row[];                         // [per_cta]: this CTA's part of the row
   __shared__ unsigned s_marks[KL_MARKS];
   __shared__ int s_at[THREADS];
@@ -586,11 +587,11 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
 
 // Clusters of `split` CTAs with `smem` bytes each that the device holds together; 0 where the kernel does not run. (A second
 // wave of a walk over all rows would double its time: of 74 clusters of 4 that 148 SMs have room for by numbers, 71 fit.)
-template <typename T, typename TT> int kl_fit(int split, size_t smem) {
-  auto kernel = kl_topk_row_kernel<T, TT>;
+template <typename T, typename TT, int THREADS> int kl_fit(int split, size_t smem) {
+  auto kernel = kl_topk_row_kernel<T, TT, THREADS>;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(sm_count() / split * split);
-  cfg.blockDim = dim3(KL_ROW_THREADS);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -606,22 +607,22 @@ template <typename T, typename TT> int kl_fit(int split, size_t smem) {
   return got;
 }
 
-template <typename T, typename TT> int kl_row_launch(const KlParams& p, int split, int per_cta, cudaStream_t stream) {
-  auto kernel = kl_topk_row_kernel<T, TT>;
+template <typename T, typename TT, int THREADS> int kl_row_launch(const KlParams& p, int split, int per_cta, cudaStream_t stream) {
+  auto kernel = kl_topk_row_kernel<T, TT, THREADS>;
   static bool opted[64] = {};
   int dev = 0;
   const size_t smem = sizeof(uint4) * per_cta;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return -3;
   if (!opted[dev]) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KL_ROW_BYTES) != cudaSuccess) return -3;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, KL_ROW_MOST) != cudaSuccess) return -3;
     opted[dev] = true;
   }
-  const long long fit = kl_fit<T, TT>(split, smem);
+  const long long fit = kl_fit<T, TT, THREADS>(split, smem);
   if (fit < 1) return -3;
   const long long groups = p.rows < fit ? p.rows : fit;
   const dim3 grid(static_cast<unsigned>(groups * split));
-  const cudaError_t e = split == 1 ? launch_pdl(kernel, grid, dim3(KL_ROW_THREADS), smem, stream, p, split, per_cta)
-                                   : launch_pdl_cluster(kernel, grid, dim3(KL_ROW_THREADS), smem, split, stream, p, split, per_cta);
+  const cudaError_t e = split == 1 ? launch_pdl(kernel, grid, dim3(THREADS), smem, stream, p, split, per_cta)
+                                   : launch_pdl_cluster(kernel, grid, dim3(THREADS), smem, split, stream, p, split, per_cta);
   return e == cudaSuccess ? 0 : -3;
 }
 
@@ -644,14 +645,19 @@ int kl_run(KlParams p, bool fwd, int* ws, bool mean, const int* count, cudaStrea
   }
   if (mean) p.count = count;
   if (fwd) {
-    // the fewest CTAs (1, 2, 4 or 8) that hold a row, more while SMs would be left without one
-    constexpr int N = Vec16<T>::N, MOST = KL_ROW_BYTES / 16;
+    // the fewest CTAs (1, 2, 4 or 8) that hold a row, more while SMs would be left without one; a row beyond 512 KB takes
+    // eight with up to 192 KB each
+    constexpr int N = Vec16<T>::N, MOST = KL_ROW_BYTES / 16, TOP = KL_ROW_MOST / 16;
     const int vectors = p.V / N > 0 ? p.V / N : 1;
     int split = 1;
     while (split < 8 && (vectors + split - 1) / split > MOST) split *= 2;
     while (split < 8 && p.rows * split < sm_count() && vectors / split > 4 * KL_ROW_THREADS) split *= 2;
-    if (p.K <= KL_ROW_THREADS && (vectors + split - 1) / split <= MOST)
-      return kl_row_launch<T, TT>(p, split, (vectors + split - 1) / split, stream);
+    const int per_cta = (vectors + split - 1) / split;
+    // Many rows of up to 32 KB: half the threads for each and up to six of them at a time. With gradient, bf16: 38910 x 2056
+    // in 177 us against 291 with 256 threads, 9765 x 8192 82 / 102, 4882 x 16384 76 / 81; but 1200 x 12160 30 / 27.
+    if (p.rows > 12LL * sm_count() && p.K <= KL_ROW_THREADS / 2 && per_cta <= MOST / 2)
+      return kl_row_launch<T, TT, KL_ROW_THREADS / 2>(p, split, per_cta, stream);
+    if (p.K <= KL_ROW_THREADS && per_cta <= TOP) return kl_row_launch<T, TT, KL_ROW_THREADS>(p, split, per_cta, stream);
   }
   const long long blocks = p.rows < 4LL * sm_count() ? p.rows : 4LL * sm_count();
   e = fwd ? launch_pdl(kl_topk_kernel<T, TT, true>, dim3(static_cast<unsigned>(blocks)), dim3(KL_THREADS), smem, stream, p)

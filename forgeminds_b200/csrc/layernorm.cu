@@ -433,7 +433,7 @@ layernorm_cols_kernel(const float* __restrict__ partial, WT* __restrict__ dw, WT
 }
 
 // ------------------------------------------------------------------ launches
-constexpr int FWD_CHUNKS = 2048;     // most chunks of a row that the forward kernel holds in registers (512 threads x 4)
+constexpr int FWD_CHUNKS = 4096;     // most chunks of a row that the forward kernel holds in registers (1024 threads x 4)
 constexpr int BWD_CHUNKS = 1024;     // and the backward kernel (512 x 2)
 
 template <typename T, typename WT, bool VEC, bool ADD>
@@ -453,7 +453,8 @@ cudaError_t fwd_launch(const T* x, long long ldx, const T* delta, long long ldd,
   if (chunks <= 256) FMB_LN_FWD(128, 2);
   if (chunks <= 512) FMB_LN_FWD(256, 2);
   if (chunks <= 1024) FMB_LN_FWD(256, 4);
-  if (chunks <= FWD_CHUNKS) FMB_LN_FWD(512, 4);
+  if (chunks <= 2048) FMB_LN_FWD(512, 4);
+  if (chunks <= FWD_CHUNKS) FMB_LN_FWD(1024, 4);
 #undef FMB_LN_FWD
   layernorm_fwd_wide_kernel<T, WT, ADD><<<static_cast<unsigned>(rows), 1024, 0, stream>>>(x, ldx, delta, ldd, w, b, xsum, y,
                                                                                          stats, d, inv_d, eps);

@@ -32,33 +32,61 @@ struct RotaryParams {
 
 constexpr int BATCH = 4;
 
+// The token, unit and heads of this thread's item; false where there is none.
+struct Item {
+  unsigned token;
+  int b, t, unit, h, h_end;
+};
+__device__ __forceinline__ bool item_of(const RotaryParams& p, Item& it) {
+  const unsigned per_token = static_cast<unsigned>(p.units) * p.groups;
+  const unsigned item = blockIdx.x * 256u + threadIdx.x;             // fewer than 2^31 items per launch
+  const unsigned local = item / per_token, rest = item - local * per_token;
+  it.token = p.token0 + local;
+  const int group = rest / p.units;
+  it.unit = rest - group * p.units;
+  it.b = it.token / p.T;
+  it.t = it.token - it.b * p.T;
+  it.h = group * p.per_group;
+  it.h_end = min(it.h + p.per_group, p.q.heads + p.k.heads);
+  return it.token < p.tokens;
+}
+__device__ __forceinline__ long long position_of(const RotaryParams& p, const Item& it) {
+  if (p.positions == nullptr) return it.t;
+  const long long at = it.b * p.pos_b + it.t;
+  return p.wide_pos ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
+}
+template <typename T> __device__ __forceinline__ void head_of(const RotaryParams& p, const Item& it, int h, const T*& src, T*& dst) {
+  const bool is_k = h >= p.q.heads;
+  const RotaryTensor& x = is_k ? p.k : p.q;
+  const int hh = is_k ? h - p.q.heads : h;
+  src = static_cast<const T*>(x.src) + it.b * x.sb + it.t * x.st + hh * x.sh;
+  dst = static_cast<T*>(x.dst) + (static_cast<long long>(it.token) * x.heads + hh) * p.D;
+}
+
 // One item: unit `u` of a token (VEC pairs, or two vectors of VEC copied values) in `per_group` heads.
 template <typename T, int VEC, bool INTER>
 __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryParams p) {
   pdl_wait();
   pdl_launch_dependents();
-  const unsigned per_token = static_cast<unsigned>(p.units) * p.groups;
-  const unsigned item = blockIdx.x * 256u + threadIdx.x;             // fewer than 2^31 items per launch
-  const unsigned local = item / per_token;
-  const unsigned token = p.token0 + local;
-  if (token >= p.tokens) return;
-  const unsigned rest = item - local * per_token;
-  const int group = rest / p.units, unit = rest - group * p.units;
-  const int b = token / p.T, t = token - b * p.T;
-  const bool turn = unit < p.rot_units;
+  Item it;
+  if (!item_of(p, it)) return;
+  const int unit = it.unit;
+  bool turn = unit < p.rot_units;
+  const int first = turn ? (INTER ? 2 * VEC * unit : VEC * unit) : p.R + 2 * VEC * (unit - p.rot_units);
+  // where the two vectors of pairs, or the two that are copied (the second may not be there), lie in a head
+  const int second = INTER || !turn ? first + VEC : first + p.R / 2;
+  const bool two = turn || second < p.D;
   float c[VEC], s[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) { c[j] = 1.f; s[j] = 0.f; }
   if (turn) {
-    long long pos = t;
-    if (p.positions != nullptr) {
-      const long long at = b * p.pos_b + t;
-      pos = p.wide_pos ? static_cast<const long long*>(p.positions)[at] : static_cast<const int*>(p.positions)[at];
-    }
+    const long long pos = position_of(p, it);
     if (pos >= p.table) {                                            // beyond the table there is no angle: say so loudly
 #pragma unroll
       for (int j = 0; j < VEC; ++j) { c[j] = CUDART_NAN_F; s[j] = CUDART_NAN_F; }
-    } else if (pos >= 0) {                                           // a negative position marks padding: left unturned
+    } else if (pos < 0) {                                            // a negative position marks padding: copied
+      turn = false;
+    } else {
       const float *cr = p.cos + pos * p.ldt + unit * VEC, *sr = p.sin + pos * p.ldt + unit * VEC;
       if constexpr (VEC % 4 == 0) {
         load_f32<float, VEC>(cr, c);
@@ -71,34 +99,22 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
       for (int j = 0; j < VEC; ++j) s[j] *= p.sign;
     }
   }
-  // where the two vectors of pairs, or the two that are copied (the second may not be there), lie in a head
-  const int first = turn ? (INTER ? 2 * VEC * unit : VEC * unit) : p.R + 2 * VEC * (unit - p.rot_units);
-  const int second = INTER || !turn ? first + VEC : first + p.R / 2;
-  const bool two = turn || second < p.D;
-  const int h_end = min((group + 1) * p.per_group, p.q.heads + p.k.heads);
-  auto place = [&](int h, const T*& src, T*& dst) {
-    const bool is_k = h >= p.q.heads;
-    const RotaryTensor& x = is_k ? p.k : p.q;
-    const int hh = is_k ? h - p.q.heads : h;
-    src = static_cast<const T*>(x.src) + b * x.sb + t * x.st + hh * x.sh;
-    dst = static_cast<T*>(x.dst) + (static_cast<long long>(token) * x.heads + hh) * p.D;
-  };
   if constexpr (VEC == Vec16<T>::N) {
     // BATCH heads are loaded before the first of them is stored: a thread has 128 bytes on their way
-    for (int h = group * p.per_group; h < h_end; h += BATCH) {
+    for (int h = it.h; h < it.h_end; h += BATCH) {
       uint4 ra[BATCH], rb[BATCH];
       T* dst[BATCH];
 #pragma unroll
       for (int i = 0; i < BATCH; ++i)
-        if (h + i < h_end) {
+        if (h + i < it.h_end) {
           const T* src;
-          place(h + i, src, dst[i]);
+          head_of<T>(p, it, h + i, src, dst[i]);
           ra[i] = *reinterpret_cast<const uint4*>(src + first);
           if (two) rb[i] = *reinterpret_cast<const uint4*>(src + second);
         }
 #pragma unroll
       for (int i = 0; i < BATCH; ++i) {
-        if (h + i >= h_end) break;
+        if (h + i >= it.h_end) break;
         if (turn) {
           float x0[VEC], x1[VEC], y0[VEC], y1[VEC];
           Vec16<T>::unpack(ra[i], x0);
@@ -128,10 +144,10 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
   } else {
     static_assert(VEC == 1, "single values otherwise");
 #pragma unroll 2
-    for (int h = group * p.per_group; h < h_end; ++h) {
+    for (int h = it.h; h < it.h_end; ++h) {
       const T* src;
       T* dst;
-      place(h, src, dst);
+      head_of<T>(p, it, h, src, dst);
       const T va = src[first], vb = two ? src[second] : va;
       if (turn) {
         const float a = to_f32(va), e = to_f32(vb);
@@ -145,11 +161,63 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
   }
 }
 
+// Heads of whole vectors of which R values are no whole vectors of pairs. One item: one vector of a head, where a value's
+// partner is its neighbour (INTER), or lies R / 2 away and is loaded by itself.
 template <typename T, bool INTER>
-cudaError_t rotary_launch(RotaryParams p, bool vec, cudaStream_t stream) {
-  const int n = vec ? Vec16<T>::N : 1, heads = p.q.heads + p.k.heads;
+__global__ void __launch_bounds__(256) rotary_mixed_kernel(const __grid_constant__ RotaryParams p) {
+  constexpr int N = Vec16<T>::N;
+  pdl_wait();
+  pdl_launch_dependents();
+  Item it;
+  if (!item_of(p, it)) return;
+  const int first = it.unit * N, half = p.R / 2;
+  float c[N], s[N];
+  int away[N];                                                       // of the partner
+  unsigned turns = 0;                                                // values that are turned
+  const long long pos = first < p.R ? position_of(p, it) : -1;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    const int e = first + j;
+    const bool upper = INTER ? e % 2 : e >= half;
+    away[j] = INTER ? (upper ? -1 : 1) : upper ? -half : half;
+    c[j] = 1.f;
+    s[j] = 0.f;
+    if (e < p.R && pos >= 0) {
+      turns |= 1u << j;
+      const long long at = pos * p.ldt + (INTER ? e / 2 : upper ? e - half : e);
+      c[j] = pos < p.table ? p.cos[at] : CUDART_NAN_F;
+      s[j] = pos < p.table ? p.sin[at] * (upper ? p.sign : -p.sign) : CUDART_NAN_F;
+    }
+  }
+#pragma unroll 2
+  for (int h = it.h; h < it.h_end; ++h) {
+    const T* src;
+    T* dst;
+    head_of<T>(p, it, h, src, dst);
+    uint4 u = *reinterpret_cast<const uint4*>(src + first);
+    if (turns != 0) {
+      float x[N], y[N];
+      Vec16<T>::unpack(u, x);
+#pragma unroll
+      for (int j = 0; j < N; ++j) y[j] = x[j];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float partner = INTER ? x[j ^ 1] : turns >> j & 1 ? to_f32(src[first + j + away[j]]) : 0.f;
+        if (turns >> j & 1) y[j] = x[j] * c[j] + partner * s[j];
+      }
+      u = Vec16<T>::pack(y);
+    }
+    *reinterpret_cast<uint4*>(dst + first) = u;
+  }
+}
+
+enum class Form { VECTORS, MIXED, SINGLE };
+
+template <typename T, bool INTER>
+cudaError_t rotary_launch(RotaryParams p, Form form, cudaStream_t stream) {
+  const int n = form == Form::SINGLE ? 1 : Vec16<T>::N, heads = p.q.heads + p.k.heads;
   p.rot_units = p.R / 2 / n;
-  p.units = p.rot_units + ((p.D - p.R) / n + 1) / 2;
+  p.units = form == Form::MIXED ? p.D / n : p.rot_units + ((p.D - p.R) / n + 1) / 2;
   // Few tokens: a thread per head, for latency. Many: up to eight heads per thread, for the tables' sake.
   const long long lanes = static_cast<long long>(p.tokens) * p.units;
   const long long room = static_cast<long long>(sm_count()) * 2048;
@@ -164,8 +232,9 @@ cudaError_t rotary_launch(RotaryParams p, bool vec, cudaStream_t stream) {
     p.token0 = static_cast<unsigned>(lo);
     const long long items = (p.tokens - lo < most ? p.tokens - lo : most) * per_token;
     const unsigned blocks = static_cast<unsigned>((items + 255) / 256);
-    e = vec ? launch_pdl(rotary_kernel<T, Vec16<T>::N, INTER>, dim3(blocks), dim3(256), 0, stream, p)
-            : launch_pdl(rotary_kernel<T, 1, INTER>, dim3(blocks), dim3(256), 0, stream, p);
+    e = form == Form::VECTORS ? launch_pdl(rotary_kernel<T, Vec16<T>::N, INTER>, dim3(blocks), dim3(256), 0, stream, p)
+        : form == Form::MIXED ? launch_pdl(rotary_mixed_kernel<T, INTER>, dim3(blocks), dim3(256), 0, stream, p)
+                              : launch_pdl(rotary_kernel<T, 1, INTER>, dim3(blocks), dim3(256), 0, stream, p);
   }
   return e;
 }
@@ -192,12 +261,13 @@ extern "C" int fmb_rotary(const FmbRotaryTensor* q, const FmbRotaryTensor* k, co
   auto fits = [&](const FmbRotaryTensor* x) {
     return x->heads == 0 || (aligned16(x->src) && aligned16(x->dst) && x->sb % n == 0 && x->st % n == 0 && x->sh % n == 0);
   };
-  const bool vec = D % n == 0 && R % (2 * n) == 0 && fits(q) && fits(k) && aligned16(cos) && aligned16(sin) && ldt % 4 == 0;
+  const bool whole = D % n == 0 && fits(q) && fits(k);
+  const Form form = !whole ? Form::SINGLE : R % (2 * n) == 0 && aligned16(cos) && aligned16(sin) && ldt % 4 == 0 ? Form::VECTORS : Form::MIXED;
   cudaError_t e;
   if (dtype == FMB_BF16)
-    e = interleaved ? rotary_launch<__nv_bfloat16, true>(p, vec, stream) : rotary_launch<__nv_bfloat16, false>(p, vec, stream);
+    e = interleaved ? rotary_launch<__nv_bfloat16, true>(p, form, stream) : rotary_launch<__nv_bfloat16, false>(p, form, stream);
   else if (dtype == FMB_F32)
-    e = interleaved ? rotary_launch<float, true>(p, vec, stream) : rotary_launch<float, false>(p, vec, stream);
+    e = interleaved ? rotary_launch<float, true>(p, form, stream) : rotary_launch<float, false>(p, form, stream);
   else
     return -1;
   return e == cudaSuccess ? 0 : -3;

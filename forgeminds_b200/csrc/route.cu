@@ -292,9 +292,9 @@ __device__ __forceinline__ void settle(const RouteParams& p, const T* row, int l
     if (za == zb && (!biased || p.bias[a] == p.bias[b])) {
       // equal in any precision, and the lower number is first; at the last choice the next one might belong before both
       doubt |= j == p.k - 1 && close(j + 1);
-    } else if (p.softmax || !biased || (j > 0 && close(j - 1)) || close(j + 1)) {
+    } else if ((biased && p.softmax) || (j > 0 && close(j - 1)) || close(j + 1)) {
       doubt = true;
-    } else if (sigmoid_ahead(za, zb, p.bias[a], p.bias[b], b < a)) {
+    } else if (biased ? sigmoid_ahead(za, zb, p.bias[a], p.bias[b], b < a) : zb > za || (zb == za && b < a)) {
       pick[j] = b;
       if (j + 1 < p.k) pick[j + 1] = a;
     }
@@ -355,8 +355,7 @@ struct RouteRoom {
 
 // The fixed point of biased scores: what 0 is, steps per score, and how near two scores may be without being told apart
 struct RouteScale {
-  float lo, unit;
-  unsigned near;
+  float lo, unit, error;                                   // error: twice that of a score of 1, in steps
   bool bad_bias, flat_bias;                                // NaN or +inf: every choice is made in 64 bits; one finite bias for all
 };
 
@@ -401,6 +400,9 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
       if (lane == 0) acc_z += lse * lse;
     }
   }
+  // no softmax score is above the largest one's, 1 / mass, and their errors are in proportion
+  const float inv_mass = p.softmax ? __fdividef(1.f, mass) : 1.f;
+  const unsigned near = static_cast<unsigned>(fminf(fmaf(scale.error, inv_mass, 4.f), 1e6f));
   // fixed-point scores and keys; first, second: the lane's two largest for its group where the lists do not hold them
   unsigned key[VPL], list[L], first = 0, second = 0;
   const bool lists_serve = me.biased || !me.by_score;
@@ -416,7 +418,7 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
   };
   if (me.grouped && !me.whole_lanes) __syncwarp();          // the scores of the token before have been read
   if (me.by_score) {
-    keys_by_score<VPL>(p.softmax, z, bias, top, p.softmax ? __fdividef(1.f, mass) : 1.f, scale.unit, e0, key);
+    keys_by_score<VPL>(p.softmax, z, bias, top, inv_mass, scale.unit, e0, key);
     if (me.grouped && !(lists_serve && me.whole_lanes)) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i) see(key[i], e0 + i);
@@ -499,7 +501,7 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
       __syncwarp();
       make_list();
     }
-    const unsigned apart = me.by_score ? 2 * scale.near : by_logit;
+    const unsigned apart = me.by_score ? 2 * near : by_logit;
     doubt |= p.top_groups < p.groups && (low >> 5) - (out >> 5) < apart;
   } else {
     make_list();
@@ -518,7 +520,7 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
   }
   const unsigned next = take_largest<LPT>(list);
   bool open = longer && list[0] == 0;                       // this lane has given away its whole list
-  const unsigned apart = me.biased ? scale.near : by_logit;
+  const unsigned apart = me.biased ? near : by_logit;
   int pick[PER];
   unsigned after[PER];
   bool hit = false;                                         // neighbours of the order that are too near to tell
@@ -663,7 +665,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
   if (AUX)
     for (int e = threadIdx.x; e <= p.E; e += ROUTE_THREADS) s_acc[e] = 0.f;
   // the range of scores in fixed point: [0, 1] and what the finite biases add
-  RouteScale scale = {0.f, 1.f, 0, false, false};
+  RouteScale scale = {0.f, 1.f, 0.f, false, false};
   float hi = 1.f, bias[VPL];
   if (me.biased) {
     float a = CUDART_INF_F, b = -CUDART_INF_F;
@@ -690,9 +692,9 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
   load_bias<VPL>(p, e0, scale, bias);
   // How far a score may be from the exact one. Sigmoid: s (1 - s) <= 1/4 of the error of e^-z (2^-22, and its argument's
   // rounding, 3.3e-7 at |z| = 5.5 and less in s beyond), 1.8e-7 from addition and reciprocal: 3.4e-7. Softmax, divided by a
-  // sum of up to 512 terms some 30 roundings deep: 3e-6. Then a step of the fixed point. Two of those, and one more: closer
-  // than that is too near.
-  scale.near = static_cast<unsigned>(fminf((p.softmax ? 6e-6f : 6.8e-7f) * scale.unit + 4.f, 1e6f));
+  // sum of up to 512 terms some 30 roundings deep: 3e-6 of the score. Then a step of the fixed point. Two of those, and one
+  // more, where a token's scores are taken: closer than that is too near.
+  scale.error = (p.softmax ? 6e-6f : 6.8e-7f) * scale.unit;
   float acc[AUX ? VPL : 1], acc_z = 0.f;
 #pragma unroll
   for (int i = 0; i < (AUX ? VPL : 1); ++i) acc[i] = 0.f;

@@ -5,6 +5,7 @@ import torch
 
 import forgeminds_b200 as fm
 from forgeminds_b200 import ops
+import test_gpu_rowwise as rowwise
 from test_gpu_rowwise import check_route
 
 pytestmark = pytest.mark.gpu
@@ -224,3 +225,43 @@ def test_route_many_tokens_that_are_decided_again(dtype):
         keep = torch.ones(len(z), dtype=torch.bool, device="cuda") if not opts else torch.isfinite(z).all(1)
         assert torch.equal(idx.long()[keep], want[keep])
         assert torch.equal(counts.long(), torch.bincount(idx.flatten().long(), minlength=64))
+
+
+# ------------------------------------------------------------------------------ forms chosen by size
+@pytest.mark.parametrize("D,R", [(64, 4), (64, 62), (96, 34), (128, 50), (256, 98), (8, 2), (80, 72)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_rotary_of_a_part_that_ends_inside_a_vector(D, R, interleaved, dtype):
+    rowwise.test_rotary_qk(2, 37, 6, 3, D, R, interleaved, dtype, True)
+    rowwise.test_rotary_qk(1, 700, 5, 1, D, R, interleaved, dtype, False)
+    x = randn(1, 4, 3, D, seed=8, dtype=rowwise.DT[dtype])
+    x[0, 1, 1] = float("inf")
+    at = torch.tensor([0, -1, 99, -7], device="cuda")
+    cos, sin = K.rotary_tables(9, R, device="cuda")
+    y = K.rotary(x, cos, sin, at, interleaved)
+    assert torch.equal(y[:, 1::2], x[:, 1::2])                 # negative positions: as they are, infinities too
+    assert bool(torch.isnan(y[0, 2, :, :R]).all()) and torch.equal(y[..., R:], x[..., R:])
+
+
+@pytest.mark.parametrize("rows,V,keep", [(2000, 1000, 100), (6000, 2056, 33), (1800, 12162, 128), (1800, 12167, 129), (2100, 31, 4)])
+@pytest.mark.parametrize("dtype,tdtype", [("bf16", "bf16"), ("fp32", "fp32")])
+def test_kl_topk_many_short_rows(rows, V, keep, dtype, tdtype):
+    student, values, index, teacher = rowwise.kl_inputs(rows, V, keep, 41, dtype, tdtype)
+    index[5::9, 1] = index[5::9, 0]                            # an index that stands twice
+    index[7::11] = -1                                          # rows that do not count
+    index[::13, keep - 1] = V                                  # and slots
+    rowwise.check_kl(student, values, index, 2.0)
+    rowwise.check_kl(student, values, index, 1.0, torch.logsumexp(teacher, -1), reduction="sum")
+
+
+@pytest.mark.parametrize("rows,V,keep,dtype", [(3, 200003, 20, "fp32"), (2, 393000, 256, "fp32"), (2, 800001, 7, "bf16"), (2, 900001, 7, "fp32")])
+def test_kl_topk_wider_than_eight_blocks_of_64_kb(rows, V, keep, dtype):
+    student, values, index, _ = rowwise.kl_inputs(rows, V, keep, 42, dtype, "fp32")
+    rowwise.check_kl(student, values, index, 1.5)
+
+
+@pytest.mark.parametrize("d", [8256, 16384, 16388, 20001])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_layer_norm_wide_rows(d, dtype):
+    rowwise.test_layer_norm(300, d, dtype, "fp32")
+    rowwise.test_add_layer_norm(41, d, dtype)
