@@ -8,6 +8,7 @@
 // statistics and the weight's gradients are fp32.
 #include "fmb_api.h"
 #include "launch.cuh"
+#include "ptx_sm100.cuh"
 #include "rows.cuh"
 
 namespace fmb {
@@ -192,23 +193,39 @@ layernorm_fwd_wide_kernel(const T* __restrict__ x, long long ldx, const T* __res
 // come through a ring of shared memory, copied STAGES - 1 rows ahead, each thread its own chunks (no barrier guards them):
 // with loads into registers a block waited out the memory's latency at every row. Two chunks per thread from 65 on: what a
 // row costs beside its columns (two sums over its threads, statistics, addresses) is as much as 130 instructions a thread.
+// SPLIT: a row of more than 1024 chunks is shared by the blocks of a cluster, `width` columns for each, which exchange their
+// two sums: 3024 x 12088 in 111 us (one block per row that reads it twice, and the columns once more: 160), a third of the
+// bandwidth, because the blocks wait for one another at every row.
 // dx, dw and db of bf16 rows with dres, the column sums included: 16384 x 4096 in 96 us (5.6 TB/s; with one chunk per
 // thread 112, from registers 125), 65536 x 1024 in 88 us (6.1 TB/s; one chunk 96).
-template <typename T, typename WT, int TPR, int VPL, bool VEC>
+template <typename T, typename WT, int TPR, int VPL, bool VEC, bool SPLIT>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : VPL > 1 ? 2 : 4)
 layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
                      const WT* __restrict__ w, const float2* __restrict__ stats, const T* __restrict__ dres, long long ldr,
-                     T* __restrict__ dx, float* __restrict__ partial, long long rows, int d, float inv_d) {
+                     T* __restrict__ dx, float* __restrict__ partial, long long rows, const int whole, float inv_d, const int split,
+                     const int width) {
   using M = RowMap<T, TPR, VEC>;
   constexpr int N = M::N, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
   constexpr int STAGES = BwdStages<VPL * THREADS>::N;
-  __shared__ float2 scratch[2][THREADS / 32];
+  static_assert(!SPLIT || RPB == 1, "a block has one row at a time");
+  __shared__ float2 scratch[2][THREADS / 32], s_peers[2][SPLIT ? 8 : 1];
   extern __shared__ uint4 s_ring[];                       // [stage][dy, x, dres][chunk][thread]; the fold below takes its place
   float* s_fold = reinterpret_cast<float*>(s_ring);       // [2, d], when several rows share a block
   pdl_wait();
   pdl_launch_dependents();
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int tensors = dres != nullptr ? 3 : 2;
+  const int rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0, group = SPLIT ? blockIdx.x / split : blockIdx.x;
+  const int groups = SPLIT ? gridDim.x / split : gridDim.x, from_col = SPLIT ? rank * width : 0;
+  const int d = SPLIT ? max(0, min(width, whole - from_col)) : whole;      // this block's columns
+  if constexpr (SPLIT) {
+    dy += from_col;
+    x += from_col;
+    dx += from_col;
+    if (dres != nullptr) dres += from_col;
+    if (w != nullptr) w += from_col;
+    cluster_sync_all();                                   // every block of the row runs before one writes to another
+  }
   constexpr int H = N / 2;
   F2 wv[VPL][H], dwa[VPL][H], dba[VPL][H];
 #pragma unroll
@@ -219,14 +236,14 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
     for (int j = 0; j < H; ++j) { wv[i][j] = f2(f[2 * j], f[2 * j + 1]); dwa[i][j] = dba[i][j] = f2(0.f, 0.f); }
   }
   // Everything a row needs moves on by one step: pointers, not products, and rows in 31 bits.
-  const int n_rows = static_cast<int>(rows), step = gridDim.x * RPB, start = blockIdx.x * RPB + sub;
+  const int n_rows = static_cast<int>(rows), step = groups * RPB, start = group * RPB + sub;
   const int row_bytes = tensors * VPL * THREADS * 16;
   const char* ring = reinterpret_cast<const char*>(s_ring + threadIdx.x);
   const uint32_t ring_at = smem_at(ring);
-  const long long step_dy = step * ldy, step_x = step * ldx, step_res = step * ldr, step_out = static_cast<long long>(step) * d;
+  const long long step_dy = step * ldy, step_x = step * ldx, step_res = step * ldr, step_out = static_cast<long long>(step) * whole;
   const int own = VEC ? M::col(0, 0, t) : 0;              // this thread's first column, where its chunks are contiguous
   const T *next_dy = dy + start * ldy + own, *next_x = x + start * ldx + own, *next_res = dres + start * ldr + own;
-  T* out = dx + static_cast<long long>(start) * d;
+  T* out = dx + static_cast<long long>(start) * whole;
   int next_row = start;
   int put = 0, get = 0;                                   // bytes from the ring's start
   auto copy = [&](const T* from, int tensor) {
@@ -262,7 +279,7 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
   }
   int turn = 0;
   float2 st = stats[min(start, n_rows - 1)];
-  for (int base = blockIdx.x * RPB; base < n_rows; base += step, out += step_out) {
+  for (int base = group * RPB; base < n_rows; base += step, out += step_out) {
     const int row = base + sub;
     const int width = RPB == 1 || row < n_rows ? d : 0;   // rows beyond the last take part in the sums with nothing
     const float2 next_st = stats[min(row + step, n_rows - 1)];
@@ -299,8 +316,21 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
       }
     }
     if constexpr (VEC) fetch();                           // into the place of the row before
-    
-    const float2 sums = row_sum2<TPR>(s1.x + s1.y, s2.x + s2.y, scratch[turn]);
+    float2 sums = row_sum2<TPR>(s1.x + s1.y, s2.x + s2.y, scratch[turn]);
+    if constexpr (SPLIT) {
+      if (threadIdx.x < split) {
+        const uint32_t to = mapa_shared(smem_at(&s_peers[turn][rank]), threadIdx.x);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.x) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sums.y) : "memory");
+      }
+      cluster_sync_all();                                 // the other half of s_peers is read by now
+      sums = make_float2(0.f, 0.f);
+      for (int i = 0; i < split; ++i) {
+        const float2 o = s_peers[turn][i];
+        sums.x += o.x;
+        sums.y += o.y;
+      }
+    }
     turn ^= 1;
     const F2 c1 = f2(-sums.x * inv_d, -sums.x * inv_d), c2 = f2(-sums.y * inv_d, -sums.y * inv_d);
 #pragma unroll
@@ -325,7 +355,7 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (partial == nullptr) return;
-  float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * d;
+  float* mine = partial + static_cast<long long>(group) * 2 * whole + from_col;
   if constexpr (RPB > 1) {
     for (int who = 0; who < RPB; ++who) {                 // the block's row groups one after another: a fixed order
       __syncthreads();
@@ -354,7 +384,7 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
         const float2 a = dwa[i][j / 2], b = dba[i][j / 2];
         if (c < d) {
           mine[c] = j % 2 ? a.y : a.x;
-          mine[d + c] = j % 2 ? b.y : b.x;
+          mine[whole + c] = j % 2 ? b.y : b.x;
         }
       }
   }
@@ -434,7 +464,9 @@ layernorm_cols_kernel(const float* __restrict__ partial, WT* __restrict__ dw, WT
 
 // ------------------------------------------------------------------ launches
 constexpr int FWD_CHUNKS = 4096;     // most chunks of a row that the forward kernel holds in registers (1024 threads x 4)
-constexpr int BWD_CHUNKS = 1024;     // and the backward kernel (512 x 2)
+constexpr int BWD_CHUNKS = 1024;     // and the backward kernel (512 x 2), beyond that clusters of
+constexpr int BWD_SPLIT = 8;         // at most so many blocks of 256 x 2
+inline int bwd_split(int chunks) { return chunks <= 2048 ? 4 : 8; }
 
 template <typename T, typename WT, bool VEC, bool ADD>
 cudaError_t fwd_launch(const T* x, long long ldx, const T* delta, long long ldd, const WT* w, const WT* b, T* xsum, T* y,
@@ -497,10 +529,10 @@ cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, co
     const size_t ring = VEC ? sizeof(uint4) * BwdStages<VPL * THREADS>::N * (dres != nullptr ? 3 : 2) * VPL * THREADS : 0;         \
     const size_t fold = TPR < 256 && partial != nullptr ? 2 * d * sizeof(float) : 0;                                     \
     const size_t smem = ring > fold ? ring : fold;                                                                       \
-    auto kernel = layernorm_bwd_kernel<T, WT, TPR, VPL, VEC>;                                                            \
+    auto kernel = layernorm_bwd_kernel<T, WT, TPR, VPL, VEC, false>;                                                     \
     if (smem > 46 * 1024 && !more_shared(reinterpret_cast<const void*>(kernel))) return cudaErrorInvalidValue;           \
     return launch_pdl(kernel, dim3(nblocks), dim3(THREADS), smem, stream, dy, ldy, x, ldx, w, stats, dres, ldr, dx,      \
-                      partial, rows, d, inv_d);                                                                          \
+                      partial, rows, d, inv_d, 1, d);                                                                    \
   } while (0)
   if (chunks <= 32) FMB_LN_BWD(32, 1);
   if (chunks <= 64) FMB_LN_BWD(64, 1);
@@ -509,6 +541,15 @@ cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, co
   if (chunks <= 512) FMB_LN_BWD(256, 2);
   if (chunks <= BWD_CHUNKS) FMB_LN_BWD(512, 2);
 #undef FMB_LN_BWD
+  if (chunks <= BWD_CHUNKS * BWD_SPLIT / 2) {
+    constexpr int N = Vec16<T>::N;
+    const int split = bwd_split(chunks), width = (chunks + split - 1) / split * N;
+    const size_t smem = VEC ? sizeof(uint4) * BwdStages<512>::N * (dres != nullptr ? 3 : 2) * 512 : 0;
+    auto kernel = layernorm_bwd_kernel<T, WT, 256, 2, VEC, true>;
+    if (smem > 46 * 1024 && !more_shared(reinterpret_cast<const void*>(kernel))) return cudaErrorInvalidValue;
+    return launch_pdl_cluster(kernel, dim3(nblocks * split), dim3(256), smem, split, stream, dy, ldy, x, ldx, w, stats, dres, ldr, dx,
+                              partial, rows, d, inv_d, split, width);
+  }
   layernorm_bwd_wide_kernel<T, WT><<<static_cast<unsigned>(rows), 1024, 0, stream>>>(dy, ldy, x, ldx, w, stats, dres, ldr, dx,
                                                                                     d, inv_d);
   if (partial != nullptr)
@@ -556,7 +597,13 @@ extern "C" int fmb_layernorm_fwd(const void* x, long long ldx, const void* delta
 extern "C" int fmb_layernorm_bwd_blocks(long long rows, int d, int dtype) {
   const int n = dtype == FMB_BF16 ? 8 : 4;
   const int chunks = (d + n - 1) / n;
-  if (chunks > BWD_CHUNKS) return static_cast<int>(rows < 32 ? (rows < 1 ? 1 : rows) : 32);
+  if (chunks > BWD_CHUNKS * BWD_SPLIT / 2) return static_cast<int>(rows < 32 ? (rows < 1 ? 1 : rows) : 32);
+  if (chunks > BWD_CHUNKS) {
+    // clusters, two blocks per SM; one in eight less than there is room for by numbers, because SMs come in groups that
+    // need not be whole clusters, and a second wave would double the time
+    const long long most = 2LL * sm_count() / bwd_split(chunks) * 7 / 8;
+    return static_cast<int>(rows < 1 ? 1 : rows < most ? rows : most);
+  }
   const int per_row = chunks <= 32 ? 32 : chunks <= 128 ? 64 : chunks <= 256 ? 128 : 256;
   const long long need = (rows + 256 / per_row - 1) / (256 / per_row);
   const long long most = static_cast<long long>(sm_count()) * (chunks <= 64 ? 4 : chunks <= 512 ? 2 : 1);      // as many as are resident

@@ -260,7 +260,7 @@ def test_kl_topk_wider_than_eight_blocks_of_64_kb(rows, V, keep, dtype):
     rowwise.check_kl(student, values, index, 1.5)
 
 
-@pytest.mark.parametrize("d", [8256, 16384, 16388, 20001])
+@pytest.mark.parametrize("d", [8256, 16384, 16388, 20001, 32768])
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_layer_norm_wide_rows(d, dtype):
     rowwise.test_layer_norm(300, d, dtype, "fp32")
