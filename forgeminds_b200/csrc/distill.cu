@@ -60,7 +60,7 @@ struct KlParams {
   const long long* index;          // [rows, K]
   const float* lse;                // [rows] or null
   float* row_loss;                 // [rows]
-  float2* stats;                   // [rows]: (maximum, sum of exponentials)
+  float2* stats;                   // [rows]: (a logit that is the maximum or near it, sum of exponentials around it)
   void* grad;                      // [rows, V] contiguous (its pitch is ldg), or null
   long long ldg;
   const int* count;                // rows that count (mean), or null
@@ -284,17 +284,20 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
 
 // ------------------------------------------------------------------ rows that stay in shared memory
 // A row is split over the CTAs of a cluster, at most 64 KB for each so that three of them share an SM: the logits are read
-// from memory once, and maximum, sum and gradient are taken from there. A thread keeps to its own 16-byte vectors, and as
-// soon as the gradient has used one, the same place receives the next row's: loads, exponentials and stores of the SM's
-// CTAs overlap. Few threads per row (256, or 128), because the reductions and the row's bookkeeping cost each warp as much as some
-// fifty vectors do. Kept logit k belongs to thread k, whose maximum and sums join the row's own reductions. The CTAs of a
-// row exchange (maximum, sum around it, loss) once. Rows are given out one by one: clusters that find no place at first,
-// while an earlier kernel still holds some SMs, would otherwise be a second wave.
-// Measured, with gradient, bf16: 8192 x 32000 in 204 us (5.1 TB/s of logits and gradient; one block per row that reads it
-// twice: 386), 4096 x 128259 over four CTAs in 472 us (4.5 TB/s; 758): there a row's CTAs wait for one another for a fifth
-// of the time. Both exponentials of a logit together hold the special function unit for 60 % of it.
+// from memory once, and the sum of exponentials and the gradient are taken from there. A thread keeps to its own 16-byte
+// vectors, and as soon as the gradient has used one, the same place receives the next row's: loads, exponentials and stores
+// of the SM's CTAs overlap. The sum is one pass: exponentials are taken around a logit that is within 2^8 of the largest so
+// far, and the threads' sums are brought to the row's largest such logit afterwards (with a pass for the maximum before it
+// 204 us where this takes 198). Few threads per row (256, or 128), because the reductions and the row's bookkeeping cost each
+// warp as much as some fifty vectors do. Kept logit k belongs to thread k, whose maximum and sums join the row's own
+// reductions. The CTAs of a row exchange (maximum, sum around it, loss) once. Rows are given out one by one: clusters that
+// find no place at first, while an earlier kernel still holds some SMs, would otherwise be a second wave.
+// Measured, with gradient, bf16: 8192 x 32000 in 198 us (5.3 TB/s of logits and gradient; one block per row that reads it
+// twice: 386), 4096 x 128259 over four CTAs in 467 us (4.5 TB/s; 758): there a row's CTAs wait for one another for a fifth
+// of the time. Both exponentials of a logit together hold the special function unit for 60 % of it, half of the issue slots
+// are used.
 struct KlPart {
-  float m, s, a;                                           // maximum, sum of exponentials around it, sum e (log e - x / tau)
+  float m, s, a;                                           // logit near the maximum, sum of exponentials around it, sum e (log e - x / tau)
 };
 
 // A row of V values: `head` of them before the first 16-byte boundary, then nv whole vectors, then the rest. The up to
@@ -354,6 +357,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
   const int first = rank * per_cta;                        // this CTA's first vector
   const bool slot = threadIdx.x < p.K;
   const F2 c2 = f2(c, c);
+  const float slack = 8.f / c;
   float single = -CUDART_INF_F;
   // vectors of this CTA in a row
   auto held = [&](const KlRow<T>& r) { return min(per_cta, r.nv - first); };
@@ -402,26 +406,43 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     const int at = slot_counts(slot_index, slot_value, p.V) ? static_cast<int>(slot_index) : -1;
     const float t = at >= 0 ? to_f32(slot_value) * inv_tau : -CUDART_INF_F;
     asm volatile("cp.async.wait_all;" ::: "memory");       // its own copies: other threads read them behind a barrier
-    // maxima of this CTA's part and of the teacher's logits
-    float m = single;
-    if constexpr (sizeof(T) == 2) {
-      uint32_t top = 0xff80ff80u;                          // -inf
-#pragma unroll 4
+    // one pass: exponentials of this thread's logits around `around`, which need not be their maximum, only within 2^8 of it
+    float around = single;
+    F2 sums = f2(single == -CUDART_INF_F ? 0.f : 1.f, 0.f), more = f2(0.f, 0.f);
+    {
+      float limit = around + slack;
+      F2 less = f2(0.f, 0.f);
+      auto start = [&](float top) {                        // rare, but for the first vector
+        const float k = around == -CUDART_INF_F ? 0.f : exp2_unit((around - top) * c);
+        sums = f2_mul(sums, f2(k, k));
+        more = f2_mul(more, f2(k, k));
+        around = top;
+        limit = top + slack;
+        less = f2(-top * c, -top * c);
+      };
+      if (around != -CUDART_INF_F) less = f2(-around * c, -around * c);
+#pragma unroll 2
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const uint4 x = s_row[i];
-        top = max_bf16x2(max_bf16x2(max_bf16x2(top, x.x), max_bf16x2(x.y, x.z)), x.w);
-      }
-      m = fmaxf(m, fmaxf(__uint_as_float(top << 16), __uint_as_float(top & 0xffff0000u)));
-    } else {
-#pragma unroll 4
-      for (int i = threadIdx.x; i < n; i += THREADS) {
-        float f[N];
-        Vec16<T>::unpack(s_row[i], f);
+        float f[N], top;
+        Vec16<T>::unpack(x, f);
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t u = max_bf16x2(max_bf16x2(x.x, x.y), max_bf16x2(x.z, x.w));
+          top = fmaxf(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+        } else {
+          top = fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3]));
+        }
+        if (!(top <= limit)) start(top);
 #pragma unroll
-        for (int j = 0; j < N; ++j) m = fmaxf(m, f[j]);
+        for (int j = 0; j < H; ++j) {
+          const float2 o = (f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, less));
+          if (j % 2) more = f2_add(more, f2(exp2_unit(o.x), exp2_unit(o.y)));
+          else sums = f2_add(sums, f2(exp2_unit(o.x), exp2_unit(o.y)));
+        }
       }
+      sums = f2_add(sums, more);
     }
-    m = lanes_max<32>(m);
+    float m = lanes_max<32>(around);
     float ref = lanes_max<32>(t);
     if (lane == 0) s_max[warp] = make_float2(m, ref);
     if (threadIdx.x < 2 * N) s_single[threadIdx.x] = single;
@@ -438,25 +459,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     float next_single = next < p.rows ? load_single(rn) : -CUDART_INF_F;
     load_slot(next);
     // sums: exponentials of the student, e = exp(t - ref) of the teacher, and e (t - ref - x / tau) where x is held here
-    const float mc = m == -CUDART_INF_F ? 0.f : m * c;
-    F2 sums = f2(0.f, 0.f);
-    {
-      const F2 mc2 = f2(-mc, -mc);
-      F2 more = f2(0.f, 0.f);
-#pragma unroll 2
-      for (int i = threadIdx.x; i < n; i += THREADS) {
-        float f[N];
-        Vec16<T>::unpack(s_row[i], f);
-#pragma unroll
-        for (int j = 0; j < H; ++j) {
-          const float2 o = (f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, mc2));
-          if (j % 2) more = f2_add(more, f2(exp2_unit(o.x), exp2_unit(o.y)));
-          else sums = f2_add(sums, f2(exp2_unit(o.x), exp2_unit(o.y)));
-        }
-      }
-      sums = f2_add(sums, more);
-    }
-    float s = sums.x + sums.y + exp2_unit(fmaf(single, c, -mc)), e = 0.f, a = 0.f, xk = 0.f;
+    float s = (sums.x + sums.y) * (around == -CUDART_INF_F ? 0.f : exp2_unit((around - m) * c)), e = 0.f, a = 0.f, xk = 0.f;
     bool mine = false, twice = false;                      // whether the student's logit at the index is held here
     int mark = -1;
     if (at >= 0) {
