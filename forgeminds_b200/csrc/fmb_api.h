@@ -88,7 +88,8 @@ int fmb_sum_f32(const float* x, float* out, long long n, float scale, int accumu
 // ---- distillation from a teacher's top logits (distill.cu)
 #define FMB_KL_MAX_KEEP 1024
 #define FMB_KL_SCRATCH 260            // ints
-// Row losses, row statistics (float2: a logit at or near the maximum, sum of exponentials around it) and, when given, the gradient for an upstream
+// Row losses, row statistics (float2: a logit at or near the maximum, sum of exponentials around it) and, when given, the
+// gradient for an upstream
 // gradient of 1 (rows `ldg` apart; may be the student itself). values / index [rows, K]; lse [rows] may be null. ws:
 // scratch of `ws_ints` >= FMB_KL_SCRATCH ints, ws[0] receives the number of rows that count when `mean` and no `count` is
 // given. loss (may be null): the sum of the rows, divided by the count when `mean`.
