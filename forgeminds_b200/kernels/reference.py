@@ -137,6 +137,7 @@ def rotary(x, cos, sin, positions=None, interleaved: bool = False):
     """Rotation of the first ``2 * cos.shape[-1]`` values of each head of ``x [B, T, H, D]`` by the angles of table row
     ``position``: a negative position leaves the head as it is, one past the table gives NaN."""
     T, R = x.shape[1], 2 * cos.shape[-1]
+    stay = None
     if positions is None:
         c, s = cos[:T], sin[:T]
     else:
@@ -149,6 +150,8 @@ def rotary(x, cos, sin, positions=None, interleaved: bool = False):
     a, b = (xf[..., 0:R:2], xf[..., 1:R:2]) if interleaved else (xf[..., : R // 2], xf[..., R // 2: R])
     u, v = a * c - b * s, a * s + b * c
     turned = torch.stack((u, v), dim=-1).flatten(-2) if interleaved else torch.cat((u, v), dim=-1)
+    if stay is not None:
+        turned = torch.where(stay.unsqueeze(-2), xf[..., :R], turned)      # infinities too
     return torch.cat((turned, xf[..., R:]), dim=-1).to(x.dtype)
 
 

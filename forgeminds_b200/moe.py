@@ -61,7 +61,7 @@ class _AllToAll(torch.autograd.Function):
 
 class Router(nn.Module):
     """Gate and choice of experts. The options beyond ``top_k`` are those of ``fm.kernels.route_experts``;
-    ``balance_bias=True`` adds the buffer ``bias [n_experts]`` (zeros), which :meth:`rebalance` moves."""
+    ``balance_bias=True`` adds the buffer ``bias [n_experts]`` (zeros, always fp32), which :meth:`rebalance` moves."""
 
     def __init__(self, dim: int, n_experts: int, top_k: int, score: str = "softmax", balance_bias: bool = False,
                  n_groups: int = 1, top_groups: int = 1, group_best: int = 2, renormalise: bool = True,
@@ -77,6 +77,14 @@ class Router(nn.Module):
                             renormalise=bool(renormalise), scale=float(scale))
         self.register_buffer("bias", torch.zeros(n_experts) if balance_bias else None)
         self.last_counts: Optional[torch.Tensor] = None
+
+    def _apply(self, fn, recurse=True):
+        """Casts of the model leave the balance bias in fp32: steps of a thousandth are lost in fewer bits."""
+        bias = self.bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.bias.dtype != torch.float32:
+            self.bias = self.bias.float() if bias.is_meta or self.bias.is_meta else bias.to(self.bias.device, torch.float32)
+        return self
 
     def choose(self, logits, aux_coef: float, z_coef: float):
         """``logits [N, E]`` -> ``(weights fp32 [N, k], idx int32 [N, k], aux)`` by the options; keeps the counts."""

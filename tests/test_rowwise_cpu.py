@@ -343,3 +343,29 @@ def test_moe_defaults_route_as_before():
     probs = moe.router.gate(x).softmax(-1)
     v, i = probs.topk(2, dim=-1)
     assert torch.equal(idx, i) and torch.allclose(w, v / v.sum(-1, keepdim=True))
+
+
+def test_rotary_leaves_negative_positions_as_they_are():
+    x = _randn(1, 3, 2, 8)
+    x[0, 1, 0, 2] = float("inf")
+    x.requires_grad_()
+    cos, sin = K.rotary_tables(4, 6)
+    for interleaved in (False, True):
+        y = K.rotary(x, cos, sin, torch.tensor([2, -1, 0]), interleaved)
+        assert torch.equal(y[:, 1], x[:, 1])
+        (g,) = torch.autograd.grad(y[:, 1].sum(), x)
+        assert torch.equal(g[:, 1], torch.ones_like(g[:, 1])) and not g[:, ::2].any()
+
+
+def test_the_balance_bias_stays_in_fp32():
+    moe = fm.MoE(16, 32, 8, 2, balance_bias=True)
+    moe.router.bias += 0.501
+    before = moe.router.bias.clone()
+    moe.to(torch.bfloat16)
+    assert moe.router.bias.dtype == torch.float32 and torch.equal(moe.router.bias, before)
+    assert moe.router.gate.weight.dtype == torch.bfloat16 and "router.bias" in moe.state_dict()
+    moe.double()
+    assert moe.router.bias.dtype == torch.float32 and moe.router.gate.weight.dtype == torch.float64
+    meta = fm.MoE(16, 32, 8, 2, balance_bias=True).to("meta").to_empty(device="cpu")
+    assert meta.router.bias.shape == (8,) and meta.router.bias.dtype == torch.float32
+    assert fm.MoE(16, 32, 8, 2).to(torch.bfloat16).router.bias is None
