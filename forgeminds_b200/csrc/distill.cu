@@ -502,7 +502,8 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(s) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a) : "memory");
       }
-      cluster_sync_all();
+      cluster_arrive_after(warp == 0);
+      cluster_wait();
       m = s_part[side][0].m;
       for (int i = 1; i < split; ++i) m = fmaxf(m, s_part[side][i].m);
       s = a = 0.f;
@@ -625,7 +626,7 @@ template <typename T, typename TT, int THREADS> int kl_row_launch(const KlParams
   const long long groups = p.rows < fit ? p.rows : fit;
   const dim3 grid(static_cast<unsigned>(groups * split));
   const cudaError_t e = split == 1 ? launch_pdl(kernel, grid, dim3(THREADS), smem, stream, p, split, per_cta)
-                                   : launch_pdl_cluster(kernel, grid, dim3(THREADS), smem, split, stream, p, split, per_cta);
+                                   : launch_cluster(kernel, grid, dim3(THREADS), smem, split, stream, p, split, per_cta);
   return e == cudaSuccess ? 0 : -3;
 }
 

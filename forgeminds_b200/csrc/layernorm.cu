@@ -193,39 +193,21 @@ layernorm_fwd_wide_kernel(const T* __restrict__ x, long long ldx, const T* __res
 // come through a ring of shared memory, copied STAGES - 1 rows ahead, each thread its own chunks (no barrier guards them):
 // with loads into registers a block waited out the memory's latency at every row. Two chunks per thread from 65 on: what a
 // row costs beside its columns (two sums over its threads, statistics, addresses) is as much as 130 instructions a thread.
-// SPLIT: a row of more than 1024 chunks is shared by the blocks of a cluster, `width` columns for each, which exchange their
-// two sums: 3024 x 12088 in 111 us (one block per row that reads it twice, and the columns once more: 160), a third of the
-// bandwidth, because the blocks wait for one another at every row.
-// dx, dw and db of bf16 rows with dres, the column sums included: 16384 x 4096 in 96 us (5.6 TB/s; with one chunk per
-// thread 112, from registers 125), 65536 x 1024 in 88 us (6.1 TB/s; one chunk 96).
-template <typename T, typename WT, int TPR, int VPL, bool VEC, bool SPLIT>
+template <typename T, typename WT, int TPR, int VPL, bool VEC>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : VPL > 1 ? 2 : 4)
 layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
                      const WT* __restrict__ w, const float2* __restrict__ stats, const T* __restrict__ dres, long long ldr,
-                     T* __restrict__ dx, float* __restrict__ partial, long long rows, const int whole, float inv_d, const int split,
-                     const int width) {
+                     T* __restrict__ dx, float* __restrict__ partial, long long rows, int d, float inv_d) {
   using M = RowMap<T, TPR, VEC>;
   constexpr int N = M::N, THREADS = TPR > 256 ? TPR : 256, RPB = THREADS / TPR;
   constexpr int STAGES = BwdStages<VPL * THREADS>::N;
-  static_assert(!SPLIT || RPB == 1, "a block has one row at a time");
-  __shared__ float2 scratch[2][THREADS / 32], s_peers[2][SPLIT ? 8 : 1];
+  __shared__ float2 scratch[2][THREADS / 32];
   extern __shared__ uint4 s_ring[];                       // [stage][dy, x, dres][chunk][thread]; the fold below takes its place
   float* s_fold = reinterpret_cast<float*>(s_ring);       // [2, d], when several rows share a block
   pdl_wait();
   pdl_launch_dependents();
   const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
   const int tensors = dres != nullptr ? 3 : 2;
-  const int rank = SPLIT ? static_cast<int>(cluster_ctarank()) : 0, group = SPLIT ? blockIdx.x / split : blockIdx.x;
-  const int groups = SPLIT ? gridDim.x / split : gridDim.x, from_col = SPLIT ? rank * width : 0;
-  const int d = SPLIT ? max(0, min(width, whole - from_col)) : whole;      // this block's columns
-  if constexpr (SPLIT) {
-    dy += from_col;
-    x += from_col;
-    dx += from_col;
-    if (dres != nullptr) dres += from_col;
-    if (w != nullptr) w += from_col;
-    cluster_sync_all();                                   // every block of the row runs before one writes to another
-  }
   constexpr int H = N / 2;
   F2 wv[VPL][H], dwa[VPL][H], dba[VPL][H];
 #pragma unroll
@@ -236,14 +218,14 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
     for (int j = 0; j < H; ++j) { wv[i][j] = f2(f[2 * j], f[2 * j + 1]); dwa[i][j] = dba[i][j] = f2(0.f, 0.f); }
   }
   // Everything a row needs moves on by one step: pointers, not products, and rows in 31 bits.
-  const int n_rows = static_cast<int>(rows), step = groups * RPB, start = group * RPB + sub;
+  const int n_rows = static_cast<int>(rows), step = gridDim.x * RPB, start = blockIdx.x * RPB + sub;
   const int row_bytes = tensors * VPL * THREADS * 16;
   const char* ring = reinterpret_cast<const char*>(s_ring + threadIdx.x);
   const uint32_t ring_at = smem_at(ring);
-  const long long step_dy = step * ldy, step_x = step * ldx, step_res = step * ldr, step_out = static_cast<long long>(step) * whole;
+  const long long step_dy = step * ldy, step_x = step * ldx, step_res = step * ldr, step_out = static_cast<long long>(step) * d;
   const int own = VEC ? M::col(0, 0, t) : 0;              // this thread's first column, where its chunks are contiguous
   const T *next_dy = dy + start * ldy + own, *next_x = x + start * ldx + own, *next_res = dres + start * ldr + own;
-  T* out = dx + static_cast<long long>(start) * whole;
+  T* out = dx + static_cast<long long>(start) * d;
   int next_row = start;
   int put = 0, get = 0;                                   // bytes from the ring's start
   auto copy = [&](const T* from, int tensor) {
@@ -279,7 +261,7 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
   }
   int turn = 0;
   float2 st = stats[min(start, n_rows - 1)];
-  for (int base = group * RPB; base < n_rows; base += step, out += step_out) {
+  for (int base = blockIdx.x * RPB; base < n_rows; base += step, out += step_out) {
     const int row = base + sub;
     const int width = RPB == 1 || row < n_rows ? d : 0;   // rows beyond the last take part in the sums with nothing
     const float2 next_st = stats[min(row + step, n_rows - 1)];
@@ -316,21 +298,7 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
       }
     }
     if constexpr (VEC) fetch();                           // into the place of the row before
-    float2 sums = row_sum2<TPR>(s1.x + s1.y, s2.x + s2.y, scratch[turn]);
-    if constexpr (SPLIT) {
-      if (threadIdx.x < split) {
-        const uint32_t to = mapa_shared(smem_at(&s_peers[turn][rank]), threadIdx.x);
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.x) : "memory");
-        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sums.y) : "memory");
-      }
-      cluster_sync_all();                                 // the other half of s_peers is read by now
-      sums = make_float2(0.f, 0.f);
-      for (int i = 0; i < split; ++i) {
-        const float2 o = s_peers[turn][i];
-        sums.x += o.x;
-        sums.y += o.y;
-      }
-    }
+    const float2 sums = row_sum2<TPR>(s1.x + s1.y, s2.x + s2.y, scratch[turn]);
     turn ^= 1;
     const F2 c1 = f2(-sums.x * inv_d, -sums.x * inv_d), c2 = f2(-sums.y * inv_d, -sums.y * inv_d);
 #pragma unroll
@@ -355,7 +323,7 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
   }
   asm volatile("cp.async.wait_all;" ::: "memory");
   if (partial == nullptr) return;
-  float* mine = partial + static_cast<long long>(group) * 2 * whole + from_col;
+  float* mine = partial + static_cast<long long>(blockIdx.x) * 2 * d;
   if constexpr (RPB > 1) {
     for (int who = 0; who < RPB; ++who) {                 // the block's row groups one after another: a fixed order
       __syncthreads();
@@ -384,10 +352,173 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
         const float2 a = dwa[i][j / 2], b = dba[i][j / 2];
         if (c < d) {
           mine[c] = j % 2 ? a.y : a.x;
-          mine[whole + c] = j % 2 ? b.y : b.x;
+          mine[d + c] = j % 2 ? b.y : b.x;
         }
       }
   }
+}
+
+// Rows of more than 1024 chunks: a cluster of blocks shares each, `width` columns (at most 512 chunks) for a block, and
+// exchanges the two sums. The blocks do not wait for one another: between a row's exchange and its result each takes the
+// sums of the next row, so three rows are in the ring, one of them on its way.
+constexpr int CLUSTER_STAGES = 3;
+template <typename T, typename WT, bool VEC>
+__global__ void __launch_bounds__(256, 2)
+layernorm_bwd_cluster_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx, const WT* __restrict__ w,
+                             const float2* __restrict__ stats, const T* __restrict__ dres, long long ldr, T* __restrict__ dx,
+                             float* __restrict__ partial, long long rows, const int whole, float inv_d, const int split, const int width) {
+  using M = RowMap<T, 256, VEC>;
+  constexpr int N = M::N, H = N / 2, VPL = 2;
+  __shared__ float2 scratch[2][8], s_peers[2][8];
+  extern __shared__ uint4 s_ring[];                       // [stage][dy, x, dres][chunk][thread]
+  pdl_wait();
+  pdl_launch_dependents();
+  const int t = threadIdx.x, rank = static_cast<int>(cluster_ctarank()), group = blockIdx.x / split, step = gridDim.x / split;
+  const int n_rows = static_cast<int>(rows), from_col = rank * width, d = max(0, min(width, whole - from_col));
+  const int tensors = dres != nullptr ? 3 : 2;
+  F2 wv[VPL][H], dwa[VPL][H], dba[VPL][H];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    float f[N];
+    M::weights(w != nullptr ? w + from_col : w, f, i, t, d, 1.f);
+#pragma unroll
+    for (int j = 0; j < H; ++j) { wv[i][j] = f2(f[2 * j], f[2 * j + 1]); dwa[i][j] = dba[i][j] = f2(0.f, 0.f); }
+  }
+  // Everything a row needs moves on by one step: pointers and bytes from the ring's start.
+  const int row_bytes = tensors * VPL * 256 * 16;
+  const char* ring = reinterpret_cast<const char*>(s_ring + t);
+  const uint32_t ring_at = smem_at(ring);
+  const long long step_dy = step * ldy, step_x = step * ldx, step_res = step * ldr, step_out = static_cast<long long>(step) * whole;
+  const int own = from_col + (VEC ? M::col(0, 0, t) : 0);
+  const T *next_dy = dy + group * ldy + own, *next_x = x + group * ldx + own, *next_res = dres + group * ldr + own;
+  T* out = dx + static_cast<long long>(group) * whole + from_col;
+  int next_row = group, put = 0;
+  auto copy = [&](const T* from, int tensor) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (M::col(i, 0, t) < d)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(ring_at + put + (tensor * VPL + i) * 256 * 16),
+                     "l"(from + i * 256 * N) : "memory");
+  };
+  auto fetch = [&]() {                                    // one group for each row, an empty one behind the last
+    if (next_row < n_rows) {
+      copy(next_dy, 0);
+      copy(next_x, 1);
+      if (dres != nullptr) copy(next_res, 2);
+      next_dy += step_dy;
+      next_x += step_x;
+      next_res += step_res;
+      next_row += step;
+    }
+    put = put == (CLUSTER_STAGES - 1) * row_bytes ? 0 : put + row_bytes;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  auto take = [&](int row, int at, int tensor, int i, F2 (&v)[H]) {
+    uint4 u;
+    if constexpr (VEC) {
+      u = M::col(i, 0, t) < d ? *reinterpret_cast<const uint4*>(ring + at + (tensor * VPL + i) * 256 * 16) : make_uint4(0, 0, 0, 0);
+    } else {
+      u = M::load((tensor == 0 ? dy + row * ldy : tensor == 1 ? x + row * ldx : dres + row * ldr) + from_col, i, t, d);
+    }
+    float f[N];
+    Vec16<T>::unpack(u, f);
+#pragma unroll
+    for (int j = 0; j < H; ++j) v[j] = f2(f[2 * j], f[2 * j + 1]);
+  };
+  if constexpr (VEC) {
+#pragma unroll
+    for (int n = 0; n < CLUSTER_STAGES; ++n) fetch();
+  }
+  cluster_sync_all();                                     // every block of the row runs before one writes to another
+  int turn = 0, here = 0, before = 0;                     // bytes of this row's and the last one's place in the ring
+  float2 st = stats[min(group, n_rows - 1)], st_before = st;
+  // one step beyond the last row, for its result
+  for (int row = group; row < n_rows + step; row += step) {
+    const bool more = row < n_rows, had = row != group;   // the same in all blocks of the cluster
+    float2 sums = make_float2(0.f, 0.f), next_st = st;
+    if (more) {
+      next_st = stats[min(row + step, n_rows - 1)];
+      const F2 mean2 = f2(-st.x, -st.x), r2 = f2(st.y, st.y);
+      if constexpr (VEC) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      F2 s1 = f2(0.f, 0.f), s2 = s1;
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        F2 g[H], xh[H];
+        take(row, here, 0, i, g);
+        take(row, here, 1, i, xh);
+#pragma unroll
+        for (int j = 0; j < H; ++j) {                     // where there is no column dy is 0 and nothing is added
+          xh[j] = f2_mul(f2_add(xh[j], mean2), r2);
+          dwa[i][j] = f2_fma(g[j], xh[j], dwa[i][j]);
+          dba[i][j] = f2_add(dba[i][j], g[j]);
+          g[j] = f2_mul(g[j], wv[i][j]);
+          s1 = f2_add(s1, g[j]);
+          s2 = f2_fma(g[j], xh[j], s2);
+        }
+      }
+      sums = row_sum2<256>(s1.x + s1.y, s2.x + s2.y, scratch[turn]);
+    }
+    float2 whole_sums = make_float2(0.f, 0.f);
+    if (had) {
+      cluster_wait();
+      for (int i = 0; i < split; ++i) {
+        const float2 o = s_peers[turn ^ 1][i];
+        whole_sums.x += o.x;
+        whole_sums.y += o.y;
+      }
+    }
+    if (more) {
+      if (t < split) {
+        const uint32_t to = mapa_shared(smem_at(&s_peers[turn][rank]), t);
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.x) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sums.y) : "memory");
+      }
+      cluster_arrive_after(t < 32);                       // waited for in the next step
+    }
+    if (had) {
+      const int done = row - step;
+      const F2 mean2 = f2(-st_before.x, -st_before.x), r2 = f2(st_before.y, st_before.y);
+      const F2 c1 = f2(-whole_sums.x * inv_d, -whole_sums.x * inv_d), c2 = f2(-whole_sums.y * inv_d, -whole_sums.y * inv_d);
+#pragma unroll
+      for (int i = 0; i < VPL; ++i) {
+        F2 g[H], xh[H], add[H];
+        take(done, before, 0, i, g);
+        take(done, before, 1, i, xh);
+        if (dres != nullptr) take(done, before, 2, i, add);
+        float o[N];
+#pragma unroll
+        for (int j = 0; j < H; ++j) {
+          xh[j] = f2_mul(f2_add(xh[j], mean2), r2);
+          const F2 inner = f2_add(f2_fma(xh[j], c2, f2_mul(g[j], wv[i][j])), c1);
+          const float2 v = (dres != nullptr ? f2_fma(inner, r2, add[j]) : f2_mul(inner, r2));
+          o[2 * j] = v.x;
+          o[2 * j + 1] = v.y;
+        }
+        M::store(out, o, i, t, d);
+      }
+      out += step_out;
+      if constexpr (VEC) fetch();                         // into the place of the row that is done
+    }
+    before = here;
+    here = here == (CLUSTER_STAGES - 1) * row_bytes ? 0 : here + row_bytes;
+    turn ^= 1;
+    st_before = st;
+    st = next_st;
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  if (partial == nullptr) return;
+  float* mine = partial + static_cast<long long>(group) * 2 * whole + from_col;
+#pragma unroll
+  for (int i = 0; i < VPL; ++i)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const int c = M::col(i, j, t);
+      const float2 a = dwa[i][j / 2], b = dba[i][j / 2];
+      if (c < d) {
+        mine[c] = j % 2 ? a.y : a.x;
+        mine[whole + c] = j % 2 ? b.y : b.x;
+      }
+    }
 }
 
 // Rows too wide for the accumulators: dx by one block per row, and the weight's gradients by blocks of 256 columns
@@ -434,30 +565,30 @@ layernorm_bwd_cols_kernel(const T* __restrict__ dy, long long ldy, const T* __re
   mine[d + c] = b;
 }
 
-// Sums of the columns of partial [n, 2d] in a fixed order: 8 columns (one sector of 32 bytes) x 128 groups of rows per
-// block, so that even 1024 columns are work for 256 blocks.
-template <typename WT>
-__global__ void __launch_bounds__(1024)
+// Sums of the columns of partial [n, 2d] in a fixed order: 32 columns (a line of 128 bytes) x GROUPS groups of rows per block.
+template <typename WT, int GROUPS>
+__global__ void __launch_bounds__(32 * GROUPS)
 layernorm_cols_kernel(const float* __restrict__ partial, WT* __restrict__ dw, WT* __restrict__ db, int n, int d) {
-  __shared__ float red[32][9];
+  __shared__ float red[GROUPS][33];
   pdl_wait();
   pdl_launch_dependents();
-  const int c = blockIdx.x * 8 + threadIdx.x % 8;
+  const int lane = threadIdx.x % 32, group = threadIdx.x / 32;
+  const int c = blockIdx.x * 32 + lane;
   float s = 0.f;
   if (c < 2 * d) {
-#pragma unroll 4
-    for (int r = threadIdx.x / 8; r < n; r += 128) s += partial[static_cast<long long>(r) * 2 * d + c];
+#pragma unroll 8
+    for (int r = group; r < n; r += GROUPS) s += partial[static_cast<long long>(r) * 2 * d + c];
   }
-  s += __shfl_xor_sync(0xffffffffu, s, 8);
-  s += __shfl_xor_sync(0xffffffffu, s, 16);
-  if (threadIdx.x % 32 < 8) red[threadIdx.x / 32][threadIdx.x % 8] = s;
+  red[group][lane] = s;
   __syncthreads();
-  if (threadIdx.x < 256) {                                // warp y adds column y's 32 warps
-    s = lanes_sum<32>(red[threadIdx.x % 32][threadIdx.x / 32]);
-    const int out = blockIdx.x * 8 + threadIdx.x / 32;
-    if (threadIdx.x % 32 == 0 && out < 2 * d) {
+#pragma unroll
+  for (int k = 0; k < 32 / GROUPS; ++k) {                 // a warp adds 32 / GROUPS columns
+    const int col = group + k * GROUPS;
+    const float sum = lanes_sum<32>(lane < GROUPS ? red[lane][col] : 0.f);
+    const int out = blockIdx.x * 32 + col;
+    if (lane == 0 && out < 2 * d) {
       WT* to = out < d ? dw : db;
-      if (to != nullptr) to[out < d ? out : out - d] = from_f32<WT>(s);
+      if (to != nullptr) to[out < d ? out : out - d] = from_f32<WT>(sum);
     }
   }
 }
@@ -466,7 +597,7 @@ layernorm_cols_kernel(const float* __restrict__ partial, WT* __restrict__ dw, WT
 constexpr int FWD_CHUNKS = 4096;     // most chunks of a row that the forward kernel holds in registers (1024 threads x 4)
 constexpr int BWD_CHUNKS = 1024;     // and the backward kernel (512 x 2), beyond that clusters of
 constexpr int BWD_SPLIT = 8;         // at most so many blocks of 256 x 2
-inline int bwd_split(int chunks) { return chunks <= 2048 ? 4 : 8; }
+inline int bwd_split(int chunks) { return (chunks + 511) / 512; }
 
 template <typename T, typename WT, bool VEC, bool ADD>
 cudaError_t fwd_launch(const T* x, long long ldx, const T* delta, long long ldd, const WT* w, const WT* b, T* xsum, T* y,
@@ -529,10 +660,10 @@ cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, co
     const size_t ring = VEC ? sizeof(uint4) * BwdStages<VPL * THREADS>::N * (dres != nullptr ? 3 : 2) * VPL * THREADS : 0;         \
     const size_t fold = TPR < 256 && partial != nullptr ? 2 * d * sizeof(float) : 0;                                     \
     const size_t smem = ring > fold ? ring : fold;                                                                       \
-    auto kernel = layernorm_bwd_kernel<T, WT, TPR, VPL, VEC, false>;                                                     \
+    auto kernel = layernorm_bwd_kernel<T, WT, TPR, VPL, VEC>;                                                            \
     if (smem > 46 * 1024 && !more_shared(reinterpret_cast<const void*>(kernel))) return cudaErrorInvalidValue;           \
     return launch_pdl(kernel, dim3(nblocks), dim3(THREADS), smem, stream, dy, ldy, x, ldx, w, stats, dres, ldr, dx,      \
-                      partial, rows, d, inv_d, 1, d);                                                                    \
+                      partial, rows, d, inv_d);                                                                          \
   } while (0)
   if (chunks <= 32) FMB_LN_BWD(32, 1);
   if (chunks <= 64) FMB_LN_BWD(64, 1);
@@ -544,11 +675,11 @@ cudaError_t bwd_launch(const T* dy, long long ldy, const T* x, long long ldx, co
   if (chunks <= BWD_CHUNKS * BWD_SPLIT / 2) {
     constexpr int N = Vec16<T>::N;
     const int split = bwd_split(chunks), width = (chunks + split - 1) / split * N;
-    const size_t smem = VEC ? sizeof(uint4) * BwdStages<512>::N * (dres != nullptr ? 3 : 2) * 512 : 0;
-    auto kernel = layernorm_bwd_kernel<T, WT, 256, 2, VEC, true>;
+    const size_t smem = VEC ? sizeof(uint4) * CLUSTER_STAGES * (dres != nullptr ? 3 : 2) * 512 : 0;
+    auto kernel = layernorm_bwd_cluster_kernel<T, WT, VEC>;
     if (smem > 46 * 1024 && !more_shared(reinterpret_cast<const void*>(kernel))) return cudaErrorInvalidValue;
-    return launch_pdl_cluster(kernel, dim3(nblocks * split), dim3(256), smem, split, stream, dy, ldy, x, ldx, w, stats, dres, ldr, dx,
-                              partial, rows, d, inv_d, split, width);
+    return launch_cluster(kernel, dim3(nblocks * split), dim3(256), smem, split, stream, dy, ldy, x, ldx, w, stats, dres, ldr, dx, partial,
+                           rows, d, inv_d, split, width);
   }
   layernorm_bwd_wide_kernel<T, WT><<<static_cast<unsigned>(rows), 1024, 0, stream>>>(dy, ldy, x, ldx, w, stats, dres, ldr, dx,
                                                                                     d, inv_d);
@@ -571,8 +702,10 @@ int bwd_run(const void* dy, long long ldy, const void* x, long long ldx, const v
   cudaError_t e = vec ? bwd_launch<T, WT, true>(gp, ldy, xp, ldx, wp, st, rp, ldr, op, partial, rows, d, nblocks, stream)
                       : bwd_launch<T, WT, false>(gp, ldy, xp, ldx, wp, st, rp, ldr, op, partial, rows, d, nblocks, stream);
   if (e == cudaSuccess && partial != nullptr)
-    e = launch_pdl(layernorm_cols_kernel<WT>, dim3((2 * d + 7) / 8), dim3(1024), 0, stream, partial, static_cast<WT*>(dw),
-                   static_cast<WT*>(db), nblocks, d);
+    e = nblocks > 96 ? launch_pdl(layernorm_cols_kernel<WT, 32>, dim3((2 * d + 31) / 32), dim3(1024), 0, stream, partial,
+                                  static_cast<WT*>(dw), static_cast<WT*>(db), nblocks, d)
+                     : launch_pdl(layernorm_cols_kernel<WT, 8>, dim3((2 * d + 31) / 32), dim3(256), 0, stream, partial,
+                                  static_cast<WT*>(dw), static_cast<WT*>(db), nblocks, d);
   return e == cudaSuccess ? 0 : -3;
 }
 
@@ -594,14 +727,41 @@ extern "C" int fmb_layernorm_fwd(const void* x, long long ldx, const void* delta
   return -1;
 }
 
+// Clusters of `split` blocks that the device holds together (SMs come in groups that need not be whole clusters; a second
+// wave of a walk over the rows would double its time). Asked once per device and size.
+static int cluster_fit(int split) {
+  static int known[64][BWD_SPLIT + 1] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 16;
+  if (known[dev][split] == 0) {
+    auto kernel = layernorm_bwd_cluster_kernel<__nv_bfloat16, float, true>;
+    const size_t smem = sizeof(uint4) * CLUSTER_STAGES * 3 * 512;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(sm_count() / split * split);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (!more_shared(reinterpret_cast<const void*>(kernel)) || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      n = 16;
+    }
+    known[dev][split] = n;
+  }
+  return known[dev][split];
+}
+
 extern "C" int fmb_layernorm_bwd_blocks(long long rows, int d, int dtype) {
   const int n = dtype == FMB_BF16 ? 8 : 4;
   const int chunks = (d + n - 1) / n;
   if (chunks > BWD_CHUNKS * BWD_SPLIT / 2) return static_cast<int>(rows < 32 ? (rows < 1 ? 1 : rows) : 32);
   if (chunks > BWD_CHUNKS) {
-    // clusters, two blocks per SM; one in eight less than there is room for by numbers, because SMs come in groups that
-    // need not be whole clusters, and a second wave would double the time
-    const long long most = 2LL * sm_count() / bwd_split(chunks) * 7 / 8;
+    const long long most = cluster_fit(bwd_split(chunks));
     return static_cast<int>(rows < 1 ? 1 : rows < most ? rows : most);
   }
   const int per_row = chunks <= 32 ? 32 : chunks <= 128 ? 64 : chunks <= 256 ? 128 : 256;

@@ -336,6 +336,13 @@ __device__ __forceinline__ void cluster_sync_all() {
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 }
+// The same in two halves for kernels in which only the warps with `wrote` have written to other CTAs' shared memory. The
+// others' stores to global memory are then not waited for, as a release by every thread would do.
+__device__ __forceinline__ void cluster_arrive_after(bool wrote) {
+  if (wrote) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+  asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // Address of the same shared-memory location in CTA `rank` of this cluster (shared::cluster window).
 __device__ __forceinline__ uint32_t mapa_shared(uint32_t addr, uint32_t rank) {
   uint32_t r;
