@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
 // reductions. The CTAs of a row exchange (maximum, sum around it, loss) once. Rows are given out one by one: clusters that
 // find no place at first, while an earlier kernel still holds some SMs, would otherwise be a second wave.
 // Measured, with gradient, bf16: 8192 x 32000 in 198 us (5.3 TB/s of logits and gradient; one block per row that reads it
-// twice: 386), 4096 x 128259 over four CTAs in 467 us (4.5 TB/s; 758): there a row's CTAs wait for one another for a fifth
+// twice: 386), 4096 x 128259 over four CTAs in 456 us (4.6 TB/s; 758): there a row's CTAs wait for one another for a fifth
 // of the time. Both exponentials of a logit together hold the special function unit for 60 % of it, half of the issue slots
 // are used.
 struct KlPart {

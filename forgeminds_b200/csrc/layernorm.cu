@@ -5,7 +5,7 @@
 //
 // Bound by HBM bandwidth: about ten operations per element. A row lives in the registers of the threads that
 // share it (16-byte chunks), so that mean and variance are two exact passes and memory is read once. Sums,
-// statistics and the weight's gradients are fp32.
+// statistics and the weight's gradients are fp32. Forward with residual, 16384 x 4096 bf16: 86 us, 6.3 TB/s.
 #include "fmb_api.h"
 #include "launch.cuh"
 #include "ptx_sm100.cuh"
@@ -193,6 +193,8 @@ layernorm_fwd_wide_kernel(const T* __restrict__ x, long long ldx, const T* __res
 // come through a ring of shared memory, copied STAGES - 1 rows ahead, each thread its own chunks (no barrier guards them):
 // with loads into registers a block waited out the memory's latency at every row. Two chunks per thread from 65 on: what a
 // row costs beside its columns (two sums over its threads, statistics, addresses) is as much as 130 instructions a thread.
+// dx, dw and db of bf16 rows with dres, the column sums included: 16384 x 4096 in 94 us (5.7 TB/s; with one chunk per
+// thread 112, from registers 125), 65536 x 1024 in 88 us (6.1 TB/s; one chunk 96).
 template <typename T, typename WT, int TPR, int VPL, bool VEC>
 __global__ void __launch_bounds__(TPR > 256 ? TPR : 256, TPR > 256 ? 1 : VPL > 1 ? 2 : 4)
 layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx,
@@ -360,7 +362,9 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
 
 // Rows of more than 1024 chunks: a cluster of blocks shares each, `width` columns (at most 512 chunks) for a block, and
 // exchanges the two sums. The blocks do not wait for one another: between a row's exchange and its result each takes the
-// sums of the next row, so three rows are in the ring, one of them on its way.
+// sums of the next row, so three rows are in the ring, one of them on its way. bf16, no dres: 3024 x 12088 in 79 us (launched
+// while the previous kernel still ran 114; one block per row that reads it twice, and the columns once more, 160), 4096 x
+// 16384 in 113. 8192 x 8192, which 512 threads hold, takes 95 there and 111 on clusters of two.
 constexpr int CLUSTER_STAGES = 3;
 template <typename T, typename WT, bool VEC>
 __global__ void __launch_bounds__(256, 2)
