@@ -275,10 +275,19 @@ __device__ __forceinline__ bool sigmoid_ahead(float za, float zb, float bias_a, 
   return b > a || (b == a && lower);
 }
 
+// The same for softmax scores with their biases, from the row's largest logit and its fp32 sum of exponentials: 1 and 0, or
+// -1 where the sum's error (of some 25 roundings, and of the terms' own 2e-7: 2e-6, taken twice) leaves it open.
+__device__ __forceinline__ int softmax_ahead(float za, float zb, float bias_a, float bias_b, float top, float mass) {
+  const double s = (exp(static_cast<double>(zb) - top) - exp(static_cast<double>(za) - top)) / mass;
+  const double ahead = s + (static_cast<double>(bias_b) - static_cast<double>(bias_a));
+  return fabs(ahead) > 4e-6 * fabs(s) + 1e-14 ? ahead > 0.0 : -1;
+}
+
 // The choice of a warp's tokens where some neighbours j, j + 1 of key[0, k + 2) are closer than `apart`, or a token is in
 // doubt already: pairs that stand alone are put in order, other tokens decided again. Writes pick[0, k).
 template <typename T, int LPT, int VPL>
 __device__ __forceinline__ void settle(const RouteParams& p, const T* row, int lane, unsigned apart, bool doubt, bool flat_bias,
+                                       float top, float mass,
                                        const unsigned* key, int* pick, double* c64, double* g64) {
   const bool biased = p.bias != nullptr;
   auto close = [&](int j) { return key[j] != 0 && key[j + 1] != 0 && key_score(key[j]) - key_score(key[j + 1]) < apart; };
@@ -292,11 +301,17 @@ __device__ __forceinline__ void settle(const RouteParams& p, const T* row, int l
     if (za == zb && (!biased || p.bias[a] == p.bias[b])) {
       // equal in any precision, and the lower number is first; at the last choice the next one might belong before both
       doubt |= j == p.k - 1 && close(j + 1);
-    } else if ((biased && p.softmax) || (j > 0 && close(j - 1)) || close(j + 1)) {
+    } else if ((j > 0 && close(j - 1)) || close(j + 1)) {
       doubt = true;
-    } else if (biased ? sigmoid_ahead(za, zb, p.bias[a], p.bias[b], b < a) : zb > za || (zb == za && b < a)) {
-      pick[j] = b;
-      if (j + 1 < p.k) pick[j + 1] = a;
+    } else {
+      const int ahead = !biased ? zb > za || (zb == za && b < a)
+                        : p.softmax ? softmax_ahead(za, zb, p.bias[a], p.bias[b], top, mass)
+                                    : sigmoid_ahead(za, zb, p.bias[a], p.bias[b], b < a);
+      doubt |= ahead < 0;
+      if (ahead > 0) {
+        pick[j] = b;
+        if (j + 1 < p.k) pick[j + 1] = a;
+      }
     }
   }
   __syncwarp();
@@ -378,24 +393,29 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
   if (p.softmax || AUX) {
     if (top == -CUDART_INF_F) top = 0.f;                    // a row of nothing but -inf: scores of 0
     mass = 0.f;
+    float share[AUX ? VPL : 1], norm = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) mass += e0 + i < p.E ? expf(z[i] - top) : 0.f;
+    for (int i = 0; i < VPL; ++i) {
+      const float e = e0 + i < p.E ? expf(z[i] - top) : 0.f;
+      mass += e;
+      if constexpr (AUX) {
+        share[i] = p.softmax ? e : e0 + i < p.E ? sigmoid(z[i]) : 0.f;
+        norm += share[i];
+      }
+    }
     mass = lanes_sum<LPT>(mass);
     if (mass == 0.f) mass = 1.f;
+    if constexpr (AUX) {
+      norm = lanes_sum<LPT>(norm);
+      const float by = norm == 0.f ? 1.f : 1.f / norm;
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) acc[i] += share[i] * by;
+      }
+    }
   }
   if constexpr (AUX) {
-    float norm = mass;
-    if (!p.softmax) {
-      norm = 0.f;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) norm += e0 + i < p.E ? sigmoid(z[i]) : 0.f;
-      norm = lanes_sum<LPT>(norm);
-      if (norm == 0.f) norm = 1.f;
-    }
     if (live) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i)
-        if (e0 + i < p.E) acc[i] += (p.softmax ? expf(z[i] - top) : sigmoid(z[i])) / norm;
       const float lse = top + logf(mass);
       if (lane == 0) acc_z += lse * lse;
     }
@@ -473,14 +493,23 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
     } else {
       __syncwarp();
       unsigned* s_g = reinterpret_cast<unsigned*>(room.g64);
-      for (int n = lane; n < p.groups; n += LPT) {
+      int per = 1;                                          // lanes for a group
+      while (2 * per * p.groups <= LPT) per *= 2;
+      for (int n0 = 0; n0 < p.groups; n0 += LPT / per) {
+        const int n = n0 + lane / per;
         unsigned a = 0, b = 0;
-        for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
-          const unsigned v = s_n[e];
-          b = max(b, min(a, v));
-          a = max(a, v);
+        if (n < p.groups)
+          for (int e = n * p.gsize + lane % per; e < (n + 1) * p.gsize; e += per) {
+            const unsigned v = s_n[e];
+            b = max(b, min(a, v));
+            a = max(a, v);
+          }
+        for (int o = 1; o < per; o *= 2) {
+          const unsigned oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
+          b = max(max(b, ob), min(a, oa));
+          a = max(a, oa);
         }
-        s_g[n] = (a + (me.two_best ? b : 0u)) << 5 | (31 - n);
+        if (n < p.groups && lane % per == 0) s_g[n] = (a + (me.two_best ? b : 0u)) << 5 | (31 - n);
       }
       __syncwarp();
       unsigned kept = 0;
@@ -551,7 +580,7 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
         room.key[p.k + 1] = then;
       }
       __syncwarp();
-      settle<T, LPT, VPL>(p, row, lane, apart, doubt, !me.biased || scale.flat_bias, room.key, room.pick, room.c64, room.g64);
+      settle<T, LPT, VPL>(p, row, lane, apart, doubt, !me.biased || scale.flat_bias, top, mass, room.key, room.pick, room.c64, room.g64);
 #pragma unroll
       for (int n = 0; n < PER; ++n)
         if (n * LPT + lane < p.k) pick[n] = room.pick[n * LPT + lane];

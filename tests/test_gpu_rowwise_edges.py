@@ -265,3 +265,20 @@ def test_kl_topk_wider_than_eight_blocks_of_64_kb(rows, V, keep, dtype):
 def test_layer_norm_wide_rows(d, dtype):
     rowwise.test_layer_norm(300, d, dtype, "fp32")
     rowwise.test_add_layer_norm(41, d, dtype)
+
+
+@pytest.mark.parametrize("E,k", [(312, 14), (64, 8), (8, 3)])
+def test_route_softmax_scores_that_a_bias_brings_together(E, k):
+    """Pairs whose biased scores differ by a few units of 32 bits, on either side, and pairs that are equal by their inputs."""
+    z = randn(400, E, seed=9)
+    z[:, 1] = z[:, 0] - 0.5
+    s = torch.softmax(z.double(), dim=1)
+    for row in range(0, 400, 57):                              # the bias that makes experts 0 and 1 of this row nearly equal
+        for off in (0.0, 3e-9, -3e-9, 1e-7):
+            bias = 0.001 * randn(E, seed=10)
+            bias[0] = 0.5
+            bias[1] = (0.5 + s[row, 0] - s[row, 1] + off).float()
+            check_route(z[row: row + 1], k, "softmax", bias)
+    bias = torch.zeros(E, device="cuda")
+    check_route(z, k, "softmax", bias)
+    check_route(z, k, "softmax", 0.02 * randn(E, seed=11))
