@@ -54,82 +54,66 @@ __device__ __forceinline__ void load_logits(const T* row, int lane, int E, int v
 
 __device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + expf(-z)); }
 
-// A token's scores with their biases in 64 bits by its LPT lanes, into c[0, E) (not needed without a bias and groups), and
-// from them the groups that are kept. g: room for the groups' scores.
-template <typename T, int LPT>
-__device__ __forceinline__ unsigned exact_scores(const RouteParams& p, const T* row, int lane, double* c, double* g) {
-  if (p.bias == nullptr && p.groups <= 1) return 0xffffffffu;
-  double top = 0.0, sum = 1.0;
+// A token's choice in 64 bits by its LPT lanes: writes the chosen experts to pick[0, k). c, g: shared memory for E scores
+// and the groups'. Rare, and tens of thousands of cycles long: a pair of neighbours alone is put in order without it.
+template <typename T, int LPT, int VPL>
+__device__ __forceinline__ void choose_exactly(const RouteParams& p, const T* row, int lane, double* c, double* g, int* pick) {
+  const int e0 = lane * VPL;
+  double own[VPL];
+  double top = -CUDART_INF, sum = 0.0;
+  unsigned open = 0;                                       // experts of this lane that can be chosen
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    own[i] = e0 + i < p.E ? static_cast<double>(to_f32(row[e0 + i])) : -CUDART_INF;
+    if (e0 + i < p.E) open |= 1u << i;
+    top = fmax(top, own[i]);
+  }
   if (p.softmax) {
-    float high = -CUDART_INF_F;
-    for (int e = lane; e < p.E; e += LPT) high = fmaxf(high, to_f32(row[e]));
-    high = lanes_max<LPT>(high);
-    top = high == -CUDART_INF_F ? 0.0 : static_cast<double>(high);
-    sum = 0.0;
-#pragma unroll 2
-    for (int e = lane; e < p.E; e += LPT) {
-      c[e] = exp(static_cast<double>(to_f32(row[e])) - top);
-      sum += c[e];
-    }
+#pragma unroll
+    for (int o = LPT / 2; o > 0; o >>= 1) top = fmax(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if (top == -CUDART_INF) top = 0.0;
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += LPT) sum += exp(static_cast<double>(to_f32(row[e])) - top);
 #pragma unroll
     for (int o = LPT / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sum == 0.0) sum = 1.0;
   }
-#pragma unroll 2
-  for (int e = lane; e < p.E; e += LPT) {
-    const double v = (p.softmax ? c[e] / sum : 1.0 / (1.0 + exp(-static_cast<double>(to_f32(row[e]))))) +
-                     (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
-    c[e] = v != v ? CUDART_INF : v;
-  }
-  __syncwarp();
-  if (p.groups <= 1) return 0xffffffffu;
-  int per = 1;                                             // lanes for a group
-  while (2 * per * p.groups <= LPT) per *= 2;
-  for (int n0 = 0; n0 < p.groups; n0 += LPT / per) {
-    const int n = n0 + lane / per;
-    double a = -CUDART_INF, b = -CUDART_INF;               // the two largest
-    if (n < p.groups)
-      for (int e = n * p.gsize + lane % per; e < (n + 1) * p.gsize; e += per) {
-        const double v = c[e];
-        if (v > b) { b = v > a ? a : v; a = v > a ? v : a; }
-      }
-    for (int o = 1; o < per; o *= 2) {
-      const double oa = __shfl_xor_sync(0xffffffffu, a, o), ob = __shfl_xor_sync(0xffffffffu, b, o);
-      b = fmax(fmax(b, ob), fmin(a, oa));
-      a = fmax(a, oa);
+  if (p.bias != nullptr || p.groups > 1) {
+#pragma unroll 1
+    for (int e = lane; e < p.E; e += LPT) {
+      const double z = to_f32(row[e]);
+      const double v = (p.softmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z))) + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
+      c[e] = v != v ? CUDART_INF : v;
     }
-    const double v = p.best > 1 && p.gsize > 1 ? a + b : a;
-    if (n < p.groups && lane % per == 0) g[n] = v != v ? CUDART_INF : v;
+    __syncwarp();
   }
-  __syncwarp();
-  unsigned kept = 0;
-  for (int n = lane; n < p.groups; n += LPT) {
-    int ahead = 0;
-    for (int m = 0; m < p.groups; ++m) ahead += g[m] > g[n] || (g[m] == g[n] && m < n);
-    if (ahead < p.top_groups) kept |= 1u << n;
-  }
+  if (p.groups > 1) {
+    for (int n = lane; n < p.groups; n += LPT) {
+      double a = -CUDART_INF, b = -CUDART_INF;             // the two largest
+      for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
+        const double v = c[e];
+        b = fmax(b, fmin(a, v));
+        a = fmax(a, v);
+      }
+      const double v = p.best > 1 && p.gsize > 1 ? a + b : a;
+      g[n] = v != v ? CUDART_INF : v;
+    }
+    __syncwarp();
+    unsigned kept = 0;
+    for (int n = lane; n < p.groups; n += LPT) {
+      int ahead = 0;
+      for (int m = 0; m < p.groups; ++m) ahead += g[m] > g[n] || (g[m] == g[n] && m < n);
+      if (ahead < p.top_groups) kept |= 1u << n;
+    }
 #pragma unroll
-  for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
-  __syncwarp();
-  return kept;
-}
-
-// A token's choice in 64 bits by its LPT lanes: writes the chosen experts to pick[0, k). c, g: shared memory for E scores
-// and the groups'. Rare, and tens of thousands of cycles long: a pair of neighbours alone is put in order without it, and of
-// groups that are too near to tell only the groups are chosen so.
-template <typename T, int LPT, int VPL>
-__device__ __forceinline__ void choose_exactly(const RouteParams& p, const T* row, int lane, double* c, double* g, int* pick) {
-  const int e0 = lane * VPL;
-  const unsigned kept = exact_scores<T, LPT>(p, row, lane, c, g);
-  double own[VPL];
-  unsigned open = 0;                                       // experts of this lane that can be chosen
+    for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
+#pragma unroll
+    for (int i = 0; i < VPL; ++i)
+      if (e0 + i < p.E && !(kept >> ((e0 + i) / p.gsize) & 1)) open &= ~(1u << i);
+  }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {                          // without a bias the order of the logits is the scores'
-    own[i] = -CUDART_INF;
-    if (e0 + i < p.E) {
-      own[i] = p.bias != nullptr ? c[e0 + i] : static_cast<double>(to_f32(row[e0 + i]));
-      if (p.groups <= 1 || (kept >> ((e0 + i) / p.gsize) & 1)) open |= 1u << i;
-    }
+    if (p.bias != nullptr && e0 + i < p.E) own[i] = c[e0 + i];
     if (own[i] != own[i]) own[i] = CUDART_INF;
   }
   for (int j = 0; j < p.k; ++j) {
@@ -485,7 +469,6 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
   const unsigned by_logit = sizeof(T) == 2 ? 0u : 4u;       // bf16 logits' keys are exact
   if (me.grouped) {
     unsigned low = 0, out = 0;                              // the lowest group kept and the highest left out
-    unsigned kept = 0xffffffffu;
     if (me.whole_lanes) {
       make_list();
       unsigned a = lists_serve ? list[0] : first, b = lists_serve ? (L > 1 ? list[L > 1 ? 1 : 0] : 0u) : second;
@@ -504,7 +487,6 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
       }
       out = lanes_umax<LPT>(mine);
       if (whole < low || !me.has_group) {                   // a group that is left out
-        kept = 0;
 #pragma unroll
         for (int i = 0; i < L; ++i) list[i] = 0;
       }
@@ -530,7 +512,7 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
         if (n < p.groups && lane % per == 0) s_g[n] = (a + (me.two_best ? b : 0u)) << 5 | (31 - n);
       }
       __syncwarp();
-      kept = 0;
+      unsigned kept = 0;
       for (int n = lane; n < p.groups; n += LPT) {
         int ahead = 0;
         for (int m = 0; m < p.groups; ++m) ahead += s_g[m] > s_g[n];
@@ -542,26 +524,14 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
       for (int o = LPT / 2; o > 0; o >>= 1) kept |= __shfl_xor_sync(0xffffffffu, kept, o);
       low = lanes_umax<LPT>(low);
       out = lanes_umax<LPT>(out);
-      __syncwarp();
-    }
-    const unsigned apart = me.by_score ? 2 * near : by_logit;
-    const bool near_groups = p.top_groups < p.groups && (low >> 5) - (out >> 5) < apart;
-    bool again = !me.whole_lanes;
-    if constexpr (EXACT) {
-      if (__any_sync(0xffffffffu, near_groups)) {
-        const unsigned exact = exact_scores<T, LPT>(p, row, lane, room.c64, room.g64);
-        if (near_groups) kept = exact;
-        again |= near_groups;
-      }
-    } else {
-      doubt |= near_groups;
-    }
-    if (again) {
 #pragma unroll
       for (int i = 0; i < VPL; ++i)
         if (e0 + i < p.E && !(kept >> ((e0 + i) / p.gsize) & 1)) key[i] = 0;
+      __syncwarp();
       make_list();
     }
+    const unsigned apart = me.by_score ? 2 * near : by_logit;
+    doubt |= p.top_groups < p.groups && (low >> 5) - (out >> 5) < apart;
   } else {
     make_list();
   }
