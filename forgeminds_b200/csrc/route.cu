@@ -13,7 +13,7 @@
 // of score and fixed point, and not equal by their inputs, is decided again, in 64 bits where it must be; so is one with NaN
 // or +inf, and one of which a lane has given away its four.
 // Bound by these instructions (600 per token of 256 experts in 8 groups and 8 choices), not by memory: 65536 such tokens in
-// 56 us at two thirds of the issue slots, 17 us of memory traffic; their backward pass, all zeros but for 8 values, 18 us.
+// 58 us at two thirds of the issue slots, 17 us of memory traffic; their backward pass, all zeros but for 8 values, 18 us.
 #include "fmb_api.h"
 #include "launch.cuh"
 #include "rows.cuh"
@@ -371,6 +371,7 @@ struct RouteRoom {
 // The fixed point of biased scores: what 0 is, steps per score, and how near two scores may be without being told apart
 struct RouteScale {
   float lo, unit, error;                                   // error: twice that of a score of 1, in steps
+  unsigned near;                                           // how near sigmoid scores may be without being told apart
   bool bad_bias, flat_bias;                                // NaN or +inf: every choice is made in 64 bits; one finite bias for all
 };
 
@@ -420,9 +421,12 @@ __device__ __forceinline__ bool decide(const RouteParams& p, const RouteLane<LPT
       if (lane == 0) acc_z += lse * lse;
     }
   }
-  // no softmax score is above the largest one's, 1 / mass, and their errors are in proportion
-  const float inv_mass = p.softmax ? __fdividef(1.f, mass) : 1.f;
-  const unsigned near = static_cast<unsigned>(fminf(fmaf(scale.error, inv_mass, 4.f), 1e6f));
+  float inv_mass = 1.f;
+  unsigned near = scale.near;
+  if (p.softmax) {                                          // no score is above the largest one's, 1 / mass, and errors are in proportion
+    inv_mass = __fdividef(1.f, mass);
+    near = static_cast<unsigned>(fminf(fmaf(scale.error, inv_mass, 4.f), 1e6f));
+  }
   // fixed-point scores and keys; first, second: the lane's two largest for its group where the lists do not hold them
   unsigned key[VPL], list[L], first = 0, second = 0;
   const bool lists_serve = me.biased || !me.by_score;
@@ -662,7 +666,7 @@ __device__ __forceinline__ void load_bias(const RouteParams& p, int e0, const Ro
 
 // A warp's tokens once more, with whole lists and what 64 bits take. Everything is loaded here again and the code stands
 // inline, in a loop of its own: as a call from the middle of the loop over the tokens it made that loop spill (67 us where
-// this takes 56, 65536 tokens of 256 experts).
+// this takes 58, 65536 tokens of 256 experts).
 template <typename T, int LPT, int VPL>
 __device__ __forceinline__ void decide_again(const RouteParams& p, RouteScale scale, RouteRoom room, int token, bool live) {
   const RouteLane<LPT, VPL> me(p);
@@ -694,7 +698,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
   if (AUX)
     for (int e = threadIdx.x; e <= p.E; e += ROUTE_THREADS) s_acc[e] = 0.f;
   // the range of scores in fixed point: [0, 1] and what the finite biases add
-  RouteScale scale = {0.f, 1.f, 0.f, false, false};
+  RouteScale scale = {0.f, 1.f, 0.f, 0, false, false};
   float hi = 1.f, bias[VPL];
   if (me.biased) {
     float a = CUDART_INF_F, b = -CUDART_INF_F;
@@ -724,6 +728,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
   // sum of up to 512 terms some 30 roundings deep: 3e-6 of the score. Then a step of the fixed point. Two of those, and one
   // more, where a token's scores are taken: closer than that is too near.
   scale.error = (p.softmax ? 6e-6f : 6.8e-7f) * scale.unit;
+  scale.near = static_cast<unsigned>(fminf(scale.error + 4.f, 1e6f));
   float acc[AUX ? VPL : 1], acc_z = 0.f;
 #pragma unroll
   for (int i = 0; i < (AUX ? VPL : 1); ++i) acc[i] = 0.f;
