@@ -16,7 +16,7 @@
 namespace fmb {
 
 constexpr int KL_THREADS = 512;
-constexpr int KL_COUNT_BLOCKS = 256;
+constexpr int KL_COUNT_BLOCKS = 256, KL_COUNT_ROWS = 4;
 constexpr float LOG2E = 1.4426950408889634f;
 
 template <typename TT> __device__ __forceinline__ bool slot_counts(long long at, TT value, int V) {
@@ -28,7 +28,8 @@ template <typename TT> __device__ __forceinline__ bool slot_counts(long long at,
 constexpr int WS_COUNT = 0, WS_TICKET = 1, WS_TAKEN = 2, WS_PARTS = 4;
 static_assert(WS_PARTS + KL_COUNT_BLOCKS == FMB_KL_SCRATCH, "the caller's scratch");
 
-// Rows that have a slot that counts. One warp per row.
+// Rows that have a slot that counts. A warp looks at the first 32 slots of four rows at once, which nearly always settles
+// them (8192 rows of 64: 6.9 us with all slots of one row after another, 4.4 with this).
 template <typename TT>
 __global__ void __launch_bounds__(256)
 kl_topk_count_kernel(const TT* __restrict__ values, const long long* __restrict__ index, int* __restrict__ ws,
@@ -40,10 +41,25 @@ kl_topk_count_kernel(const TT* __restrict__ values, const long long* __restrict_
   __syncthreads();
   const int lane = threadIdx.x & 31;
   int n = 0;
-  for (long long row = blockIdx.x * 8LL + (threadIdx.x >> 5); row < rows; row += gridDim.x * 8LL) {
-    bool any = false;
-    for (int k = lane; k < K; k += 32) any |= slot_counts(index[row * K + k], values[row * K + k], V);
-    n += __any_sync(0xffffffffu, any) ? 1 : 0;
+  for (long long row = (blockIdx.x * 8LL + (threadIdx.x >> 5)) * KL_COUNT_ROWS; row < rows; row += gridDim.x * 8LL * KL_COUNT_ROWS) {
+    long long at[KL_COUNT_ROWS];
+    TT value[KL_COUNT_ROWS];
+#pragma unroll
+    for (int i = 0; i < KL_COUNT_ROWS; ++i) {
+      at[i] = -1;
+      value[i] = from_f32<TT>(0.f);
+      if (row + i < rows && lane < K) {
+        at[i] = index[(row + i) * K + lane];
+        value[i] = values[(row + i) * K + lane];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KL_COUNT_ROWS; ++i) {
+      bool any = __any_sync(0xffffffffu, slot_counts(at[i], value[i], V));
+      for (int k = 32 + lane; !any && row + i < rows && k - lane < K; k += 32)
+        any = __any_sync(0xffffffffu, k < K && slot_counts(index[(row + i) * K + min(k, K - 1)], values[(row + i) * K + min(k, K - 1)], V));
+      n += any ? 1 : 0;
+    }
   }
   if (lane == 0 && n) atomicAdd(&s_n, n);
   __syncthreads();
@@ -639,7 +655,8 @@ int kl_run(KlParams p, bool fwd, int* ws, bool mean, const int* count, cudaStrea
     p.taken = ws + WS_TAKEN;
   }
   if (fwd && mean && count == nullptr) {
-    p.n_parts = static_cast<int>((p.rows + 7) / 8 < KL_COUNT_BLOCKS ? (p.rows + 7) / 8 : KL_COUNT_BLOCKS);
+    const long long need = (p.rows + 8 * KL_COUNT_ROWS - 1) / (8 * KL_COUNT_ROWS);
+    p.n_parts = static_cast<int>(need < KL_COUNT_BLOCKS ? need : KL_COUNT_BLOCKS);
     p.parts = ws;
     e = launch_pdl(kl_topk_count_kernel<TT>, dim3(p.n_parts), dim3(256), 0, stream, static_cast<const TT*>(p.values), p.index, ws,
                    p.rows, p.V, p.K);

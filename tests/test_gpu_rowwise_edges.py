@@ -81,7 +81,7 @@ def test_kl_topk_scratch_holds_what_the_kernels_leave_there(rows):
     index[::3] = -1
     counted = rows - (rows + 2) // 3
     ws = ops.require().kl_topk_fwd(student, values, index, None, 1.0, True, True, None, True, False)[4]
-    blocks = min((rows + 7) // 8, 256)
+    blocks = min((rows + 31) // 32, 256)                       # 32 rows for each, as long as there are blocks
     assert ws.numel() >= 4 + blocks and int(ws[0]) == counted and int(ws[4: 4 + blocks].sum()) == counted
 
 
@@ -282,3 +282,34 @@ def test_route_softmax_scores_that_a_bias_brings_together(E, k):
     bias = torch.zeros(E, device="cuda")
     check_route(z, k, "softmax", bias)
     check_route(z, k, "softmax", 0.02 * randn(E, seed=11))
+
+
+@pytest.mark.parametrize("rows,keep", [(1, 33), (37, 64), (9000, 40), (300, 500)])
+def test_kl_topk_rows_whose_first_slots_do_not_count(rows, keep):
+    student, values, index, _ = rowwise.kl_inputs(rows, 600, keep, 43, "fp32", "fp32")
+    index[::2, : keep - 1] = -1                                # the last slot alone
+    index[1::7] = 600
+    values[3::5, :32] = float("-inf")
+    rowwise.check_kl(student, values, index, 1.0)
+
+
+def test_wide_layer_norm_in_a_captured_graph():
+    """Kernels on clusters, launched and measured for the first time while a graph is captured."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        x = randn(70, 24008, seed=44, dtype=torch.bfloat16).requires_grad_()
+        w, dy = randn(24008, seed=45).requires_grad_(), randn(70, 24008, seed=46, dtype=torch.bfloat16)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            y = K.layer_norm(x, w)
+            dx, dw = torch.autograd.grad(y, (x, w), dy)
+        for seed in (47, 48):
+            with torch.no_grad():
+                x.copy_(randn(70, 24008, seed=seed))
+            graph.replay()
+            other, weight = x.detach().clone().requires_grad_(), w.detach().clone().requires_grad_()
+            want = K.layer_norm(other, weight)
+            gx, gw = torch.autograd.grad(want, (other, weight), dy)
+            assert torch.equal(y, want) and torch.equal(dx, gx) and torch.equal(dw, gw)
+    torch.cuda.current_stream().wait_stream(side)
