@@ -78,24 +78,40 @@ __device__ __forceinline__ void choose_exactly(const RouteParams& p, const T* ro
     for (int o = LPT / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     if (sum == 0.0) sum = 1.0;
   }
+  auto biased = [&](int e) {                               // NaN is the largest
+    const double v = c[e] + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
+    return v != v ? CUDART_INF : v;
+  };
   if (p.bias != nullptr || p.groups > 1) {
 #pragma unroll 1
     for (int e = lane; e < p.E; e += LPT) {
       const double z = to_f32(row[e]);
-      const double v = (p.softmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z))) + (p.bias != nullptr ? static_cast<double>(p.bias[e]) : 0.0);
-      c[e] = v != v ? CUDART_INF : v;
+      c[e] = p.softmax ? exp(z - top) / sum : 1.0 / (1.0 + exp(-z));
     }
     __syncwarp();
   }
   if (p.groups > 1) {
     for (int n = lane; n < p.groups; n += LPT) {
-      double a = -CUDART_INF, b = -CUDART_INF;             // the two largest
+      double a = -CUDART_INF, b = -CUDART_INF;             // the two largest, and where they are
+      int at_a = n * p.gsize, at_b = p.gsize > 1 ? at_a + 1 : at_a;
       for (int e = n * p.gsize; e < (n + 1) * p.gsize; ++e) {
-        const double v = c[e];
-        b = fmax(b, fmin(a, v));
-        a = fmax(a, v);
+        const double v = biased(e);
+        if (v > a || e == n * p.gsize) {
+          b = a;
+          at_b = e == n * p.gsize ? at_b : at_a;
+          a = v;
+          at_a = e;
+        } else if (v > b || e == n * p.gsize + 1) {
+          b = v;
+          at_b = e;
+        }
       }
-      const double v = p.best > 1 && p.gsize > 1 ? a + b : a;
+      // scores and biases are added apart: groups with the same logits and the same biases in another order are equal
+      double v = a;
+      if (p.best > 1 && p.gsize > 1) {
+        v = c[at_a] + c[at_b];
+        if (p.bias != nullptr) v += static_cast<double>(p.bias[at_a]) + static_cast<double>(p.bias[at_b]);
+      }
       g[n] = v != v ? CUDART_INF : v;
     }
     __syncwarp();
@@ -113,7 +129,7 @@ __device__ __forceinline__ void choose_exactly(const RouteParams& p, const T* ro
   }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {                          // without a bias the order of the logits is the scores'
-    if (p.bias != nullptr && e0 + i < p.E) own[i] = c[e0 + i];
+    if (p.bias != nullptr && e0 + i < p.E) own[i] = biased(e0 + i);
     if (own[i] != own[i]) own[i] = CUDART_INF;
   }
   for (int j = 0; j < p.k; ++j) {
@@ -852,6 +868,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_bwd_kernel(const RouteGra
       w[n] = p.weights[token * p.k + j];
       dw[n] = p.dweights != nullptr ? p.dweights[token * p.k + j] : 0.f;
       if (!p.softmax) s[n] = sigmoid(to_f32(row[e[n]]));
+      if (p.renorm) w[n] = p.scale == 0.f ? 0.f : w[n] / p.scale;      // the share: of a single choice exactly 1
       dot += w[n] * dw[n];
     }
   }
@@ -861,7 +878,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_bwd_kernel(const RouteGra
 #pragma unroll
   for (int n = 0; n < PER; ++n) {
     // d w_j / d s_i = scale (delta_ij - s_j / S) / S and d s / d z = s (s (1 - s)): both leave a factor w_j
-    dz[n] = w[n] * (p.renorm ? (p.scale == 0.f ? 0.f : dw[n] - dot / p.scale) : dw[n]);
+    dz[n] = p.renorm ? p.scale * w[n] * (dw[n] - dot) : w[n] * dw[n];
     if (!p.softmax) dz[n] *= 1.f - s[n];
   }
   if (p.softmax && !p.renorm) flow = dot;

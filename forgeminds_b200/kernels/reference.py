@@ -189,6 +189,7 @@ def route_experts(logits, k: int, softmax: bool = True, bias=None, groups: int =
             pick = pick.masked_fill((z == float("-inf")).all(dim=-1, keepdim=True), 0.0)
         else:
             pick = torch.sigmoid(z)
+        score = pick
         pick = pick if bias is None else pick + bias.double()
         order = z if bias is None else pick           # without a bias the logits have the scores' order
         largest = lambda t: torch.nan_to_num(t, nan=float("inf"), posinf=float("inf"), neginf=float("-inf"))  # noqa: E731
@@ -196,7 +197,12 @@ def route_experts(logits, k: int, softmax: bool = True, bias=None, groups: int =
         shut = torch.zeros_like(order, dtype=torch.bool)
         if groups > 1:
             each = pick.view(N, groups, -1)
-            score = largest(each.sort(dim=-1, descending=True).values[..., :best].sum(dim=-1))
+            top = each.sort(dim=-1, descending=True, stable=True).indices[..., :best]
+            # scores and biases are added apart: the same ones in another order are equal
+            score = score.view_as(each).gather(-1, top).sum(dim=-1)
+            if bias is not None:
+                score = score + bias.double().view(1, groups, -1).expand_as(each).gather(-1, top).sum(dim=-1)
+            score = largest(score)
             out = score.sort(dim=-1, descending=True, stable=True).indices[:, top_groups:]
             shut = torch.zeros_like(score, dtype=torch.bool).scatter_(-1, out, True)
             shut = shut.unsqueeze(-1).expand_as(each).reshape(N, E)

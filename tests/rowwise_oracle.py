@@ -137,9 +137,14 @@ def route(logits, k, score, bias, groups, top_groups, best, renorm, scale, dw=No
     order = z.clone() if bias is None else c.clone()
     if groups > 1:
         size = E // groups
+        extra = torch.zeros(E, dtype=z.dtype, device=z.device) if bias is None else bias.double()
+        rows, scores, extra = c.tolist(), s.tolist(), extra.tolist()
         for t in range(N):
-            marks = [(-float(sorted((float(v) for v in c[t, g * size:(g + 1) * size]), reverse=True)[0] if best == 1 or size == 1 else
-                            sum(sorted((float(v) for v in c[t, g * size:(g + 1) * size]), reverse=True)[:2])), g) for g in range(groups)]
+            marks = []
+            for g in range(groups):
+                top = sorted(range(g * size, (g + 1) * size), key=lambda e: (-rows[t][e], e))[:best]
+                # scores and biases apart: the same ones in another order are equal, as they are in exact arithmetic
+                marks.append((-(sum(scores[t][e] for e in top) + sum(extra[e] for e in top)), g))
             for _, g in sorted(marks)[top_groups:]:
                 order[t, g * size:(g + 1) * size] = -float("inf")
     idx = torch.tensor([sorted(range(E), key=lambda e: (-o[e], e))[:k] for o in order.tolist()], dtype=torch.int64).reshape(N, k)

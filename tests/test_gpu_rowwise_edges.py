@@ -313,3 +313,20 @@ def test_wide_layer_norm_in_a_captured_graph():
             gx, gw = torch.autograd.grad(want, (other, weight), dy)
             assert torch.equal(y, want) and torch.equal(dx, gx) and torch.equal(dw, gw)
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_groups_that_differ_only_in_the_order_of_their_biases(score):
+    """The same two logits with the same two biases, exchanged: equal groups, of which the lower ones are kept."""
+    steps = (2 * randn(40, seed=12)).round() * 1e-3
+    for size, groups in ((2, 16), (7, 16), (13, 4), (32, 8)):
+        z = (randn(300, size * groups, seed=13)).round() / 2
+        bias = steps[torch.randint(0, 40, (size * groups,), device="cuda", generator=torch.Generator(device="cuda").manual_seed(14))]
+        z[::2] = z[::2, :size].repeat(1, groups)               # the same logits in every group
+        z[::4, :size] = z[::4, :size].flip(1)                  # and in another order
+        for dtype in (torch.float32, torch.bfloat16):
+            for b in (None, bias):
+                check_route(z.to(dtype), 2, score, b, groups, groups // 2)
+    leaf = randn(64, 16, seed=16).requires_grad_()
+    (g,) = torch.autograd.grad(K.route_experts(leaf, 1, scale=1.5)[0], leaf, randn(64, 1, seed=17))
+    assert not g.any()                                         # one renormalised choice has the weight 1, whatever its score
