@@ -485,7 +485,7 @@ def kl_topk_logits(student: torch.Tensor, teacher_values: torch.Tensor, teacher_
 
     ``p`` is the softmax of the kept ``teacher_values / temperature``; with ``teacher_lse`` (the logsumexp of ALL teacher
     logits over ``temperature``) it is their share of the whole distribution. The loss is not multiplied by
-    ``temperature^2``. The teacher is a constant. A slot whose index lies outside ``[0, V)`` (-1 for padding) or whose value
+    ``temperature^2`` (temperatures from 1e-20 to 1e20). The teacher is a constant. A slot whose index lies outside ``[0, V)`` (-1 for padding) or whose value
     is ``-inf`` does not count; a row without slots that count has neither loss nor gradient, and ``"mean"`` is over the
     other rows. An index that stands twice counts twice."""
     if reduction not in ("mean", "sum", "none"):
@@ -572,7 +572,7 @@ def route_experts(logits: torch.Tensor, k: int, *, score: str = "softmax", bias:
 
     Scores are ``softmax`` or ``sigmoid`` of the logits. Chosen are the ``k`` experts with the largest score plus ``bias``
     (``[experts]``, a constant that balances the load and does not enter the weights), in falling order, equal ones by
-    ascending number; the order is that of the exact scores. With ``n_groups`` > 1 (equal groups of neighbours) only the
+    ascending number; the order is that of the exact scores, as far as 64 bits tell them apart. With ``n_groups`` > 1 (equal groups of neighbours) only the
     ``top_groups`` groups with the largest sum of their ``group_best`` (1 or 2) largest biased scores are chosen from.
     Weights are the chosen scores, divided by their sum with ``renormalise``, times ``scale``. ``counts`` are the tokens each
     expert got. ``aux`` is ``aux_coef * E * sum_e load_e * mean(share_e) + z_coef * mean(logsumexp^2)`` with ``share`` the
