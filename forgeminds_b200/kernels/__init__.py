@@ -485,9 +485,9 @@ def kl_topk_logits(student: torch.Tensor, teacher_values: torch.Tensor, teacher_
 
     ``p`` is the softmax of the kept ``teacher_values / temperature``; with ``teacher_lse`` (the logsumexp of ALL teacher
     logits over ``temperature``) it is their share of the whole distribution. The loss is not multiplied by
-    ``temperature^2`` (temperatures from 1e-20 to 1e20). The teacher is a constant. A slot whose index lies outside ``[0, V)`` (-1 for padding) or whose value
-    is ``-inf`` does not count; a row without slots that count has neither loss nor gradient, and ``"mean"`` is over the
-    other rows. An index that stands twice counts twice."""
+    ``temperature^2`` (temperatures from 1e-20 to 1e20). The teacher is a constant. A slot whose index lies outside
+    ``[0, V)`` (-1 for padding) or whose value is ``-inf`` does not count; a row without slots that count has neither loss
+    nor gradient, and ``"mean"`` is over the other rows. An index that stands twice counts twice."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"reduction must be mean|sum|none, got {reduction!r}")
     if _kl_small(student, teacher_index) and fast_ok(student):
