@@ -7,7 +7,9 @@
 // A slot whose index is outside [0, V), or whose teacher logit is -inf, does not count; a row without slots that
 // count has no loss and no gradient. An index that stands twice in a row counts twice.
 // Bound by HBM bandwidth: one exponential per student logit and pass. Sums and statistics are fp32; exponentials are
-// 2^x of the special function unit (relative error 2^-22) with the argument folded into one multiply-add.
+// 2^x of the special function unit (relative error 2^-22). Their argument is a difference of logits, taken before it is
+// scaled: m / tau of a large logit, or of a small tau, is rounded to more than the exponent can bear, and of a mask of the
+// type's lowest value it overflows (folded into one multiply-add, x / tau - m / tau, such rows were NaN).
 #include "fmb_api.h"
 #include "launch.cuh"
 #include "ptx_sm100.cuh"
@@ -135,21 +137,25 @@ __device__ __forceinline__ float teacher_row(const KlParams& p, long long row, i
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
     const long long at = ti[k];
     const bool ok = slot_counts(at, tv[k], p.V);
-    const float t = to_f32(tv[k]) * inv_tau;
+    const float t = to_f32(tv[k]);
     s_at[k] = ok ? static_cast<int>(at) : -1;
     s_logp[k] = ok ? t : -CUDART_INF_F;
     if (ok) top = fmaxf(top, t);
   }
-  float base;
+  float base = 0.f;
   if (p.lse != nullptr) {
-    base = p.lse[row];
+    const float lse = p.lse[row];
+    for (int k = threadIdx.x; k < p.K; k += blockDim.x) s_logp[k] = fmaf(s_logp[k], inv_tau, -lse);
     __syncthreads();
   } else {
     top = block_max(top, scratch);
     if (top == -CUDART_INF_F) top = 0.f;                   // nothing counts (or NaN alone, which the sum carries on)
     float s = 0.f;
-    for (int k = threadIdx.x; k < p.K; k += blockDim.x) s += expf(s_logp[k] - top);
-    base = top + logf(block_sum(s, scratch));
+    for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
+      s_logp[k] = (s_logp[k] - top) * inv_tau;
+      s += expf(s_logp[k]);
+    }
+    base = logf(block_sum(s, scratch));
   }
   float mass = 0.f;
   for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
@@ -167,10 +173,10 @@ template <typename T> __device__ __forceinline__ int head_of(const T* p, int V) 
   return to < V ? to : V;
 }
 
-// The gradient of one row, `total` = sum of exponentials around `mc` = maximum * c.
+// The gradient of one row, `share` = sum p / sum of exponentials around `m`.
 template <typename T>
 __device__ __forceinline__ void write_gradient(const KlParams& p, const T* sr, T* gr, const int* s_at, const float* s_p, float c,
-                                               float mc, float share, float scale) {
+                                               float m, float share, float scale) {
   constexpr int N = Vec16<T>::N;
   const float a = share * scale;
   const int head = head_of(sr, p.V);
@@ -180,12 +186,12 @@ __device__ __forceinline__ void write_gradient(const KlParams& p, const T* sr, T
     float f[N];
     Vec16<T>::unpack(reinterpret_cast<const uint4*>(sr + head)[i], f);
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = exp2_unit(fmaf(f[j], c, -mc)) * a;
+    for (int j = 0; j < N; ++j) f[j] = exp2_unit((f[j] - m) * c) * a;
     reinterpret_cast<uint4*>(gr + head)[i] = Vec16<T>::pack(f);
   }
   if (wide)
-    for (int i = threadIdx.x; i < head; i += blockDim.x) gr[i] = from_f32<T>(exp2_unit(fmaf(to_f32(sr[i]), c, -mc)) * a);
-  for (int i = body + threadIdx.x; i < p.V; i += blockDim.x) gr[i] = from_f32<T>(exp2_unit(fmaf(to_f32(sr[i]), c, -mc)) * a);
+    for (int i = threadIdx.x; i < head; i += blockDim.x) gr[i] = from_f32<T>(exp2_unit((to_f32(sr[i]) - m) * c) * a);
+  for (int i = body + threadIdx.x; i < p.V; i += blockDim.x) gr[i] = from_f32<T>(exp2_unit((to_f32(sr[i]) - m) * c) * a);
 }
 
 template <typename T, typename TT, bool FWD>
@@ -230,7 +236,7 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
           ts *= tm == -CUDART_INF_F ? 0.f : exp2_unit((tm - top) * c);
           tm = top;
         }
-        ts += sum(tm == -CUDART_INF_F ? 0.f : tm * c);
+        ts += sum(tm == -CUDART_INF_F ? 0.f : tm);
       };
       for (int i = threadIdx.x; i < nv; i += blockDim.x) {
         float f[N];
@@ -238,16 +244,16 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
         float top = f[0];
 #pragma unroll
         for (int j = 1; j < N; ++j) top = fmaxf(top, f[j]);
-        add(top, [&](float mc) {
+        add(top, [&](float from) {
           float s = 0.f;
 #pragma unroll
-          for (int j = 0; j < N; ++j) s += exp2_unit(fmaf(f[j], c, -mc));
+          for (int j = 0; j < N; ++j) s += exp2_unit((f[j] - from) * c);
           return s;
         });
       }
       for (int i = threadIdx.x; i < p.V - nv * N; i += blockDim.x) {
         const float f = to_f32(sr[i < head ? i : i + nv * N]);
-        add(f, [&](float mc) { return exp2_unit(fmaf(f, c, -mc)); });
+        add(f, [&](float from) { return exp2_unit((f - from) * c); });
       }
       m = block_max(tm, scratch);
       total = block_sum(tm == -CUDART_INF_F ? ts : ts * exp2_unit((tm - m) * c), scratch);
@@ -270,16 +276,16 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
         if (s_at[k] >= 0) s_x[k] = to_f32(sr[s_at[k]]);
     }
     if (gr == nullptr) continue;
-    const float mc = m * c, share = mass / total, scale = per_row * up * inv_tau;
+    const float share = mass / total, scale = per_row * up * inv_tau;
     __syncthreads();                                       // all of the teacher's logits are read: gr may be sr itself
-    write_gradient<T>(p, sr, gr, s_at, s_p, c, mc, share, scale);
+    write_gradient<T>(p, sr, gr, s_at, s_p, c, m, share, scale);
     __syncthreads();
     // an index that stands more than once: each of its slots writes the same sum, taken in slot order
     for (int k = threadIdx.x; k < p.K; k += blockDim.x) {
       if (s_at[k] < 0) continue;
       float want = 0.f;
       for (int j = 0; j < p.K; ++j) want += s_at[j] == s_at[k] ? s_p[j] : 0.f;
-      gr[s_at[k]] = from_f32<T>((exp2_unit(fmaf(s_x[k], c, -mc)) * share - want) * scale);
+      gr[s_at[k]] = from_f32<T>((exp2_unit((s_x[k] - m) * c) * share - want) * scale);
     }
   }
   if constexpr (FWD) {
@@ -420,7 +426,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     const KlRow<T> r(static_cast<const T*>(p.student) + row * p.ld, p.V);
     const int n = held(r);
     const int at = slot_counts(slot_index, slot_value, p.V) ? static_cast<int>(slot_index) : -1;
-    const float t = at >= 0 ? to_f32(slot_value) * inv_tau : -CUDART_INF_F;
+    const float t = at >= 0 ? to_f32(slot_value) : -CUDART_INF_F;
     asm volatile("cp.async.wait_all;" ::: "memory");       // its own copies: other threads read them behind a barrier
     // one pass: exponentials of this thread's logits around `around`, which need not be their maximum, only within 2^8 of it
     float around = single;
@@ -434,9 +440,9 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
         more = f2_mul(more, f2(k, k));
         around = top;
         limit = top + slack;
-        less = f2(-top * c, -top * c);
+        less = f2(-top, -top);
       };
-      if (around != -CUDART_INF_F) less = f2(-around * c, -around * c);
+      if (around != -CUDART_INF_F) less = f2(-around, -around);
 #pragma unroll 2
       for (int i = threadIdx.x; i < n; i += THREADS) {
         const uint4 x = s_row[i];
@@ -451,7 +457,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
         if (!(top <= limit)) start(top);
 #pragma unroll
         for (int j = 0; j < H; ++j) {
-          const float2 o = (f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, less));
+          const float2 o = f2_mul(f2_add(f2(f[2 * j], f[2 * j + 1]), less), c2);
           if (j % 2) more = f2_add(more, f2(exp2_unit(o.x), exp2_unit(o.y)));
           else sums = f2_add(sums, f2(exp2_unit(o.x), exp2_unit(o.y)));
         }
@@ -468,13 +474,13 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
       m = lanes_max<WARPS>(o.x);
       ref = lanes_max<WARPS>(o.y);
     }
-    if (p.lse != nullptr) ref = lse;
-    else if (ref == -CUDART_INF_F) ref = 0.f;              // nothing counts, or NaN alone
+    if (ref == -CUDART_INF_F) ref = 0.f;                   // nothing counts, or NaN alone
+    const float logit = p.lse != nullptr ? fmaf(t, inv_tau, -lse) : (t - ref) * inv_tau;      // log of e below
     const KlRow<T> rn(static_cast<const T*>(p.student) + next * p.ld, p.V);
     const int nn = next < p.rows ? held(rn) : 0;
     float next_single = next < p.rows ? load_single(rn) : -CUDART_INF_F;
     load_slot(next);
-    // sums: exponentials of the student, e = exp(t - ref) of the teacher, and e (t - ref - x / tau) where x is held here
+    // sums: exponentials of the student, e of the teacher, and e (log e - x / tau) where x is held here
     float s = (sums.x + sums.y) * (around == -CUDART_INF_F ? 0.f : exp2_unit((around - m) * c)), e = 0.f, a = 0.f, xk = 0.f;
     bool mine = false, twice = false;                      // whether the student's logit at the index is held here
     int mark = -1;
@@ -487,8 +493,8 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
         mine = true;
         xk = to_f32(reinterpret_cast<const T*>(s_row)[w]);
       }
-      e = expf(t - ref);
-      if (mine && !(e == 0.f)) a = e * (t - ref - xk * inv_tau);
+      e = expf(logit);
+      if (mine && !(e == 0.f)) a = e * (logit - xk * inv_tau);
       // a mark that is set already: an index that stands twice, or in a few rows of a hundred two that share a mark
       const unsigned h = static_cast<unsigned>(at) * 2654435761u >> 17;
       mark = h >> 5;
@@ -540,21 +546,21 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     if (p.grad == nullptr) {
       for (int i = threadIdx.x; i < nn; i += THREADS) fetch(from, i);
     } else {
-      const float share = __fdividef(whole, s), gmc = m * c;
+      const float share = __fdividef(whole, s);
       T* gr = static_cast<T*>(p.grad) + row * p.ldg;
       T* to = gr + r.head + first * N;
       const bool wide = ((reinterpret_cast<uintptr_t>(r.at) ^ reinterpret_cast<uintptr_t>(gr)) & 15) == 0;
       if (rank == 0 && static_cast<int>(threadIdx.x) < p.V - r.nv * N)
-        gr[r.single(threadIdx.x)] = from_f32<T>(some ? exp2_unit(fmaf(single, c, -gmc)) * (share * scale) : 0.f);
+        gr[r.single(threadIdx.x)] = from_f32<T>(some ? exp2_unit((single - m) * c) * (share * scale) : 0.f);
       if (wide && some) {
-        const F2 gmc2 = f2(-gmc, -gmc), by2 = f2(share * scale, share * scale);
+        const F2 less = f2(-m, -m), by2 = f2(share * scale, share * scale);
 #pragma unroll 2
         for (int i = threadIdx.x; i < n; i += THREADS) {
           float f[N];
           Vec16<T>::unpack(s_row[i], f);
 #pragma unroll
           for (int j = 0; j < H; ++j) {
-            float2 o = (f2_fma(f2(f[2 * j], f[2 * j + 1]), c2, gmc2));
+            float2 o = f2_mul(f2_add(f2(f[2 * j], f[2 * j + 1]), less), c2);
             o = (f2_mul(f2(exp2_unit(o.x), exp2_unit(o.y)), by2));
             f[2 * j] = o.x;
             f[2 * j + 1] = o.y;
@@ -567,7 +573,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
           float f[N];
           Vec16<T>::unpack(s_row[i], f);
 #pragma unroll
-          for (int j = 0; j < N; ++j) to[i * N + j] = from_f32<T>(some ? exp2_unit(fmaf(f[j], c, -gmc)) * (share * scale) : 0.f);
+          for (int j = 0; j < N; ++j) to[i * N + j] = from_f32<T>(some ? exp2_unit((f[j] - m) * c) * (share * scale) : 0.f);
           if (i < nn) fetch(from, i);
         }
       }
@@ -582,7 +588,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
             want = 0.f;
             for (int j = 0; j < p.K; ++j) want += s_at[j] == at ? s_e[j] : 0.f;
           }
-          gr[at] = from_f32<T>((exp2_unit(fmaf(xk, c, -gmc)) * share - want * norm) * scale);
+          gr[at] = from_f32<T>((exp2_unit((xk - m) * c) * share - want * norm) * scale);
         }
       }
     }

@@ -1,0 +1,103 @@
+"""Row operators at the ends of their ranges: masks of the type's lowest value over whole vectors, threads and blocks,
+temperatures and offsets that scale every logit up, biases far from 0."""
+import pytest
+import torch
+
+import forgeminds_b200 as fm
+from rowwise_oracle import U32, within
+
+pytestmark = pytest.mark.gpu
+K = fm.kernels
+DT = {"bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def randn(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)).to(dtype)
+
+
+# ------------------------------------------------------------------------------ top-logit KL
+def kl_exact(student, values, index, tau):
+    """Row losses and gradients of their sum in 64 bits, with bounds that do not know how large the logits are, only how far
+    they lie from their row's largest one: fp32 arithmetic that takes this difference first is off by four units of the
+    exponent (difference, 1 / tau with its logarithm, product), 2^x by 2^-22, sums of V values in chains of V / 512.
+    A sum may be taken around a logit that is up to 8 in base 2 below the largest (6 in base e)."""
+    V, keep = student.shape[1], index.shape[1]
+    z, t = student.double(), values.double()
+    high, first = z.amax(1, keepdim=True), t.amax(1, keepdim=True)
+    x, tv = (z - high) / tau, (t - first) / tau
+    total, mass = x.exp().sum(1, keepdim=True), tv.exp().sum(1, keepdim=True)
+    q, p = x.exp() / total, tv.exp() / mass
+    logp, logq = tv - mass.log(), x.gather(1, index) - total.log()
+    row = torch.where(p > 0, p * (logp - logq), torch.zeros_like(p)).sum(1)
+    want = torch.zeros_like(q).scatter_add_(1, index, p)
+    span, tspan = x.abs().masked_fill(x == -float("inf"), 0.0), tv.abs()
+    rtotal = 2.0 ** -20 + U32 * (V / 512 + 64) + 8 * U32 * (q * (span + 6)).sum(1, keepdim=True)
+    rq = rtotal + 2.0 ** -22 + 8 * U32 * (span + 6)
+    rp = 2.0 ** -22 + U32 * (16 + keep) + 8 * U32 * (tspan + (p * tspan).sum(1, keepdim=True))
+    # (what 2^x gives below 2^-126 is 0)
+    off_grad = ((rq + U32 * 8) * q + torch.zeros_like(q).scatter_add_(1, index, (rp + 8 * U32) * p) + 2.0 ** -125) / tau
+    parts = rp * (logp - logq).abs() + 8 * U32 * (span.gather(1, index) + tspan + 6) + rtotal
+    parts = parts + (keep + 40) * U32 * (logp.abs() + logq.abs() + total.log().abs())
+    off_row = torch.where(p > 0, p * parts, torch.zeros_like(p)).sum(1)
+    return row, (q - want) / tau, off_row, off_grad
+
+
+def check_kl(student, values, index, tau, gradient_only=False):
+    """Loss and both gradients: the one that the forward pass leaves (an upstream gradient of 1) and the backward kernel's."""
+    row, grad, off_row, off_grad = kl_exact(student, values, index, tau)
+    s = student.detach().requires_grad_()
+    for up in (1.0, 0.5):
+        rows = K.kl_topk_logits(s, values, index, temperature=tau, reduction="none")
+        (g,) = torch.autograd.grad(rows, s, torch.full_like(rows, up))
+        assert within(g, grad * up, off_grad * up) <= 0
+        if not gradient_only:
+            assert within(rows.detach(), row, off_row) <= 0
+
+
+def kl_inputs(rows, V, keep, seed, dtype, lo=0, hi=None):
+    """Teacher logits are those of [lo, hi) alone."""
+    student = (randn(rows, V, seed=seed) * 2).to(DT[dtype])
+    values, index = (randn(rows, V, seed=seed + 1) * 2)[:, lo:hi].topk(keep, dim=-1)
+    return student, values.contiguous(), (index + lo).contiguous()
+
+
+MASKED = [  # rows, V, kept, masked range: tails, heads, a middle, whole blocks of rows that a cluster shares, all but one
+    (3, 1000, 16, 500, 700), (5, 1000, 16, 500, 1000), (5, 1000, 300, 500, 1000), (3, 1003, 8, 0, 640), (3, 40, 4, 8, 40),
+    (2100, 520, 9, 256, 520), (2, 128259, 64, 0, 64000), (2, 128259, 64, 70001, 128259), (2, 128259, 500, 9, 128000),
+    (40, 128259, 20, 40000, 128259), (2, 700001, 5, 8, 700001), (2, 900001, 5, 100, 800000)]
+
+
+@pytest.mark.parametrize("rows,V,keep,lo,hi", MASKED)
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("mask", ["lowest", "inf"])
+def test_kl_topk_ranges_of_masked_student_logits(rows, V, keep, lo, hi, dtype, mask):
+    """Whole vectors, whole threads and whole blocks of nothing but masked logits."""
+    open_lo, open_hi = (0, lo) if lo >= V - hi else (hi, V)
+    student, values, index = kl_inputs(rows, V, min(keep, open_hi - open_lo), 10, dtype, open_lo, open_hi)
+    student[:, lo:hi] = torch.finfo(DT[dtype]).min if mask == "lowest" else float("-inf")
+    for tau in (1.0, 0.5, 2.0):
+        check_kl(student, values, index, tau)
+
+
+@pytest.mark.parametrize("V,keep", [(1000, 4), (1000, 300), (128259, 4)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_kl_topk_gradient_of_a_row_of_equal_lowest_logits(V, keep, dtype):
+    student, values, index = kl_inputs(2, V, keep, 13, dtype)
+    student[0] = torch.finfo(DT[dtype]).min
+    check_kl(student, values, index, 1.0, gradient_only=True)
+
+
+@pytest.mark.parametrize("V,keep", [(1001, 9), (1001, 300), (128259, 9)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("tau", [1e-3, 1e-6, 1e-9, 1e-12, 1e-20, 1e4, 1e20])
+def test_kl_topk_gradient_at_any_temperature(V, keep, dtype, tau):
+    student, values, index = kl_inputs(3, V, keep, 16, dtype)
+    check_kl(student, values, index, tau, gradient_only=True)
+
+
+@pytest.mark.parametrize("V,keep", [(1001, 9), (1001, 300), (128259, 9)])
+@pytest.mark.parametrize("offset", [1e3, -1e4, 1e5])
+@pytest.mark.parametrize("tau", [1.0, 3.0])
+def test_kl_topk_gradient_of_logits_far_from_zero(V, keep, offset, tau):
+    student, values, index = kl_inputs(3, V, keep, 19, "fp32")
+    check_kl(student + offset, values, index, tau, gradient_only=True)
