@@ -318,8 +318,10 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
 // twice: 386), 4096 x 128259 over four CTAs in 456 us (4.6 TB/s; 758): there a row's CTAs wait for one another for a fifth
 // of the time. Both exponentials of a logit together hold the special function unit for 60 % of it, half of the issue slots
 // are used.
+// m: a logit near the maximum of the CTA's own; s: sum of exponentials around it; over the kept logits that are held here
+// a: sum e (log e - (x - m) / tau), w: sum e, which brings a to the row's m
 struct KlPart {
-  float m, s, a;                                           // logit near the maximum, sum of exponentials around it, sum e (log e - x / tau)
+  float m, s, a, w;
 };
 
 // A row of V values: `head` of them before the first 16-byte boundary, then nv whole vectors, then the rest. The up to
@@ -353,7 +355,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
   __shared__ float s_e[THREADS];
   __shared__ KlPart s_part[2][8];
   __shared__ float2 s_max[WARPS];
-  __shared__ float3 s_sum[WARPS];
+  __shared__ float4 s_sum[WARPS];
   __shared__ float scratch[32], s_single[2 * N];
   __shared__ int s_last;
   __shared__ int2 s_given[2];                              // rows that this CTA is told
@@ -480,21 +482,22 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     const int nn = next < p.rows ? held(rn) : 0;
     float next_single = next < p.rows ? load_single(rn) : -CUDART_INF_F;
     load_slot(next);
-    // sums: exponentials of the student, e of the teacher, and e (log e - x / tau) where x is held here
+    // sums: exponentials of the student, e of the teacher, and KlPart's a and w
+    const float base = m == -CUDART_INF_F ? 0.f : m;
     float s = (sums.x + sums.y) * (around == -CUDART_INF_F ? 0.f : exp2_unit((around - m) * c)), e = 0.f, a = 0.f, xk = 0.f;
     bool mine = false, twice = false;                      // whether the student's logit at the index is held here
     int mark = -1;
     if (at >= 0) {
-      const int v = at - r.head, w = v - first * N;
+      const int v = at - r.head, own = v - first * N;
       if (v < 0 || v >= r.nv * N) {
         mine = rank == 0;
         xk = s_single[v < 0 ? at : at - r.nv * N];
-      } else if (w >= 0 && w < per_cta * N) {
+      } else if (own >= 0 && own < per_cta * N) {
         mine = true;
-        xk = to_f32(reinterpret_cast<const T*>(s_row)[w]);
+        xk = to_f32(reinterpret_cast<const T*>(s_row)[own]);
       }
       e = expf(logit);
-      if (mine && !(e == 0.f)) a = e * (logit - xk * inv_tau);
+      if (mine && !(e == 0.f)) a = e * (logit - (xk - base) * inv_tau);
       // a mark that is set already: an index that stands twice, or in a few rows of a hundred two that share a mark
       const unsigned h = static_cast<unsigned>(at) * 2654435761u >> 17;
       mark = h >> 5;
@@ -507,15 +510,18 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
     s = lanes_sum<32>(s);
     float mass = lanes_sum<32>(e);
     a = lanes_sum<32>(a);
-    if (lane == 0) s_sum[warp] = make_float3(s, mass, a);
+    float w = 0.f;
+    if (split > 1) w = lanes_sum<32>(mine ? e : 0.f);
+    if (lane == 0) s_sum[warp] = make_float4(s, mass, a, w);
     if (rank == 0 && threadIdx.x == 0) give(side, next < p.rows ? after : static_cast<int>(p.rows), 0);
     twice = __syncthreads_or(twice);                       // also: every logit at an index has been taken from the row's copy
     if (mark >= 0) s_marks[mark] = 0;                      // the next row's first mark is behind another barrier
     {
-      const float3 o = s_sum[lane % WARPS];
+      const float4 o = s_sum[lane % WARPS];
       s = lanes_sum<WARPS>(o.x);
       mass = lanes_sum<WARPS>(o.y);
       a = lanes_sum<WARPS>(o.z);
+      if (split > 1) w = lanes_sum<WARPS>(o.w);
     }
     if (split > 1) {
       if (threadIdx.x < split) {                           // a copy of this CTA's part for each of the row's CTAs
@@ -523,6 +529,7 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(m) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(s) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 8), "f"(a) : "memory");
+        asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 12), "f"(w) : "memory");
       }
       cluster_arrive_after(warp == 0);
       cluster_wait();
@@ -532,14 +539,14 @@ kl_topk_row_kernel(const __grid_constant__ KlParams p, int split, int per_cta) {
       for (int i = 0; i < split; ++i) {
         const KlPart o = s_part[side][i];
         s += o.m == -CUDART_INF_F ? o.s : o.s * exp2_unit((o.m - m) * c);
-        a += o.a;
+        a += o.w == 0.f ? o.a : o.a + o.w * ((m - (o.m == -CUDART_INF_F ? 0.f : o.m)) * inv_tau);
       }
     }
     // p = e / sum e, or e itself beside the teacher's own normaliser
     const float norm = p.lse != nullptr || !some ? 1.f : __fdividef(1.f, mass);
     const float whole = p.lse != nullptr ? mass : 1.f;     // sum p
     if (rank == 0 && threadIdx.x == 0) {
-      p.row_loss[row] = some ? a * norm - (p.lse != nullptr ? 0.f : logf(mass)) + whole * (m * inv_tau + logf(s)) : 0.f;
+      p.row_loss[row] = some ? a * norm - (p.lse != nullptr ? 0.f : logf(mass)) + whole * logf(s) : 0.f;
       p.stats[row] = make_float2(m, s);
     }
     const uint4* from = rn.vectors() + first;

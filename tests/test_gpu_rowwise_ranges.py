@@ -101,3 +101,30 @@ def test_kl_topk_gradient_at_any_temperature(V, keep, dtype, tau):
 def test_kl_topk_gradient_of_logits_far_from_zero(V, keep, offset, tau):
     student, values, index = kl_inputs(3, V, keep, 19, "fp32")
     check_kl(student + offset, values, index, tau, gradient_only=True)
+
+
+@pytest.mark.parametrize("V,keep", [(1001, 9), (1001, 300), (128259, 9)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("tau", [1e-3, 1e-6, 1e-9, 1e-12, 1e-20, 1e4, 1e20])
+def test_kl_topk_loss_at_any_temperature(V, keep, dtype, tau):
+    student, values, index = kl_inputs(3, V, keep, 22, dtype)
+    check_kl(student, values, index, tau)
+
+
+@pytest.mark.parametrize("V,keep", [(1001, 9), (1001, 300), (128259, 9)])
+@pytest.mark.parametrize("offset,teacher_offset", [(1e3, 0), (-1e4, 1e4), (1e5, -1e5)])
+@pytest.mark.parametrize("tau", [1.0, 3.0])
+def test_kl_topk_loss_of_logits_far_from_zero(V, keep, offset, teacher_offset, tau):
+    """Adding a number to all of a row's logits, or to all of the teacher's, changes nothing but their own roundings."""
+    student, values, index = kl_inputs(3, V, keep, 25, "fp32")
+    check_kl(student + offset, values + teacher_offset, index, tau)
+
+
+@pytest.mark.parametrize("V,keep", [(1000, 4), (1000, 300), (128259, 4)])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_kl_topk_of_rows_of_equal_lowest_logits(V, keep, dtype):
+    student, values, index = kl_inputs(3, V, keep, 28, dtype)
+    student[0] = torch.finfo(DT[dtype]).min
+    values[1] = torch.finfo(torch.float32).min
+    for tau in (1.0, 0.5, 2.0):
+        check_kl(student, values, index, tau)
