@@ -165,12 +165,14 @@ def kl_topk(student, values, index, lse=None, temperature: float = 1.0):
     """Per-row ``sum_k p_k (log p_k - log q[index_k])`` (fp32, or fp64 for fp64 logits) of 2-D inputs."""
     held = kl_topk_counts(values, index, student.shape[-1])
     has = held.any(dim=-1, keepdim=True)
-    z = (_wide(student) / temperature).masked_fill(~has, 0.0)
-    t = (values.to(z.dtype) / temperature).masked_fill(~held, float("-inf"))
+    z = _wide(student)
+    # differences before they are scaled: a large logit over tau is rounded to more than the exponent can bear, or overflows
+    z = ((z - z.detach().amax(dim=-1, keepdim=True)) / temperature).masked_fill(~has, 0.0)
+    t = values.to(z.dtype).masked_fill(~held, float("-inf"))
     if lse is None:
-        logp = torch.log_softmax(t.masked_fill(~has, 0.0), dim=-1)
+        logp = torch.log_softmax(((t - t.amax(dim=-1, keepdim=True)) / temperature).masked_fill(~has, 0.0), dim=-1)
     else:
-        logp = t - lse.to(z.dtype).unsqueeze(-1)
+        logp = t / temperature - lse.to(z.dtype).unsqueeze(-1)
     p = logp.exp().masked_fill(~held, 0.0)
     logq = torch.log_softmax(z, dim=-1).gather(-1, index.masked_fill(~held, 0))
     return torch.where(held & (p != 0), p * (logp - logq), torch.zeros_like(p)).sum(dim=-1)
