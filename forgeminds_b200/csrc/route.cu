@@ -715,7 +715,7 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
     for (int e = threadIdx.x; e <= p.E; e += ROUTE_THREADS) s_acc[e] = 0.f;
   // the range of scores in fixed point: [0, 1] and what the finite biases add
   RouteScale scale = {0.f, 1.f, 0.f, 0, false, false};
-  float hi = 1.f, bias[VPL];
+  float range = 1.f, bias[VPL];
   if (me.biased) {
     float a = CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
@@ -729,15 +729,17 @@ __global__ void __launch_bounds__(ROUTE_THREADS, VPL > 8 ? 3 : 6) route_fwd_kern
     if (threadIdx.x % 32 == 0) { s_range[0][threadIdx.x / 32] = a; s_range[1][threadIdx.x / 32] = b; }
     __syncthreads();
     for (int w = 0; w < ROUTE_THREADS / 32; ++w) { a = fminf(a, s_range[0][w]); b = fmaxf(b, s_range[1][w]); }
-    if (a <= b) { scale.lo = a; hi = 1.f + b; }
+    if (a <= b) { scale.lo = a; range = (b - a) + 1.f; }      // ((1 + b) - a would lose a unit of b's, which may be anything)
     bool same = a == b;
 #pragma unroll
     for (int i = 0; i < VPL; ++i) same &= e0 + i >= p.E || bias[i] == a;
     scale.flat_bias = __all_sync(0xffffffffu, same);
   }
   __syncthreads();
-  // steps per score, so few less that no rounding goes past the last one; what the bias adds to the fixed point
-  scale.unit = static_cast<float>(FIXED - 16) / (hi - scale.lo);
+  // Steps per score, so few less that no rounding goes past the last one: the range is off by two units of 2^-24 of itself,
+  // the quotient and a bias without the lowest by one each (two steps in all), a score may be 2^-21 above 1 (four), and two
+  // additions round to a step (one): seven at the most. And what the bias adds to the fixed point.
+  scale.unit = static_cast<float>(FIXED - 16) / range;
   load_bias<VPL>(p, e0, scale, bias);
   // How far a score may be from the exact one. Sigmoid: s (1 - s) <= 1/4 of the error of e^-z (2^-22, and its argument's
   // rounding, 3.3e-7 at |z| = 5.5 and less in s beyond), 1.8e-7 from addition and reciprocal: 3.4e-7. Softmax, divided by a

@@ -128,3 +128,32 @@ def test_kl_topk_of_rows_of_equal_lowest_logits(V, keep, dtype):
     values[1] = torch.finfo(torch.float32).min
     for tau in (1.0, 0.5, 2.0):
         check_kl(student, values, index, tau)
+
+
+# ------------------------------------------------------------------------------ routing
+def check_choice(logits, k, bias, **options):
+    """The choice is the 64-bit statement's."""
+    _, idx, counts, _ = K.route_experts(logits, k, bias=bias, **options)
+    from forgeminds_b200.kernels import reference
+    softmax = options.get("score", "softmax") == "softmax"
+    _, want, want_counts, _ = reference.route_experts(logits, k, softmax, bias, options.get("n_groups", 1), options.get("top_groups", 1))
+    assert torch.equal(idx, want) and torch.equal(counts, want_counts)
+
+
+@pytest.mark.parametrize("E,k,groups", [(8, 2, 1), (64, 6, 8), (60, 6, 4), (256, 8, 8), (256, 8, 1), (512, 4, 1)])
+@pytest.mark.parametrize("near", [3.5, 31.5, 63.5, 127.5, 255.5, 2e4, -63.5])
+def test_route_with_biases_far_from_zero(E, k, groups, near):
+    """One bias for all experts, a unit or more beyond ``near``, and biases spread over less than 1: whatever is added to
+    them in 32 bits crosses a power of two. Scores reach 1."""
+    logits = randn(300, E, seed=40) * 2
+    at = torch.arange(300, device="cuda")
+    logits[at, at * 7 % E] = 40.0                            # sigmoid 1, softmax 1
+    logits[at[::3], at[::3] * 5 % E] = 14.0                  # sigmoid 1 - 8e-7
+    base = torch.tensor(near, dtype=torch.float32, device="cuda")
+    for units in (0, 1, 3, 2 ** 12):
+        bias = (base.view(torch.int32) + units).view(torch.float32).repeat(E)
+        for score in ("sigmoid", "softmax"):
+            check_choice(logits, k, bias, score=score, n_groups=groups, top_groups=max(1, groups // 2))
+            check_choice(logits.bfloat16(), k, bias, score=score, n_groups=groups, top_groups=max(1, groups // 2))
+            spread = bias + randn(E, seed=41 + units) * 0.1
+            check_choice(logits, k, spread, score=score, n_groups=groups, top_groups=max(1, groups // 2))
