@@ -365,7 +365,10 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
 // sums of the next row, so three rows are in the ring, one of them on its way. bf16, no dres: 3024 x 12088 in 79 us (launched
 // while the previous kernel still ran 114; one block per row that reads it twice, and the columns once more, 160), 4096 x
 // 16384 in 113. 8192 x 8192, which 512 threads hold, takes 95 there and 111 on clusters of two.
-constexpr int CLUSTER_STAGES = 3;
+// A block's sums lie in one of three slots of each peer. A peer writes a slot again three rows later, and by then the reads of
+// the slot are ordered before it: they stand before the __syncthreads of the next row's own sums, and so before the fence and
+// the arrival that warp 0 makes behind that. With two slots only a relaxed arrival of the reading warps stood in between.
+constexpr int CLUSTER_STAGES = 3, CLUSTER_SLOTS = 3;
 template <typename T, typename WT, bool VEC>
 __global__ void __launch_bounds__(256, 2)
 layernorm_bwd_cluster_kernel(const T* __restrict__ dy, long long ldy, const T* __restrict__ x, long long ldx, const WT* __restrict__ w,
@@ -373,7 +376,7 @@ layernorm_bwd_cluster_kernel(const T* __restrict__ dy, long long ldy, const T* _
                              float* __restrict__ partial, long long rows, const int whole, float inv_d, const int split, const int width) {
   using M = RowMap<T, 256, VEC>;
   constexpr int N = M::N, H = N / 2, VPL = 2;
-  __shared__ float2 scratch[2][8], s_peers[2][8];
+  __shared__ float2 scratch[2][8], s_peers[CLUSTER_SLOTS][8];
   extern __shared__ uint4 s_ring[];                       // [stage][dy, x, dres][chunk][thread]
   pdl_wait();
   pdl_launch_dependents();
@@ -435,6 +438,7 @@ layernorm_bwd_cluster_kernel(const T* __restrict__ dy, long long ldy, const T* _
   }
   cluster_sync_all();                                     // every block of the row runs before one writes to another
   int turn = 0, here = 0, before = 0;                     // bytes of this row's and the last one's place in the ring
+  int slot = 0, slot_before = 0;                          // of this row's and the last one's sums
   float2 st = stats[min(group, n_rows - 1)], st_before = st;
   // one step beyond the last row, for its result
   for (int row = group; row < n_rows + step; row += step) {
@@ -466,14 +470,14 @@ layernorm_bwd_cluster_kernel(const T* __restrict__ dy, long long ldy, const T* _
     if (had) {
       cluster_wait();
       for (int i = 0; i < split; ++i) {
-        const float2 o = s_peers[turn ^ 1][i];
+        const float2 o = s_peers[slot_before][i];
         whole_sums.x += o.x;
         whole_sums.y += o.y;
       }
     }
     if (more) {
       if (t < split) {
-        const uint32_t to = mapa_shared(smem_at(&s_peers[turn][rank]), t);
+        const uint32_t to = mapa_shared(smem_at(&s_peers[slot][rank]), t);
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(sums.x) : "memory");
         asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4), "f"(sums.y) : "memory");
       }
@@ -506,6 +510,8 @@ layernorm_bwd_cluster_kernel(const T* __restrict__ dy, long long ldy, const T* _
     before = here;
     here = here == (CLUSTER_STAGES - 1) * row_bytes ? 0 : here + row_bytes;
     turn ^= 1;
+    slot_before = slot;
+    slot = slot == CLUSTER_SLOTS - 1 ? 0 : slot + 1;
     st_before = st;
     st = next_st;
   }

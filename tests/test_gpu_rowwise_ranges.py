@@ -157,3 +157,17 @@ def test_route_with_biases_far_from_zero(E, k, groups, near):
             check_choice(logits.bfloat16(), k, bias, score=score, n_groups=groups, top_groups=max(1, groups // 2))
             spread = bias + randn(E, seed=41 + units) * 0.1
             check_choice(logits, k, spread, score=score, n_groups=groups, top_groups=max(1, groups // 2))
+
+
+# ------------------------------------------------------------------------------ LayerNorm on clusters
+@pytest.mark.parametrize("rows,d,dtype", [(700, 8200, "bf16"), (300, 16384, "bf16"), (301, 16384, "fp32"), (500, 4100, "fp32"), (3, 32768, "bf16")])
+def test_layer_norm_wide_backward_is_the_same_every_time(rows, d, dtype):
+    """Several rows for each cluster, whose blocks exchange their sums row by row."""
+    x, dy, ds = (randn(rows, d, seed=50 + i, dtype=DT[dtype]) for i in range(3))
+    w, b = 1 + 0.1 * randn(d, seed=53), randn(d, seed=54)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    total, y = K.add_layer_norm(x, torch.zeros_like(x), w, b)
+    first = torch.autograd.grad((total, y), leaves, (ds, dy), retain_graph=True)
+    for _ in range(20):
+        again = torch.autograd.grad((total, y), leaves, (ds, dy), retain_graph=True)
+        assert all(torch.equal(p, q) for p, q in zip(first, again))

@@ -39,3 +39,66 @@ def test_kl_topk_takes_differences_first(offset, tau):
     # exponents are spans over tau, each off by a few units of its own size; the loss is of the size of the spans
     assert torch.allclose(rows.detach().double(), want, rtol=100 * 2.0 ** -24, atol=200 * 2.0 ** -24)
     assert torch.allclose(grad.double() * tau, wgrad * tau, rtol=1e-4, atol=1e-6)
+
+
+# ------------------------------------------------------------------------------ sums that the blocks of a cluster exchange
+def _unordered(slots, rows=8, ctas=2, warps=2):
+    """Accesses of an exchange slot that the memory model leaves unordered, in the order of events of LayerNorm's backward
+    kernel on clusters: per row the __syncthreads of the row's sums, the wait for the last row's exchange, reads of its slot,
+    warp 0's writes to the peers' slots, its fence, the arrival. Warp 0's fence and arrival are ordered before a wait; the
+    other warps' relaxed arrivals order nothing."""
+    before = {}                                              # event -> events that happen before it, directly
+
+    def event(name, *after):
+        before.setdefault(name, set()).update(after)
+        return name
+
+    last = {}
+    for i in range(rows + 1):
+        more, had = i < rows, i > 0
+        for c in range(ctas):
+            if more:                                         # what stands before a __syncthreads is before what follows in any warp
+                event(("sync", c, i), *[last[c, w] for w in range(warps) if (c, w) in last])
+                for w in range(warps):
+                    last[c, w] = ("sync", c, i)
+        for c in range(ctas):
+            for w in range(warps):
+                def then(name, *after):
+                    last[c, w] = event(name, *after, *([last[c, w]] if (c, w) in last else []))
+                if had:
+                    then(("wait", c, w, i - 1), *[("fence", o, i - 1) for o in range(ctas)])
+                    then(("read", c, w, i - 1))
+                if more and w == 0:
+                    for o in range(ctas):
+                        then(("write", c, o, i))
+                    then(("fence", c, i))
+    reach = {}
+
+    def past(e):                                             # everything that happens before e
+        if e not in reach:
+            reach[e] = set()
+            for b in before.get(e, ()):
+                reach[e] |= {b} | past(b)
+        return reach[e]
+
+    bad = set()
+    for i in range(rows):
+        for c in range(ctas):
+            for o in range(ctas):
+                for w in range(warps):
+                    read, write = ("read", o, w, i), ("write", c, o, i)
+                    if write not in past(read):
+                        bad.add((write, read))
+                    if i + slots < rows and read not in past(("write", c, o, i + slots)):
+                        bad.add((read, ("write", c, o, i + slots)))
+    return bad
+
+
+def test_the_exchange_of_wide_layer_norm_rows_is_ordered():
+    import re
+    from pathlib import Path
+    source = (Path(fm.__file__).parent / "csrc" / "layernorm.cu").read_text()
+    found = re.search(r"s_peers\[(\w+)\]\[8\];", source).group(1)
+    slots = int(found) if found.isdigit() else int(re.search(rf"{found} = (\d+);", source).group(1))
+    assert not _unordered(slots)
+    assert _unordered(1) and _unordered(2) and not _unordered(4)
