@@ -33,7 +33,10 @@ def _looks_like_swiglu(m: nn.Module) -> bool:
 
 
 def _is_layer_norm(m: nn.Module) -> bool:
-    return isinstance(m, nn.LayerNorm) and len(m.normalized_shape) == 1
+    """A LayerNorm of one dimension that computes what ``nn.LayerNorm.forward`` does: a subclass or an instance with a forward
+    of its own (channels first, casts, scales) is another operator."""
+    return isinstance(m, nn.LayerNorm) and len(m.normalized_shape) == 1 and type(m).forward is nn.LayerNorm.forward \
+        and "forward" not in vars(m)
 
 
 def _eps_of(m: nn.Module, x: torch.Tensor) -> float:
@@ -130,7 +133,7 @@ def patch(module: nn.Module, split: bool = False, kind: "str | None" = None) -> 
 def enable(model: nn.Module, norm: bool = True, swiglu_mlp: bool = True, split: bool = False,
            layer_norm: bool = False) -> nn.Module:
     """Patch every recognised norm / gated MLP under ``model``, and with ``layer_norm`` every ``torch.nn.LayerNorm`` of one
-    dimension; counts land on ``model._fm_fused``."""
+    dimension that has no forward of its own; counts land on ``model._fm_fused``."""
     counts = {"norm": 0, "mlp": 0}
     if layer_norm:
         counts["layer_norm"] = 0

@@ -102,3 +102,31 @@ def test_the_exchange_of_wide_layer_norm_rows_is_ordered():
     slots = int(found) if found.isdigit() else int(re.search(rf"{found} = (\d+);", source).group(1))
     assert not _unordered(slots)
     assert _unordered(1) and _unordered(2) and not _unordered(4)
+
+
+# ------------------------------------------------------------------------------ modules
+class _ChannelsFirst(torch.nn.LayerNorm):
+    def forward(self, x):
+        return super().forward(x.movedim(1, -1)).movedim(-1, 1)
+
+
+class _Renamed(torch.nn.LayerNorm):
+    """No forward of its own."""
+
+
+def test_layer_norms_with_a_forward_of_their_own_are_left_alone():
+    own, plain, renamed, by_hand = _ChannelsFirst(6), torch.nn.LayerNorm(6), _Renamed(6), torch.nn.LayerNorm(6)
+    by_hand.forward = lambda x: 2 * torch.nn.LayerNorm.forward(by_hand, x)
+    model = torch.nn.ModuleList([own, plain, renamed, by_hand])
+    x = _randn(2, 6, 6, 6, seed=5)
+    want = [m(x) for m in model]
+    K.enable(model, layer_norm=True)
+    assert model._fm_fused["layer_norm"] == 2
+    for m, y in zip(model, want):
+        assert torch.allclose(m(x), y, atol=1e-5)
+    for m in (own, by_hand):
+        with pytest.raises(TypeError, match="layer_norm"):
+            K.patch(m, kind="layer_norm")
+        assert not getattr(m, "_fm_norm", False)
+    K.revert(model)
+    assert torch.equal(plain(x), want[1])
