@@ -18,15 +18,16 @@ F32 = torch.float32
 
 class _LinearKLTopK(torch.autograd.Function):
     """Mean top-logit KL of ``h @ W.T`` without fp32 logits: each chunk of bf16 logits becomes its gradient in place;
-    the two gradient products run once in the backward pass, scaled by the incoming gradient on the device."""
+    the two gradient products run once in the backward pass, scaled by the incoming gradient on the device. ``need``:
+    whether there will be one (``ctx.needs_input_grad`` says so of a Parameter under ``no_grad`` too); all ``n`` rows are
+    held until then, and ``chunk`` of them otherwise."""
 
     @staticmethod
-    def forward(ctx, h, weight, values, index, lse, tau, count, chunk):
+    def forward(ctx, h, weight, values, index, lse, tau, count, chunk, need):
         C = require()
         w = bf16_of(weight)
         h2 = h.reshape(-1, h.shape[-1]).contiguous()
         n, V = h2.shape[0], w.shape[0]
-        need = any(ctx.needs_input_grad[:2])
         logits = torch.empty((n if need else min(n, chunk), V), dtype=BF16, device=h.device)
         parts = []
         for lo in range(0, n, chunk):
@@ -55,9 +56,10 @@ class _LinearKLTopK(torch.autograd.Function):
             else:
                 dw = gemm(dlogits, h2, a_mn=True, b_mn=True, out_dtype=F32, alpha_dev=g32, allow_split=True)
                 dw = dw if dw.dtype == weight.dtype else dw.to(weight.dtype)
-        return dh, dw, None, None, None, None, None, None
+        return dh, dw, None, None, None, None, None, None, None
 
 
 def linear_kl_topk(h, weight, values, index, lse, tau, count, chunk):
     """``h`` bf16 ``[.., d]``, ``weight [V, d]``; ``count`` (device int32 ``[1]``): the rows that the mean is over."""
-    return _LinearKLTopK.apply(h, weight, values, index, lse, tau, count, chunk)
+    need = torch.is_grad_enabled() and (h.requires_grad or weight.requires_grad)
+    return _LinearKLTopK.apply(h, weight, values, index, lse, tau, count, chunk, need)
