@@ -8,6 +8,7 @@
 // which 50 are what autograd takes for any function).
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -269,11 +270,16 @@ Tensor route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& idx,
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The kernels carry no tangents of forward mode: a dual number is refused, whether or not it requires a gradient too.
+bool has_tangent(const Tensor& t) { return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined(); }
 bool wants_grad(std::initializer_list<const Tensor*> tensors) {
-  if (!at::GradMode::is_enabled()) return false;
-  for (const Tensor* t : tensors)
-    if (t != nullptr && t->defined() && t->requires_grad()) return true;
-  return false;
+  bool any = false;
+  for (const Tensor* t : tensors) {
+    if (t == nullptr || !t->defined()) continue;
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(*t), "forgeminds_b200: this operator has no derivative in forward mode");
+    any |= t->requires_grad();
+  }
+  return any && at::GradMode::is_enabled();
 }
 const Tensor* opt(const OptTensor& t) { return given(t) ? &*t : nullptr; }
 Tensor detached(const OptTensor& t) { return given(t) ? t->detach() : Tensor(); }
@@ -415,7 +421,8 @@ RotaryTables rotary_args(const char* op, const Tensor& q, const OptTensor& k, Te
            " differ in more than their heads");
   refuse(cos.device() != q.device() || sin.device() != q.device() || (given(positions) && positions->device() != q.device()), op,
          ": q is on ", q.device(), ", its tables or positions are not");
-  refuse(cos.requires_grad() || sin.requires_grad(), op, ": the tables are constants, but one of them requires a gradient");
+  refuse(cos.requires_grad() || sin.requires_grad() || has_tangent(cos) || has_tangent(sin), op,
+         ": the tables are constants, but one of them requires a gradient or carries a tangent");
   if (cos.dim() == 4 && cos.size(0) == 1 && cos.size(2) == 1) {
     cos = cos.select(0, 0).select(1, 0);
     if (sin.dim() == 4) sin = sin.reshape({sin.size(1), sin.size(3)});
