@@ -95,14 +95,19 @@ class Router(nn.Module):
 
     @torch.no_grad()
     def rebalance(self, rate: float, group=None) -> None:
-        """``bias += rate * sign(mean load - load)`` by the last forward pass's counts, summed over the ranks of ``group``
-        when it is given: experts with less than their share become easier to choose."""
+        """``bias += rate * sign(mean load - load)`` by the last forward pass's counts, summed over the ranks of ``group``:
+        experts with less than their share become easier to choose. The ranks that hold copies of a router have to move them
+        alike, so in a run of several ranks ``group`` has to be given: the data-parallel group, or ``"self"`` for a router
+        that no other rank has a copy of."""
         if self.bias is None:
             raise RuntimeError("rebalance needs a router with balance_bias=True")
         if self.last_counts is None:
             raise RuntimeError("rebalance needs the counts of a forward pass")
+        if group is None and dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1:
+            raise ValueError("rebalance in a run of several ranks needs the group whose ranks hold copies of this router "
+                             "(ctx.dp_group), or group=\"self\": by its own counts each copy would move away from the others")
         load = self.last_counts.float()
-        if group is not None:
+        if group is not None and group != "self":
             dist.all_reduce(load, group=group)
         self.bias += (rate * torch.sign(load.mean() - load)).to(self.bias.dtype)
 

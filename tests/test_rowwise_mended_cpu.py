@@ -130,3 +130,31 @@ def test_layer_norms_with_a_forward_of_their_own_are_left_alone():
         assert not getattr(m, "_fm_norm", False)
     K.revert(model)
     assert torch.equal(plain(x), want[1])
+
+
+def _rebalance_rank(rank, path):
+    import torch.distributed as dist
+    torch.set_num_threads(1)
+    dist.init_process_group("gloo", init_method=f"file://{path}", rank=rank, world_size=2)
+    try:
+        torch.manual_seed(8)
+        moe = fm.MoE(16, 32, 4, 1, score="sigmoid", balance_bias=True)
+        with torch.no_grad():
+            moe(_randn(50 + 30 * rank, 16, seed=60 + rank).abs())
+        router, own = moe.router, moe.router.last_counts.float()
+        with pytest.raises(ValueError, match="several ranks"):
+            router.rebalance(0.1)
+        assert not router.bias.any()
+        router.rebalance(0.1, dist.group.WORLD)
+        total = own.clone()
+        dist.all_reduce(total)
+        assert torch.allclose(router.bias, 0.1 * torch.sign(total.mean() - total))
+        router.bias.zero_()
+        router.rebalance(0.1, "self")
+        assert torch.allclose(router.bias, 0.1 * torch.sign(own.mean() - own))
+    finally:
+        dist.destroy_process_group()
+
+
+def test_rebalance_of_several_ranks_needs_a_group(tmp_path):
+    torch.multiprocessing.spawn(_rebalance_rank, args=(str(tmp_path / "store"),), nprocs=2)
