@@ -225,8 +225,8 @@ std::vector<Tensor> route_fwd(const Tensor& logits, const OptTensor& bias, int64
                               double z_coef) {
   rows_of(logits, "logits");
   const int64_t N = logits.size(0), E = logits.size(1);
-  TORCH_CHECK(E <= FMB_ROUTE_MAX_EXPERTS && k <= FMB_ROUTE_MAX_K && groups <= 32, "route: at most ", FMB_ROUTE_MAX_EXPERTS,
-              " experts, ", FMB_ROUTE_MAX_K, " of them, 32 groups");
+  TORCH_CHECK(E <= FMB_ROUTE_MAX_EXPERTS && k <= FMB_ROUTE_MAX_K && groups <= FMB_ROUTE_MAX_GROUPS, "route: at most ",
+              FMB_ROUTE_MAX_EXPERTS, " experts, ", FMB_ROUTE_MAX_K, " of them, ", FMB_ROUTE_MAX_GROUPS, " groups");
   if (given(bias)) beside(*bias, logits, E, at::kFloat, "bias");
   c10::cuda::CUDAGuard guard(logits.device());
   auto f32 = logits.options().dtype(at::kFloat);

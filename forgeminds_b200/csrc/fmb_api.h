@@ -105,6 +105,7 @@ int fmb_kl_topk_bwd(const void* student, long long ld, const void* values, const
 // ---- routing to experts (route.cu)
 #define FMB_ROUTE_MAX_EXPERTS 512
 #define FMB_ROUTE_MAX_K 32
+#define FMB_ROUTE_MAX_GROUPS 32
 // counts [E] is cleared and filled; partial ([blocks, E + 1] fp32) and aux are given together, or neither is.
 int fmb_route_blocks(long long tokens, int E);
 int fmb_route_fwd(const void* logits, long long ld, int dtype, const float* bias, float* weights, int* idx, int* counts,

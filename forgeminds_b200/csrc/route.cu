@@ -970,7 +970,11 @@ __global__ void __launch_bounds__(ROUTE_THREADS) route_bwd_kernel(const RouteGra
 template <typename T, int LPT, int VPL>
 int route_fwd_run(RouteParams p, int blocks, cudaStream_t stream) {
   constexpr int TPB = ROUTE_THREADS / LPT, BYTES = VPL * sizeof(T) < 16 ? VPL * sizeof(T) : 16;
-  // at most 8 (64 + 32) or 4 (512 + 32) values of 64 bits and two arrays of 512: with the static ones below 48 KB
+  // values of 64 bits of the block's 16, 8 or 4 tokens, counts and sums: with the kernel's static arrays (keys and choices of
+  // each token, ranges) no opt-in is needed
+  constexpr int MOST_E = LPT * VPL, MOST_K = MOST_E < FMB_ROUTE_MAX_K ? MOST_E : FMB_ROUTE_MAX_K;
+  static_assert(sizeof(double) * TPB * (MOST_E + FMB_ROUTE_MAX_GROUPS) + sizeof(int) * (2 * MOST_E + 1) +
+                sizeof(int) * TPB * (2 * MOST_K + 2) + sizeof(float) * ROUTE_THREADS / 16 <= 48 * 1024, "beyond 48 KB a kernel has to opt in");
   const size_t smem = sizeof(double) * TPB * (p.E + p.groups) + sizeof(int) * (2 * p.E + 1);
   p.vec = p.E % VPL == 0 && p.ld % VPL == 0 && reinterpret_cast<uintptr_t>(p.logits) % BYTES == 0;
   auto kernel = p.partial != nullptr ? route_fwd_kernel<T, LPT, VPL, true> : route_fwd_kernel<T, LPT, VPL, false>;
@@ -1024,7 +1028,7 @@ extern "C" int fmb_route_fwd(const void* logits, long long ld, int dtype, const 
                              int* counts, float* partial, float* aux, long long tokens, int E, int k, int softmax, int groups,
                              int top_groups, int best, int renorm, float scale, float aux_coef, float z_coef, int blocks,
                              cudaStream_t stream) {
-  if (E < 1 || E > FMB_ROUTE_MAX_EXPERTS || k < 1 || k > FMB_ROUTE_MAX_K || k > E || groups < 1 || groups > 32 || E % groups ||
+  if (E < 1 || E > FMB_ROUTE_MAX_EXPERTS || k < 1 || k > FMB_ROUTE_MAX_K || k > E || groups < 1 || groups > FMB_ROUTE_MAX_GROUPS || E % groups ||
       top_groups < 1 || top_groups > groups || k > E / groups * top_groups || best < 1 || best > 2 || blocks < 1)
     return -2;
   if (cudaMemsetAsync(counts, 0, E * sizeof(int), stream) != cudaSuccess) return -3;
