@@ -41,7 +41,19 @@ template <typename... P> void refuse(bool when, const P&... parts) {
   if (when) throw pybind11::value_error(c10::str(parts...));
 }
 
+// The kernels read memory by pointers: what a tensor says of itself has to be what lies there. A wrapper (DTensor, whose
+// pointer is null, vmap's and torch.func's tensors), a sparse one and a view that is negated lazily are refused.
+void plain(const char* op, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    if (t != nullptr && t->defined() &&
+        (t->layout() != at::kStrided || t->unsafeGetTensorImpl()->is_python_dispatch() || !t->has_storage() || t->is_neg() ||
+         t->_is_zerotensor()))
+      throw pybind11::type_error(c10::str(op, ": the sm_100a kernels take plain strided tensors, not wrappers (DTensor, vmap), sparse "
+                                              "tensors or lazily negated views"));
+}
+
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+const Tensor* opt(const OptTensor& t) { return given(t) ? &*t : nullptr; }
 const void* ptr(const OptTensor& t) { return given(t) ? t->data_ptr() : nullptr; }
 
 // a tensor that a kernel reads next to `like`: on its device, with `n` values in one piece
@@ -177,6 +189,7 @@ void kl_check(const Tensor& student, const Tensor& values, const Tensor& index, 
 // here). in_place: the gradient takes the student's place.
 std::vector<Tensor> kl_topk_fwd(const Tensor& student, const Tensor& values, const Tensor& index, const OptTensor& lse, double tau,
                                 bool total, bool mean, const OptTensor& count, bool need_grad, bool in_place) {
+  plain("kl_topk", {&student, &values, &index, opt(lse), opt(count)});
   kl_check(student, values, index, lse);
   const int64_t rows = student.size(0), V = student.size(1), K = index.size(1);
   if (given(count)) TORCH_CHECK(count->device() == student.device() && count->scalar_type() == at::kInt && count->numel() >= 1,
@@ -281,9 +294,15 @@ bool wants_grad(std::initializer_list<const Tensor*> tensors) {
   }
   return any && at::GradMode::is_enabled();
 }
-const Tensor* opt(const OptTensor& t) { return given(t) ? &*t : nullptr; }
 Tensor detached(const OptTensor& t) { return given(t) ? t->detach() : Tensor(); }
 OptTensor as_opt(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+// an incoming gradient as memory: a lazily negated view or a tensor of zeros that has none is written out
+Tensor solid(const char* op, const Tensor& g) {
+  if (!g.defined()) return g;
+  const Tensor t = g._is_zerotensor() ? at::zeros(g.sizes(), g.options()) : g.resolve_neg();
+  plain(op, {&t});
+  return t;
+}
 bool capturing() { return c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None; }
 
 // The kernels' gradients are not differentiable themselves: with create_graph a second derivative raises, it is not dropped.
@@ -321,6 +340,7 @@ std::pair<OptTensor, OptTensor> gain(const Tensor& x, const OptTensor& w, const 
 Tensor shaped(const Tensor& t, const Tensor& like) { return like.dim() == 2 ? t : t.view(like.sizes()); }
 
 void check_norm(const char* op, const Tensor& x, const OptTensor& delta, const OptTensor& w, const OptTensor& b) {
+  plain(op, {&x, opt(delta), opt(w), opt(b)});
   refuse(x.dim() < 1 || x.size(-1) < 1, op, " normalises the last dimension; the input is ", x.sizes());
   if (given(delta))
     refuse(delta->sizes() != x.sizes() || delta->scalar_type() != x.scalar_type() || delta->device() != x.device(), op,
@@ -356,7 +376,7 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const int64_t how = ctx->saved_data["how"].toInt();
     const bool has_w = how & 1, has_b = how & 2, add = how & 8;
-    const Tensor gy = add ? g[1] : g[0], gsum = add ? g[0] : Tensor();
+    const Tensor gy = solid("layer_norm backward", add ? g[1] : g[0]), gsum = solid("layer_norm backward", add ? g[0] : Tensor());
     if (!gy.defined()) return {gsum, add ? gsum : Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     const size_t first = add ? 2 : 1;
@@ -396,7 +416,7 @@ struct RotaryNode : public torch::autograd::Function<RotaryNode> {
     return given(k) ? variable_list{out[0], out[1]} : variable_list{out[0]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const Tensor gq = g[0], gk = g.size() > 1 ? g[1] : Tensor();
+    const Tensor gq = solid("rotary backward", g[0]), gk = g.size() > 1 ? solid("rotary backward", g[1]) : Tensor();
     if (!gq.defined() && !gk.defined()) return variable_list(6);
     const auto saved = ctx->get_saved_variables();
     const bool both = gq.defined() && gk.defined();
@@ -413,6 +433,7 @@ struct RotaryTables {
 
 // The arguments of a rotation as its kernel takes them: tables [positions, R / 2] (or [1, positions, 1, R / 2]) in fp32
 RotaryTables rotary_args(const char* op, const Tensor& q, const OptTensor& k, Tensor cos, Tensor sin, const OptTensor& positions) {
+  plain(op, {&q, opt(k), &cos, &sin, opt(positions)});
   refuse(q.dim() != 4 || (given(k) && k->dim() != 4), op, " needs [batch, tokens, heads, head_dim], got ", q.sizes());
   const int64_t B = q.size(0), T = q.size(1), D = q.size(3);
   if (given(k))
@@ -484,6 +505,7 @@ struct KlTopkNode : public torch::autograd::Function<KlTopkNode> {
       if (!capturing()) ready = at->second.toTensor();
       ctx->saved_data.erase(at);
     }
+    g[0] = solid("kl_topk_logits backward", g[0]);
     const Tensor up = g[0].dim() ? f32_flat(g[0], g[0].numel()) : g[0].to(at::kFloat);
     const Tensor s2 = rows2(saved[0]);
     auto sizes = g[0].sizes().vec();
@@ -496,6 +518,7 @@ struct KlTopkNode : public torch::autograd::Function<KlTopkNode> {
 
 // reduction: 0 mean, 1 sum, 2 none
 Tensor kl_topk(const Tensor& student, const Tensor& values, const Tensor& index, const OptTensor& lse, double tau, int64_t reduction) {
+  plain("kl_topk_logits", {&student, &values, &index, opt(lse)});
   refuse(student.dim() < 1 || student.size(-1) < 1, "kl_topk_logits: student must be [.., V], got ", student.sizes());
   refuse(!(tau >= 1e-20 && tau <= 1e20), "kl_topk_logits: temperature must be from 1e-20 to 1e20, got ", tau);
   refuse((index.scalar_type() != at::kInt && index.scalar_type() != at::kLong) || !values.is_floating_point(),
@@ -542,7 +565,8 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
     return need_aux ? variable_list{out[0], out[1], out[2], out[3]} : variable_list{out[0], out[1], out[2]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
-    const Tensor daux = g.size() > 3 ? g[3] : Tensor();
+    g[0] = solid("route_experts backward", g[0]);
+    const Tensor daux = g.size() > 3 ? solid("route_experts backward", g[3]) : Tensor();
     if (!g[0].defined() && !daux.defined()) return variable_list(11);
     const auto saved = ctx->get_saved_variables();
     const OptTensor dw = g[0].defined() ? OptTensor(g[0].to(at::kFloat).contiguous()) : OptTensor();
@@ -558,6 +582,7 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
 std::tuple<Tensor, Tensor, Tensor, OptTensor> route(const Tensor& logits, const OptTensor& bias, int64_t k, bool softmax, int64_t groups,
                                                     int64_t top_groups, int64_t best, bool renorm, double scale, double aux_coef,
                                                     double z_coef) {
+  plain("route_experts", {&logits, opt(bias)});
   refuse(logits.dim() != 2 || logits.size(1) < 1, "route_experts needs [tokens, experts], got ", logits.sizes());
   OptTensor steer = bias;
   if (given(bias)) {

@@ -78,6 +78,14 @@ def _miss(why: str) -> bool:
     return False
 
 
+_PLAIN = (torch.Tensor, torch.nn.Parameter)
+
+
+def _wrapper(t: torch.Tensor) -> bool:
+    """A subclass that is not the memory it seems to be (DTensor and other wrappers, whose pointer is null)."""
+    return type(t) not in _PLAIN and torch._C._dispatch_keys(t).has(torch._C.DispatchKey.Python)
+
+
 def fast_ok(*tensors) -> bool:
     """Can the CUDA kernels serve these tensors right now? Records the decision in ``stats()``."""
     if _BACKEND == "fallback":
@@ -94,6 +102,8 @@ def fast_ok(*tensors) -> bool:
             return _miss("not cuda")
         if t.dtype not in _DTYPES:
             return _miss(f"dtype {t.dtype}")
+        if _wrapper(t):
+            return _miss(type(t).__name__)
         device = t.get_device()
     if device in _SERVED:
         _COUNTS["fast"] += 1

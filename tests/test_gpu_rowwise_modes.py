@@ -72,3 +72,51 @@ def test_tables_with_tangents_are_refused(which):
         tables[which] = fwd.make_dual(tables[which], torch.ones_like(tables[which]))
         with pytest.raises(ValueError, match="constants"):
             K.rotary(q, *tables)
+
+
+def _negated(t):
+    """``t``'s values as a view that is negated lazily."""
+    view = torch.imag(torch.complex(torch.zeros_like(t), -t).conj())
+    assert view.is_neg() and torch.equal(view, t)
+    return view
+
+
+def test_gradients_that_are_lazily_negated():
+    x, q = randn(6, 64).requires_grad_(), randn(2, 6, 4, 32, seed=5).requires_grad_()
+    tables = K.rotary_tables(6, 32, device="cuda")
+    v, i = randn(6, 64, seed=7).topk(5, dim=-1)
+    outs = [(K.layer_norm(x), x), (K.add_layer_norm(x, x.detach())[1], x), (K.rotary(q, *tables), q),
+            (K.kl_topk_logits(x, v, i, reduction="none"), x), (K.route_experts(x, 4)[0], x)]
+    for n, (y, leaf) in enumerate(outs):
+        up = randn(*y.shape, seed=20 + n)
+        (lazy,) = torch.autograd.grad(y, leaf, _negated(up), retain_graph=True)
+        (want,) = torch.autograd.grad(y, leaf, up)
+        assert torch.allclose(lazy, want, rtol=1e-5, atol=1e-6), n     # (of the loss another kernel's roundings)
+
+
+def test_a_dtensor_takes_the_pytorch_statements(tmp_path):
+    import torch.distributed as dist
+    from torch.distributed.tensor import DTensor, Replicate, init_device_mesh
+    if dist.is_initialized():
+        pytest.skip("a process group is there already")
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path}/store", rank=0, world_size=1)
+    try:
+        mesh = init_device_mesh("cuda", (1,))
+
+        def wrap(t):
+            return DTensor.from_local(t, mesh, [Replicate()], run_check=False)
+        x, w = randn(6, 64), 1 + 0.1 * randn(64, seed=3)
+        K.reset_stats()
+        y = K.layer_norm(wrap(x), wrap(w))
+        z = K.rms_norm(wrap(x), wrap(w))
+        assert K.stats()["fast"] == 0 and K.stats()["fallback"] == 2
+        assert torch.allclose(y.to_local(), K.layer_norm(x, w), rtol=1e-5, atol=1e-5)
+        assert torch.allclose(z.to_local(), K.rms_norm(x, w), rtol=1e-5, atol=1e-5)
+        v, i = randn(6, 64, seed=7).topk(5, dim=-1)
+        q, (cos, sin) = randn(2, 6, 4, 32, seed=5), K.rotary_tables(6, 32, device="cuda")
+        for call in (lambda: K.kl_topk_logits(x, wrap(v), i), lambda: K.kl_topk_logits(x, v, wrap(i)), lambda: K.rotary(q, wrap(cos), sin),
+                     lambda: K.route_experts(x, 4, bias=wrap(w)), lambda: K.kl_topk_distill_loss(x, randn(40, 64), wrap(v), i % 40)):
+            with pytest.raises((TypeError, RuntimeError)):
+                call()
+    finally:
+        dist.destroy_process_group()

@@ -158,3 +158,49 @@ def _rebalance_rank(rank, path):
 
 def test_rebalance_of_several_ranks_needs_a_group(tmp_path):
     torch.multiprocessing.spawn(_rebalance_rank, args=(str(tmp_path / "store"),), nprocs=2)
+
+
+# ------------------------------------------------------------------------------ tensors that are not the memory they seem to be
+def _no_memory():
+    """A wrapper subclass like DTensor, whose pointer is null; a lazily negated view; a sparse tensor."""
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            raise NotImplementedError(str(func))
+    return [Wrapper(torch.ones(3, 8)), torch.imag(torch.ones(3, 8, dtype=torch.complex64).conj()), torch.eye(3, 8).to_sparse()]
+
+
+def test_the_kernels_refuse_tensors_that_are_not_plain_memory():
+    """The extension's own functions, before they look at anything else (so this needs no GPU)."""
+    ext = pytest.importorskip("forgeminds_b200._C")
+    x, v = torch.ones(3, 8), torch.ones(8)
+    q, i = torch.ones(1, 3, 2, 4), torch.zeros(3, 8, dtype=torch.int64)
+    for bad in _no_memory():
+        calls = [lambda: ext.layer_norm(bad, v, v, 1e-5), lambda: ext.layer_norm(x, bad, v, 1e-5), lambda: ext.layer_norm(x, v, bad, 1e-5),
+                 lambda: ext.add_layer_norm(x, bad, None, None, 1e-5), lambda: ext.rotary_one(bad, x, x, None, False),
+                 lambda: ext.rotary_qk(q, bad, x, x, None, False), lambda: ext.rotary_one(q, bad, x, None, False),
+                 lambda: ext.rotary_one(q, x, bad, None, False), lambda: ext.rotary_one(q, x, x, bad, False),
+                 lambda: ext.kl_topk(bad, x, i, None, 1.0, 0), lambda: ext.kl_topk(x, bad, i, None, 1.0, 0),
+                 lambda: ext.kl_topk(x, x, bad, None, 1.0, 0), lambda: ext.kl_topk(x, x, i, bad, 1.0, 0),
+                 lambda: ext.kl_topk_fwd(x, bad, i, None, 1.0, True, True, None, True, False),
+                 lambda: ext.route(bad, None, 2, True, 1, 1, 2, True, 1.0, 0.0, 0.0),
+                 lambda: ext.route(x, bad, 2, True, 1, 1, 2, True, 1.0, 0.0, 0.0)]
+        for call in calls:
+            with pytest.raises(TypeError, match="plain strided"):
+                call()
+    with pytest.raises(TypeError, match="plain strided"):
+        torch.func.vmap(lambda t: ext.layer_norm(t, v, v, 1e-5))(torch.ones(2, 3, 8))
+
+
+def test_wrappers_are_seen_before_a_kernel_is_chosen():
+    from forgeminds_b200.kernels import _state
+
+    class Plain(torch.Tensor):
+        pass
+    wrapper = _no_memory()[0]
+    assert _state._wrapper(wrapper) and not _state._wrapper(torch.ones(2)) and not _state._wrapper(torch.nn.Parameter(torch.ones(2)))
+    assert not _state._wrapper(torch.ones(2).as_subclass(Plain))
