@@ -309,15 +309,17 @@ __global__ void __launch_bounds__(KL_THREADS) kl_topk_kernel(const KlParams p) {
 // from memory once, and the sum of exponentials and the gradient are taken from there. A thread keeps to its own 16-byte
 // vectors, and as soon as the gradient has used one, the same place receives the next row's: loads, exponentials and stores
 // of the SM's CTAs overlap. The sum is one pass: exponentials are taken around a logit that is within 2^8 of the largest so
-// far, and the threads' sums are brought to the row's largest such logit afterwards (with a pass for the maximum before it
-// 204 us where this takes 198). Few threads per row (256, or 128), because the reductions and the row's bookkeeping cost each
+// far, and the threads' sums are brought to the row's largest such logit afterwards (a pass for the maximum before it cost
+// 3 % more). Few threads per row (256, or 128), because the reductions and the row's bookkeeping cost each
 // warp as much as some fifty vectors do. Kept logit k belongs to thread k, whose maximum and sums join the row's own
 // reductions. The CTAs of a row exchange (maximum, sum around it, loss) once. Rows are given out one by one: clusters that
 // find no place at first, while an earlier kernel still holds some SMs, would otherwise be a second wave.
-// Measured, with gradient, bf16: 8192 x 32000 in 198 us (5.3 TB/s of logits and gradient; one block per row that reads it
-// twice: 386), 4096 x 128259 over four CTAs in 456 us (4.6 TB/s; 758): there a row's CTAs wait for one another for a fifth
-// of the time. Both exponentials of a logit together hold the special function unit for 60 % of it, half of the issue slots
-// are used.
+// Measured, with gradient and the count of rows, bf16, one call behind another: 8192 x 32000 in 185 us (5.7 TB/s of logits and
+// gradient; one block per row that reads it twice took twice as long), 4096 x 128259 over four CTAs in 460 us (4.6 TB/s): there
+// a row's CTAs wait for one another for a fifth of the time. Exponents folded into one multiply-add, which is wrong for some
+// rows (see the top), took 181 and 440. Both exponentials of a logit together hold the special function unit for 60 % of the
+// time, half of the issue slots are used.
+
 // m: a logit near the maximum of the CTA's own; s: sum of exponentials around it; over the kept logits that are held here
 // a: sum e (log e - (x - m) / tau), w: sum e, which brings a to the row's m
 struct KlPart {
@@ -687,8 +689,8 @@ int kl_run(KlParams p, bool fwd, int* ws, bool mean, const int* count, cudaStrea
     while (split < 8 && (vectors + split - 1) / split > MOST) split *= 2;
     while (split < 8 && p.rows * split < sm_count() && vectors / split > 4 * KL_ROW_THREADS) split *= 2;
     const int per_cta = (vectors + split - 1) / split;
-    // Many rows of up to 32 KB: half the threads for each and up to six of them at a time. With gradient, bf16: 38910 x 2056
-    // in 177 us against 291 with 256 threads, 9765 x 8192 82 / 102, 4882 x 16384 76 / 81; but 1200 x 12160 30 / 27.
+    // Many rows of up to 32 KB: half the threads for each and up to six of them at a time. With gradient, bf16, 64 kept:
+    // 38910 x 2056 in 166 us against 279 with 256 threads, 9765 x 8192 76 / 98, 4882 x 16384 69 / 76; but 1200 x 12160 26 / 24.
     if (p.rows > 12LL * sm_count() && p.K <= KL_ROW_THREADS / 2 && per_cta <= MOST / 2)
       return kl_row_launch<T, TT, KL_ROW_THREADS / 2>(p, split, per_cta, stream);
     if (p.K <= KL_ROW_THREADS && per_cta <= TOP) return kl_row_launch<T, TT, KL_ROW_THREADS>(p, split, per_cta, stream);

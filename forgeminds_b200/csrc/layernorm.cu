@@ -362,9 +362,10 @@ layernorm_bwd_kernel(const T* __restrict__ dy, long long ldy, const T* __restric
 
 // Rows of more than 1024 chunks: a cluster of blocks shares each, `width` columns (at most 512 chunks) for a block, and
 // exchanges the two sums. The blocks do not wait for one another: between a row's exchange and its result each takes the
-// sums of the next row, so three rows are in the ring, one of them on its way. bf16, no dres: 3024 x 12088 in 79 us (launched
-// while the previous kernel still ran 114; one block per row that reads it twice, and the columns once more, 160), 4096 x
-// 16384 in 113. 8192 x 8192, which 512 threads hold, takes 95 there and 111 on clusters of two.
+// sums of the next row, so three rows are in the ring, one of them on its way. bf16, no dres, with the column sums: 3024 x
+// 12088 in 73 us (launched while the previous kernel still ran half as long again; one block per row that reads it twice, and
+// the columns once more, twice as long), 4096 x 16384 in 110. 8192 x 8192, which 512 threads hold, takes 93 there and a sixth
+// more on clusters of two.
 // A block's sums lie in one of three slots of each peer. A peer writes a slot again three rows later, and by then the reads of
 // the slot are ordered before it: they stand before the __syncthreads of the next row's own sums, and so before the fence and
 // the arrival that warp 0 makes behind that. With two slots only a relaxed arrival of the reading warps stood in between.

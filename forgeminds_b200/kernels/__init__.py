@@ -520,8 +520,11 @@ _KL_MAX_KEEP = 1024          # FMB_KL_MAX_KEEP: more kept logits than this take 
 
 def kl_topk_distill_loss(hs: torch.Tensor, w: torch.Tensor, teacher_values: torch.Tensor, teacher_index: torch.Tensor, *,
                          temperature: float = 1.0, teacher_lse: torch.Tensor | None = None, chunk: int = 4096) -> torch.Tensor:
-    """Mean :func:`kl_topk_logits` of the student logits ``hs @ w.T``, which exist ``chunk`` rows at a time (bf16 ``hs`` on
-    the GPU: as bf16 logits that become their gradient in place, scaled inside the two gradient products)."""
+    """Mean :func:`kl_topk_logits` of the student logits ``hs @ w.T``, which are made ``chunk`` rows at a time. Without
+    gradients no more than that exists of them. In training all rows are held until the backward pass: once, as bf16 logits
+    that become their gradient in place and are scaled inside the two gradient products, for bf16 ``hs`` on the GPU and a head
+    whose two sizes are multiples of 8; otherwise the logits and a gradient of each chunk, which is made again in the
+    backward pass because the mean is taken behind it."""
     if hs.dim() < 1 or w.dim() != 2 or hs.shape[-1] != w.shape[1]:
         raise ValueError(f"kl_topk_distill_loss: hidden states {tuple(hs.shape)} and head {tuple(w.shape)}")
     if chunk < 1:

@@ -99,6 +99,7 @@ def apply_ddp(model, ctx: DistContext):
     """``DistributedDataParallel`` over the flattened data-parallel group; rank-local experts are
     kept out of the reducer when expert parallelism is on. Buffers are not re-broadcast at every
     forward: the only buffers of the models here are RoPE tables, which every rank computes itself, and
+    a router's balance bias, which ``Router.rebalance`` moves alike on every rank of its group; and
     an in-place broadcast would invalidate the graphs of the micro-batches a pipeline schedule keeps
     in flight."""
     from torch.nn.parallel import DistributedDataParallel as DDP
