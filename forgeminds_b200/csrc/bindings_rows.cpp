@@ -79,9 +79,10 @@ void rows_like(const Tensor& t, const Tensor& like, const char* name) {
 }
 
 // ---- LayerNorm
-// x [rows, d] (rows may be apart), w and b [d] or none, delta like x or none: (y, sum or none, stats or none)
+// x [rows, d] (rows may be apart), w and b [d] or none, delta like x or none: (y, sum or none, stats or none). y and sum are made
+// in the shape of the caller's x: a view of them, taken inside an autograd node, could not be changed in place afterwards.
 std::vector<Tensor> layernorm_fwd(const Tensor& x, const OptTensor& delta, const OptTensor& w, const OptTensor& b, double eps,
-                                  bool need_stats) {
+                                  bool need_stats, at::IntArrayRef shape) {
   rows_of(x, "x");
   const int64_t rows = x.size(0), d = x.size(1);
   if (given(delta)) rows_like(*delta, x, "delta");
@@ -90,8 +91,9 @@ std::vector<Tensor> layernorm_fwd(const Tensor& x, const OptTensor& delta, const
   if (given(w)) beside(*w, x, d, wt, "w");
   if (given(b)) beside(*b, x, d, wt, "b");
   c10::cuda::CUDAGuard guard(x.device());
-  Tensor y = at::empty({rows, d}, x.options()), sum, stats;
-  if (given(delta)) sum = at::empty({rows, d}, x.options());
+  Tensor y = at::empty(shape, x.options()), sum, stats;
+  if (given(delta)) sum = at::empty(shape, x.options());
+  TORCH_CHECK(y.numel() == rows * d, "layer_norm: a result of ", shape, " for ", rows, " rows of ", d);
   if (need_stats) stats = at::empty({rows, 2}, x.options().dtype(at::kFloat));
   ok(fmb_layernorm_fwd(x.data_ptr(), pitch(x), ptr(delta), given(delta) ? pitch(*delta) : 0, ptr(w), ptr(b),
                        given(delta) ? sum.data_ptr() : nullptr, y.data_ptr(), need_stats ? stats.data_ptr<float>() : nullptr, rows,
@@ -362,9 +364,8 @@ struct LayerNormNode : public torch::autograd::Function<LayerNormNode> {
     const bool add = given(delta);
     const Tensor x2 = rows2(x.detach());
     auto [wd, bd] = gain(x, w, b);
-    auto out = layernorm_fwd(x2, add ? OptTensor(rows2(delta->detach())) : OptTensor(), wd, bd, eps, true);
-    Tensor y = shaped(out[0], x);
-    Tensor sum = add ? shaped(out[1], x) : Tensor();
+    auto out = layernorm_fwd(x2, add ? OptTensor(rows2(delta->detach())) : OptTensor(), wd, bd, eps, true, x.sizes());
+    const Tensor y = out[0], sum = out[1];
     const Tensor weight = given(wd) ? (given(w) && wd->is_same(*w) ? *w : wd->detach()) : Tensor();
     if (add) ctx->save_for_backward({sum, weight, out[2]});
     else ctx->save_for_backward({x2.is_alias_of(x) && x2.sizes() == x.sizes() ? x : x2, weight, out[2]});
@@ -392,7 +393,7 @@ Tensor layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, doubl
   check_norm("layer_norm", x, OptTensor(), w, b);
   if (wants_grad({&x, opt(w), opt(b)})) return LayerNormNode::apply(x, OptTensor(), w, b, eps)[0];
   auto [wd, bd] = gain(x, w, b);
-  return shaped(layernorm_fwd(rows2(x), OptTensor(), wd, bd, eps, false)[0], x);
+  return layernorm_fwd(rows2(x), OptTensor(), wd, bd, eps, false, x.sizes())[0];
 }
 
 std::tuple<Tensor, Tensor> add_layer_norm(const Tensor& x, const Tensor& delta, const OptTensor& w, const OptTensor& b, double eps) {
@@ -402,8 +403,8 @@ std::tuple<Tensor, Tensor> add_layer_norm(const Tensor& x, const Tensor& delta, 
     return {out[0], out[1]};
   }
   auto [wd, bd] = gain(x, w, b);
-  auto out = layernorm_fwd(rows2(x), rows2(delta), wd, bd, eps, false);
-  return {shaped(out[1], x), shaped(out[0], x)};
+  auto out = layernorm_fwd(rows2(x), rows2(delta), wd, bd, eps, false, x.sizes());
+  return {out[1], out[0]};
 }
 
 struct RotaryNode : public torch::autograd::Function<RotaryNode> {
@@ -495,7 +496,7 @@ struct KlTopkNode : public torch::autograd::Function<KlTopkNode> {
                             reduction == 0 ? out[4] : Tensor()});
     ctx->saved_data["tau"] = tau;
     if (out[3].defined()) ctx->saved_data["ready"] = out[3];
-    return reduction == 2 ? out[1].view(student.sizes().slice(0, student.dim() - 1)) : out[0];
+    return reduction == 2 ? out[1] : out[0];               // (the student is 2-D: one loss per row)
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto saved = ctx->get_saved_variables();

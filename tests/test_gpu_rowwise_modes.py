@@ -120,3 +120,18 @@ def test_a_dtensor_takes_the_pytorch_statements(tmp_path):
                 call()
     finally:
         dist.destroy_process_group()
+
+
+def test_results_can_be_changed_in_place():
+    """As those of ``torch.nn.functional.layer_norm``, which a patched module stands for."""
+    x, w, up = randn(2, 3, 64).requires_grad_(), (1 + 0.1 * randn(64, seed=1)).requires_grad_(), randn(2, 3, 64, seed=2)
+    v, i = randn(2, 3, 64, seed=3).topk(4, dim=-1)
+    zero = torch.zeros_like(x)
+    for n, call in enumerate((lambda: K.layer_norm(x, w), lambda: K.layer_norm(x[0], w), lambda: K.add_layer_norm(x, zero, w)[1],
+                              lambda: K.kl_topk_logits(x, v, i, reduction="none"), lambda: K.kl_topk_logits(x[0], v[0], i[0], reduction="none"),
+                              lambda: K.kl_topk_logits(x[0, 0], v[0, 0], i[0, 0], reduction="none"))):
+        y = call()
+        g = up.flatten()[: y.numel()].view(y.shape)
+        (want,) = torch.autograd.grad(y * 2, x, g)
+        (got,) = torch.autograd.grad(call().mul_(2), x, g)
+        assert torch.equal(got, want), n
