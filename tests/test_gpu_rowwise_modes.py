@@ -135,3 +135,33 @@ def test_results_can_be_changed_in_place():
         (want,) = torch.autograd.grad(y * 2, x, g)
         (got,) = torch.autograd.grad(call().mul_(2), x, g)
         assert torch.equal(got, want), n
+
+
+def _leaf_calls():
+    x, q = randn(6, 64).requires_grad_(), randn(2, 6, 4, 32, seed=5).requires_grad_()
+    v, i = randn(6, 64, seed=7).topk(5, dim=-1)
+    tables = K.rotary_tables(6, 32, device="cuda")
+    return [(lambda a: K.layer_norm(a), x), (lambda a: K.add_layer_norm(a, a)[1], x), (lambda a: K.rotary(a, *tables), q),
+            (lambda a: K.kl_topk_logits(a, v, i, reduction="none"), x), (lambda a: K.route_experts(a, 4, aux_coef=0.1)[0], x)]
+
+
+def test_checkpointed_and_offloaded_activations():
+    from torch.utils.checkpoint import checkpoint
+    for n, (f, leaf) in enumerate(_leaf_calls()):
+        (want,) = torch.autograd.grad(f(leaf).square().sum(), leaf)
+        (again,) = torch.autograd.grad(checkpoint(f, leaf, use_reentrant=False).square().sum(), leaf)
+        with torch.autograd.graph.save_on_cpu():
+            loss = f(leaf).square().sum()
+        (moved,) = torch.autograd.grad(loss, leaf)
+        assert torch.equal(again, want) and torch.equal(moved, want), n
+
+
+def test_transforms_that_wrap_tensors_are_refused():
+    for f, leaf in _leaf_calls():
+        y = f(leaf)
+        with pytest.raises((TypeError, RuntimeError), match="plain strided"):
+            torch.autograd.grad(y, leaf, randn(3, *y.shape), is_grads_batched=True)
+        for call in (lambda: torch.func.grad(lambda a: f(a).sum())(leaf.detach()), lambda: torch.func.vmap(f)(torch.stack([leaf.detach()] * 2)),
+                     lambda: torch.func.jvp(f, (leaf.detach(),), (leaf.detach(),))):
+            with pytest.raises(TypeError, match="plain strided"):
+                call()
